@@ -133,10 +133,9 @@ __device__ __forceinline__ float gelu_fast(float x) {
   return x >= 0.f ? x * (1.0f - 0.5f * q) : x * (0.5f * q);
 }
 
-// gelu_fast on two values with packed fp32 math (v_pk_mul / v_pk_fma / v_pk_add: two lanes'
-// worth of work per instruction; the reciprocal and exp2 stay scalar).  The same IEEE operations
-// in the same order as gelu_fast, so the results are bit-identical to it (1 - 0.5 q: 0.5 q is
-// exact, so the fused and the separate forms round alike).
+// gelu_fast on two values at once (element by element: the build disables packed fp32
+// instructions).  The same IEEE operations in the same order as gelu_fast, so the results are
+// bit-identical to it (1 - 0.5 q: 0.5 q is exact, so the fused and the separate forms round alike).
 typedef __attribute__((ext_vector_type(2))) float f32x2v;
 __device__ __forceinline__ f32x2v gelu_fast2(f32x2v x) {
 #pragma clang fp contract(off)

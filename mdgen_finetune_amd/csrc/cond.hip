@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64) void ipa_attn_kernel(int R, int B, int L, int H
 #pragma unroll
         for (int p = 0; p < PQ + PV; ++p) {
           const int jj = h * (PQ + PV) + p;
-          const float x = kr[okvp + jj], y = kr[okvp + HPkv + jj], z = kr[okvp + 2 * HPkv + jj];
+          const float x = ld1(kr + okvp + jj), y = ld1(kr + okvp + HPkv + jj), z = ld1(kr + okvp + 2 * HPkv + jj);
 #pragma unroll
           for (int a = 0; a < 3; ++a) dst[2 * CH + 3 * p + a] = Rj[a][0] * x + Rj[a][1] * y + Rj[a][2] * z + tj[a];
         }

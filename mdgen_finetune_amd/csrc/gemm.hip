@@ -2844,7 +2844,7 @@ bool mlp_pre_supported(const mdg_gemm_desc& r, const mdg_gemm_desc& f1, const md
 //     (2 x 32 KiB) and b1;
 //   * a P wave keeps its 32 xn rows in registers (the fc1 B operand, loaded once) and computes a
 //     chunk as two 64-hidden halves over two phases each (6 K-steps of 32 per phase); each half's
-//     GELU (packed fp32 math) runs inside the next-but-one phase's K-steps, beside the MFMAs of
+//     GELU runs inside the next-but-one phase's K-steps, beside the MFMAs of
 //     the other half: half A's in phase 2 of the same chunk, half B's in phase 0 of the next.
 //     Q's fc2 steps over H(c - 1) read hidden 0-63 in phases 0-1 of chunk c and 64-127 in
 //     phases 2-3.
