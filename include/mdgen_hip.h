@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define MDG_ABI_VERSION 24
+#define MDG_ABI_VERSION 25
 #define MDG_MAX_LAYERS 16
 #define MDG_SEG_MAX 16 /* segments of one mdg_seg_linear */
 #define MDG_DP 32      /* padded head dim of the attention operand buffers for head_dim <= 31 */
@@ -652,6 +652,111 @@ typedef struct {
 } mdg_train_unpack;
 int mdg_train_pack_layer(const mdg_train_pack* p, void* stream);
 int mdg_train_unpack_layer(const mdg_train_unpack* u, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+   A conditioned block's operators (ABI 25): cross attention to an encoder's states, rotary
+   positions on several axes, and the norms around a block with its gate and residual scale.
+   The reference's MultiheadAttention takes key / value inputs of their own (mha.py:161-264) and
+   its block keeps LN -> branch -> gated residual (latent_model.py:456-493); the denoiser uses the
+   self-attention, single-axis and no-affine forms that the entry points above fuse. */
+
+/* A [B][n][heads][D] tensor: element strides of batch, token and head, the head dim contiguous.
+   A stride may be 0 (an input shared by the batch or the heads); outputs must not overlap. */
+typedef struct {
+  const void* p;
+  int64_t sb, sn, sh;
+} mdg_heads;
+
+enum { MDG_MASK_NONE = 0, MDG_MASK_U8 = 1, MDG_MASK_F32 = 2 };
+
+/* o = softmax(scale q k^T over the keys that are there) v, q / o [B][Nq][H][D], k / v [B][Nk][Hk][D],
+   H % Hk == 0 (query head h reads key head h / (H / Hk)), 1 <= D <= 128, dtype MDG_F32 or MDG_BF16.
+   Key j of sequence b is there when j < kv_len[b] (null: Nk; values are clamped to 0..Nk) and
+   mask[b * mask_sb + j * mask_sn] != 0 (MDG_MASK_U8 bytes or MDG_MASK_F32, null: all); what k / v
+   hold elsewhere, NaN included, is without effect.  A row without keys gives 0; query rows at or past
+   q_len[b] give 0 and their dout is not read.  scale: 1e-18 .. 1e18.
+   lse [B][H][Nq] fp32 (log2 of the row's normaliser in scaled log2 units, -inf without keys) and o_lo
+   (o's rounding residual, as o; bf16) are what the backward reads: null in inference.
+   Backward: dout as o; dq as q, dk / dv as k / v (gradients of keys that are not there are 0);
+   dk and dv both null: dq alone. */
+typedef struct {
+  int32_t dtype, B, Nq, Nk, H, Hk, D, mask_type;
+  float scale;
+  mdg_heads q, k, v, o, o_lo, dout, dq, dk, dv;
+  const int32_t* q_len;
+  const int32_t* kv_len;
+  const void* mask;
+  int64_t mask_sb, mask_sn;
+  float* lse;
+} mdg_attn_cross;
+/* workspace of either pass (backward 0 / 1); 0 bytes may be passed as null.  (size_t)-1: bad shape */
+size_t mdg_attn_cross_workspace_bytes(const mdg_attn_cross* a, int32_t backward);
+int mdg_attn_cross_fwd(const mdg_attn_cross* a, void* ws, size_t ws_bytes, void* stream);
+int mdg_attn_cross_bwd(const mdg_attn_cross* a, void* ws, size_t ws_bytes, void* stream);
+
+/* Rotary positions with several axes.  Pair p < npairs of a head's columns (cols[p], cols[npairs + p])
+   turns by pos[b][n][axis[p]] * turns[p] full turns (turns = frequency / 2 pi, double); columns from
+   2 npairs on pass through.  pairs: MDG_ROPE_HALF (p, p + npairs), MDG_ROPE_INTERLEAVED (2p, 2p + 1),
+   MDG_ROPE_AXIS (halves within each axis's own section; section[a] = that axis's pairs, their sum
+   npairs).  cols, axis and turns are device tables [2 npairs], [npairs], [npairs].  pos: int32 or int64
+   (pos_i64) [B][N][naxes], element strides pos_sb (0: shared) and pos_sn.  nseg 1 or 2 tensors x[i]
+   [B][N][H[i]][D] -> out[i] (may be x[i] itself).  inverse 1: the transposed rotation, the backward. */
+enum { MDG_ROPE_HALF = 0, MDG_ROPE_INTERLEAVED = 1, MDG_ROPE_AXIS = 2 };
+#define MDG_ROPE_MAX_AXES 8
+typedef struct {
+  int32_t dtype, pairs, nseg, B, N, D, npairs, naxes, pos_i64, inverse;
+  int32_t H[2], section[MDG_ROPE_MAX_AXES];
+  const void* pos;
+  int64_t pos_sb, pos_sn;
+  const double* turns;
+  const int32_t* axis;
+  const int32_t* cols;
+  mdg_heads x[2], out[2];
+} mdg_rope_axes_desc;
+int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream);
+
+/* The norms around a block: h_out = resid_scale h + gate u, u = post(y) post_w + post_b;
+   xn = (pre(h_out) pre_w + pre_b) (1 + scale) + shift.  post / pre: MDG_NORM_NONE, _RMS, _LAYER (eps as
+   given).  h [M][ldh], h_out res_dtype; y [M][ldy], xn dtype (y null: h_out = resid_scale h, only the
+   norm before a block); res_dtype fp32, or equal to dtype.  gate / shift / scale fp32 rows
+   m / rows_per_mod of stride mod_stride (null: 1, 0, 0); weights fp32 [C] or null.  1 <= C <= 8192.
+   h_out may be h (ldh == C) or null when pre forms xn; outputs are contiguous rows of C.
+   Backward: dh_out / dxn (either may be null: zero) -> dh, dy, the modulation gradients (rows of
+   stride dmod_stride) and the weights' [C]; each may be null.  It reads h and y, not h_out. */
+enum { MDG_NORM_NONE = 0, MDG_NORM_RMS = 1, MDG_NORM_LAYER = 2 };
+typedef struct {
+  int32_t dtype, res_dtype, M, C, rows_per_mod, post, pre;
+  float resid_scale, eps;
+  const void* h;
+  const void* y;
+  int64_t ldh, ldy;
+  const float* gate;
+  const float* shift;
+  const float* scale;
+  int64_t mod_stride;
+  const float* post_w;
+  const float* post_b;
+  const float* pre_w;
+  const float* pre_b;
+  void* h_out;
+  void* xn;
+  const void* dh_out;
+  const void* dxn;
+  void* dh;
+  void* dy;
+  float* dgate;
+  float* dshift;
+  float* dscale;
+  int64_t dmod_stride;
+  float* dpost_w;
+  float* dpost_b;
+  float* dpre_w;
+  float* dpre_b;
+} mdg_gate_res_norm_desc;
+int mdg_gate_res_norm(const mdg_gate_res_norm_desc* d, void* stream);
+/* workspace of the backward (column-sum partials; 0 without parameter gradients).  (size_t)-1: bad shape */
+size_t mdg_gate_res_norm_bwd_workspace_bytes(const mdg_gate_res_norm_desc* d);
+int mdg_gate_res_norm_bwd(const mdg_gate_res_norm_desc* d, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

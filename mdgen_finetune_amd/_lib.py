@@ -24,6 +24,10 @@ MDG_PREP_TPS, MDG_PREP_NO_OFFSETS, MDG_PREP_COND_FIRST, MDG_PREP_COND_LAST = 1, 
 MDG_MAX_LAYERS = 16
 MDG_SEG_MAX = 16
 MDG_IPA_LOCAL_POINTS, MDG_IPA_RAW_HW = 1, 2
+MDG_MASK_NONE, MDG_MASK_U8, MDG_MASK_F32 = 0, 1, 2
+MDG_ROPE_HALF, MDG_ROPE_INTERLEAVED, MDG_ROPE_AXIS = 0, 1, 2
+MDG_ROPE_MAX_AXES = 8
+MDG_NORM_NONE, MDG_NORM_RMS, MDG_NORM_LAYER = 0, 1, 2
 MDG_DP = 32
 MDG_DP_WIDE = 64
 
@@ -34,7 +38,9 @@ def head_stride(D: int) -> int:
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+SIZE_MAX = ctypes.c_size_t(-1).value  # what the size queries return for a shape that they refuse
 
 
 class MdgDims(ctypes.Structure):
@@ -132,6 +138,31 @@ class MdgAdamTensor(ctypes.Structure):
     _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("step", _vp), ("n", ctypes.c_int64)]
 
 
+class MdgHeads(ctypes.Structure):
+    _fields_ = [("p", _vp), ("sb", _i64), ("sn", _i64), ("sh", _i64)]
+
+
+class MdgAttnCross(ctypes.Structure):
+    _fields_ = ([(n, _i32) for n in ("dtype", "B", "Nq", "Nk", "H", "Hk", "D", "mask_type")] + [("scale", _f32)]
+                + [(n, MdgHeads) for n in ("q", "k", "v", "o", "o_lo", "dout", "dq", "dk", "dv")]
+                + [("q_len", _vp), ("kv_len", _vp), ("mask", _vp), ("mask_sb", _i64), ("mask_sn", _i64), ("lse", _vp)])
+
+
+class MdgRopeAxes(ctypes.Structure):
+    _fields_ = ([(n, _i32) for n in ("dtype", "pairs", "nseg", "B", "N", "D", "npairs", "naxes", "pos_i64", "inverse")]
+                + [("H", _i32 * 2), ("section", _i32 * MDG_ROPE_MAX_AXES), ("pos", _vp), ("pos_sb", _i64), ("pos_sn", _i64),
+                   ("turns", _vp), ("axis", _vp), ("cols", _vp), ("x", MdgHeads * 2), ("out", MdgHeads * 2)])
+
+
+class MdgGateResNorm(ctypes.Structure):
+    _fields_ = ([(n, _i32) for n in ("dtype", "res_dtype", "M", "C", "rows_per_mod", "post", "pre")]
+                + [("resid_scale", _f32), ("eps", _f32), ("h", _vp), ("y", _vp), ("ldh", _i64), ("ldy", _i64)]
+                + [(n, _vp) for n in ("gate", "shift", "scale")] + [("mod_stride", _i64)]
+                + [(n, _vp) for n in ("post_w", "post_b", "pre_w", "pre_b", "h_out", "xn", "dh_out", "dxn", "dh", "dy",
+                                      "dgate", "dshift", "dscale")] + [("dmod_stride", _i64)]
+                + [(n, _vp) for n in ("dpost_w", "dpost_b", "dpre_w", "dpre_b")])
+
+
 # (name, restype, argtypes) of every exported entry point — the test suite checks that the
 # built library exports exactly these and that include/mdgen_hip.h declares them.
 SIGNATURES = [
@@ -203,9 +234,17 @@ SIGNATURES = [
     ("mdg_adam_workspace_bytes", ctypes.c_size_t, [_i32]),
     ("mdg_adam_step", _i32, [_i32, _i32, _vp] + [ctypes.c_double] * 5 + [_i32, ctypes.c_double, _vp, _vp,
                                                                           ctypes.c_size_t, _vp]),
+    # (the descriptors as void*: a ctypes structure by reference, or its packed image as bytes)
+    ("mdg_attn_cross_workspace_bytes", ctypes.c_size_t, [_vp, _i32]),
+    ("mdg_attn_cross_fwd", _i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    ("mdg_attn_cross_bwd", _i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    ("mdg_rope_axes", _i32, [_vp, _vp]),
+    ("mdg_gate_res_norm", _i32, [_vp, _vp]),
+    ("mdg_gate_res_norm_bwd_workspace_bytes", ctypes.c_size_t, [_vp]),
+    ("mdg_gate_res_norm_bwd", _i32, [_vp, _vp, ctypes.c_size_t, _vp]),
 ]
 
-ABI_VERSION = 24
+ABI_VERSION = 25
 _LIB = None
 
 

@@ -1,0 +1,445 @@
+"""A conditioned block's operators on libmdgen_hip.so, forward and backward: cross attention to an
+encoder's states, rotary positions on several axes, and the norms around a block with its gate and
+residual scale.
+
+    q, k = rope_axes(plan, pos, q, k)                      # plan = RopeAxes((pairs per axis, ...))
+    o = cross_attention(q, k, v, mask=mask)                # [B, Nq, H, D] over [B, Nk, Hk, D]
+    h, xn = gate_residual_norm(h, y, gate=gate, post="rms", pre="layer", shift=shift, scale=scale)
+
+The reference's MultiheadAttention takes key and value inputs of their own (mha.py:161-264), rotates
+by one axis (mha.py:356-357) and its block keeps LayerNorm -> branch -> gated residual
+(latent_model.py:456-493).  Here the key side has its own length, heads and mask, a token has a
+position on each of several axes (frame, residue, ...), and the branch is normalised on both sides.
+
+Tensors are fp32 or bf16 on a ROCm device, any strides with a contiguous last dim (other orders are
+copied).  Calls run on the current stream of the tensors' device, allocate only outputs and
+workspaces through torch's caching allocator (so they may be captured into a HIP graph), and are
+differentiable where an input requires grad.  Wrong types and shapes raise TypeError / ValueError
+before any launch; a missing library or a CPU tensor raises RuntimeError (there is no other path).
+"""
+from __future__ import annotations
+
+import functools
+import math
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.MDG_F32, torch.bfloat16: _lib.MDG_BF16}
+_NORMS = {"none": _lib.MDG_NORM_NONE, "rms": _lib.MDG_NORM_RMS, "layer": _lib.MDG_NORM_LAYER}
+_PAIRS = {"half": _lib.MDG_ROPE_HALF, "interleaved": _lib.MDG_ROPE_INTERLEAVED, "axis": _lib.MDG_ROPE_AXIS}
+_MASKS = {torch.bool: _lib.MDG_MASK_U8, torch.uint8: _lib.MDG_MASK_U8, torch.float32: _lib.MDG_MASK_F32}
+
+# The descriptors' images (include/mdgen_hip.h), packed by one call each: filling the ctypes mirrors
+# field by field costs several times a small launch.
+_CROSS = struct.Struct("<8if4x42q")
+_ROPE = struct.Struct("<20i22q")
+_GRN = struct.Struct("<7i2f4x26q")
+_NO_HEADS = (0, 0, 0, 0)
+
+
+def _check_device(t, *others):
+    if not t.is_cuda:
+        raise RuntimeError("mdgen_finetune_amd.cross_hip runs on a ROCm device; got a tensor on " + str(t.device))
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+
+
+class _On:
+    """The tensors' device made current for the launch, where it is not."""
+    __slots__ = ("prev", "idx")
+
+    def __init__(self, t):
+        self.idx = t.device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+        return torch.cuda.current_stream(self.idx).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+
+
+def _unit(t):
+    """The tensor with its last dim contiguous (a copy only where it is not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _heads(t):
+    return (t.data_ptr(), *t.stride()[:3])
+
+
+def _ws(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+# ------------------------------------------------------------------------------------------
+# cross attention
+
+@functools.lru_cache(maxsize=512)
+def _cross_ws_bytes(dtype, B, Nq, Nk, H, Hk, D, backward):
+    n = _lib.load().mdg_attn_cross_workspace_bytes(_CROSS.pack(dtype, B, Nq, Nk, H, Hk, D, 0, 1.0, *([0] * 42)), backward)
+    if n == _lib.SIZE_MAX:
+        _lib.check(1, "mdg_attn_cross_workspace_bytes")
+    return n
+
+
+def _cross_call(backward, q, k, v, o, o_lo, lse, mask, q_len, kv_len, scale, dout=None, dq=None, dk=None, dv=None):
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    dt = _DTYPES[q.dtype]
+    nbytes = _cross_ws_bytes(dt, B, Nq, Nk, H, Hk, D, backward)
+    ws = _ws(nbytes, q.device)
+    grads = (_NO_HEADS * 4 if dout is None else
+             (*_heads(dout), *_heads(dq), *(_heads(dk) if dk is not None else _NO_HEADS),
+              *(_heads(dv) if dv is not None else _NO_HEADS)))
+    desc = _CROSS.pack(dt, B, Nq, Nk, H, Hk, D, 0 if mask is None else _MASKS[mask.dtype], scale,
+                       *_heads(q), *_heads(k), *_heads(v), *_heads(o), *(_heads(o_lo) if o_lo is not None else _NO_HEADS),
+                       *grads, 0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(),
+                       *((0, 0, 0) if mask is None else (mask.data_ptr(), *mask.stride())),
+                       0 if lse is None else lse.data_ptr())
+    lib = _lib.load()
+    with _On(q) as stream:
+        if backward:
+            _lib.check(lib.mdg_attn_cross_bwd(desc, _lib.ptr(ws), nbytes, stream), "mdg_attn_cross_bwd")
+        else:
+            _lib.check(lib.mdg_attn_cross_fwd(desc, _lib.ptr(ws), nbytes, stream), "mdg_attn_cross_fwd")
+
+
+class _CrossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, q_len, kv_len, scale):
+        q, k, v = _unit(q), _unit(k), _unit(v)
+        B, Nq, H, _ = q.shape
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o_lo = torch.empty_like(o) if q.dtype == torch.bfloat16 else None
+        lse = torch.empty(B, H, Nq, device=q.device)
+        if o.numel():
+            _cross_call(0, q, k, v, o, o_lo, lse, mask, q_len, kv_len, scale)
+        ctx.save_for_backward(q, k, v, o, o_lo, lse, mask, q_len, kv_len)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, o, o_lo, lse, mask, q_len, kv_len = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = dv = None
+        if need[1] or need[2]:  # (a frozen encoder leaves the key side's pass out)
+            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        if q.numel():
+            _cross_call(1, q, k, v, o, o_lo, lse, mask, q_len, kv_len, ctx.scale, _unit(dout), dq, dk, dv)
+        elif dk is not None:
+            dk.zero_(), dv.zero_()
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+
+
+def _check_len(name, t, B):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+        raise ValueError(f"cross_attention: {name} must be a contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+
+
+def cross_attention(q, k, v, mask=None, q_len=None, kv_len=None, scale=None):
+    """softmax(scale q k^T) v over the keys that are there: q [B, Nq, H, D], k / v [B, Nk, Hk, D] with
+    H % Hk == 0 (query head h reads key head h // (H / Hk)) and D <= 128; returns [B, Nq, H, D].
+
+    mask [B, Nk] or [1, Nk] (bool, uint8 or fp32; nonzero: the key is there), kv_len / q_len int32 [B]:
+    the sequences' own lengths.  What k and v hold at keys that are not there is without effect (NaN
+    too) and has gradient 0; a row without keys gives 0, and so do query rows past q_len.  scale
+    defaults to D ** -0.5.  Accumulation and the softmax are fp32; with bf16 inputs the probabilities
+    are rounded to bf16 before their product with v."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"cross_attention: {n} must be [B, N, heads, D], got {tuple(t.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"cross_attention: q, k, v must be fp32 or bf16 of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hk == 0 or H % Hk or not 1 <= D <= 128:
+        raise ValueError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    _check_device(q, k, v, mask, q_len, kv_len)
+    if mask is not None:
+        if mask.dtype not in _MASKS or mask.dim() != 2 or mask.shape[1] != Nk or mask.shape[0] not in (1, B):
+            raise ValueError(f"cross_attention: mask must be bool, uint8 or fp32 [{B} or 1, {Nk}], got {mask.dtype} "
+                             f"{tuple(mask.shape)}")
+        mask = mask.expand(B, Nk)
+    _check_len("q_len", q_len, B)
+    _check_len("kv_len", kv_len, B)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-18 <= scale <= 1e18:
+        raise ValueError(f"cross_attention: scale {scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossFn.apply(q, k, v, mask, q_len, kv_len, scale)
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if o.numel():
+        _cross_call(0, q, k, v, o, None, None, mask, q_len, kv_len, scale)
+    return o
+
+
+# ------------------------------------------------------------------------------------------
+# rotary positions with several axes
+
+class RopeAxes:
+    """The rotary plan of a head: sections[a] pairs of columns turn by a token's position on axis a, pair i
+    of an axis with n pairs at frequency base ** (-i / n) (or freq: one frequency per pair, all sections in
+    order).  pairs: "half" couples column p with p + sum(sections), "interleaved" 2p with 2p + 1, "axis"
+    halves within each axis's own section.  Columns past 2 * sum(sections) pass through."""
+
+    def __init__(self, sections, base=10000.0, pairs="half", freq=None, device=None):
+        sections = [int(s) for s in sections]
+        if not 1 <= len(sections) <= _lib.MDG_ROPE_MAX_AXES or min(sections) < 0 or sum(sections) < 1:
+            raise ValueError(f"RopeAxes: sections {sections}")
+        if pairs not in _PAIRS:
+            raise ValueError(f"RopeAxes: pairs {pairs!r} (one of {sorted(_PAIRS)})")
+        n = sum(sections)
+        if freq is None:
+            freq = [float(base) ** (-i / s) for s in sections for i in range(s)]
+        freq = torch.as_tensor(freq, dtype=torch.float64).cpu()
+        if tuple(freq.shape) != (n,):
+            raise ValueError(f"RopeAxes: {n} pairs but freq {tuple(freq.shape)}")
+        first, second, at = [], [], 0
+        for s in sections:
+            first += [at + i for i in range(s)]
+            second += [at + s + i for i in range(s)]
+            at += 2 * s
+        if pairs == "half":
+            first, second = list(range(n)), list(range(n, 2 * n))
+        elif pairs == "interleaved":
+            first, second = list(range(0, 2 * n, 2)), list(range(1, 2 * n, 2))
+        self.sections, self.pairs, self.npairs = sections, pairs, n
+        device = torch.device("cuda" if device is None else device)
+        self.turns = (freq / (2.0 * math.pi)).to(device)
+        self.axis = torch.tensor([a for a, s in enumerate(sections) for _ in range(s)], dtype=torch.int32).to(device)
+        self.cols = torch.tensor(first + second, dtype=torch.int32).to(device)
+        self._head = (n, len(sections))
+        self._sections8 = tuple(sections + [0] * (_lib.MDG_ROPE_MAX_AXES - len(sections)))
+
+
+def _rope_call(plan, pos, xs, outs, inverse):
+    B, N, _, D = xs[0].shape
+    x = [_heads(t) for t in xs] + [_NO_HEADS] * (2 - len(xs))
+    y = [_heads(t) for t in outs] + [_NO_HEADS] * (2 - len(xs))
+    desc = _ROPE.pack(_DTYPES[xs[0].dtype], _PAIRS[plan.pairs], len(xs), B, N, D, *plan._head, pos.dtype == torch.int64,
+                      inverse, xs[0].shape[2], xs[1].shape[2] if len(xs) > 1 else 0, *plan._sections8,
+                      pos.data_ptr(), 0 if pos.shape[0] == 1 else pos.stride(0), pos.stride(1), plan.turns.data_ptr(),
+                      plan.axis.data_ptr(), plan.cols.data_ptr(), *x[0], *x[1], *y[0], *y[1])
+    with _On(xs[0]) as stream:
+        _lib.check(_lib.load().mdg_rope_axes(desc, stream), "mdg_rope_axes")
+
+
+def _rope_new(plan, pos, xs, inverse):
+    xs = [_unit(t) for t in xs]
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+    if xs[0].shape[0] and xs[0].shape[1]:
+        _rope_call(plan, pos, xs, outs, inverse)
+    return outs
+
+
+class _RopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, pos, inverse, *xs):
+        ctx.plan, ctx.inverse = plan, inverse
+        ctx.save_for_backward(pos)
+        return tuple(_rope_new(plan, pos, xs, inverse))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *gs):  # the rotation's transpose is the rotation by the negative angle
+        (pos,) = ctx.saved_tensors
+        return (None, None, None, *_rope_new(ctx.plan, pos, gs, 1 - ctx.inverse))
+
+
+def rope_axes(plan, pos, q, k=None, inverse=False, inplace=False):
+    """q (and k, in the same launch) [B, N, heads, D] rotated by their tokens' positions: pos [N, axes],
+    [1, N, axes] or [B, N, axes], int32 or int64.  Returns q or (q, k).  inverse: by the negative angle.
+    inplace: writes into q and k (no gradient through the call then)."""
+    xs = (q,) if k is None else (q, k)
+    for t in xs:
+        if t.dim() != 4 or t.dtype not in _DTYPES or t.dtype != q.dtype:
+            raise TypeError(f"rope_axes: tensors must be fp32 or bf16 [B, N, heads, D] of one type, got {t.dtype} "
+                            f"{tuple(t.shape)}")
+        if t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3] or not 1 <= t.shape[2] <= 1024:
+            raise ValueError(f"rope_axes: q {tuple(q.shape)}, k {tuple(t.shape)}")
+    B, N, _, D = q.shape
+    if 2 * plan.npairs > D:
+        raise ValueError(f"rope_axes: {plan.npairs} pairs in a head of {D}")
+    _check_device(q, k, pos, plan.turns)
+    if pos.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rope_axes: pos must be int32 or int64, got {pos.dtype}")
+    if pos.dim() == 2:
+        pos = pos[None]
+    if pos.dim() != 3 or pos.shape[0] not in (1, B) or tuple(pos.shape[1:]) != (N, plan._head[1]):
+        raise ValueError(f"rope_axes: pos {tuple(pos.shape)} for tokens [{B}, {N}] on {plan._head[1]} axes")
+    pos = _unit(pos)
+    inverse = int(bool(inverse))
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in xs)
+    if inplace:
+        if grad:
+            raise ValueError("rope_axes: inplace on a tensor that requires grad")
+        for t in xs:
+            if (t.stride(-1) != 1 and D > 1) or any(t.stride(i) == 0 and t.shape[i] > 1 for i in range(3)):
+                raise ValueError("rope_axes: inplace needs a contiguous head dim and no shared memory between tokens or heads")
+        if B and N:
+            _rope_call(plan, pos, xs, xs, inverse)
+        outs = xs
+    else:
+        outs = _RopeFn.apply(plan, pos, inverse, *xs) if grad else _rope_new(plan, pos, xs, inverse)
+    return outs[0] if k is None else tuple(outs)
+
+
+# ------------------------------------------------------------------------------------------
+# the norms around a block, its gate and residual scale
+
+def _rows2d(t, C):
+    t = t.reshape(-1, C)
+    return t if (t.stride(1) == 1 or C == 1) and (t.stride(0) >= C or t.shape[0] == 1) else t.contiguous()
+
+
+def _ld(t, C):
+    return t.stride(0) if t.shape[0] > 1 else C
+
+
+def _same_rows(mods):
+    """gate / shift / scale with one common row stride (copied where they differ)."""
+    have = [t for t in mods if t is not None]
+    if not have:
+        return mods, 0
+    ok = all((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) == have[0].stride(0) >= t.shape[1] for t in have)
+    if not ok:
+        mods = [None if t is None else t.contiguous() for t in mods]
+        have = [t for t in mods if t is not None]
+    return mods, (have[0].stride(0) if have[0].shape[0] > 1 else have[0].shape[1])
+
+
+def _grn_desc(cfg, h, y, mods, mod_stride, ws, out, grads_in=(0, 0), grads=(0,) * 9, dmod_stride=0):
+    M, C = h.shape
+    ptrs = [0 if t is None else t.data_ptr() for t in (*mods, *ws)]
+    return _GRN.pack(_DTYPES[cfg["ct"]], _DTYPES[h.dtype], M, C, cfg["R"], cfg["post"], cfg["pre"], cfg["rs"], cfg["eps"],
+                     h.data_ptr(), 0 if y is None else y.data_ptr(), _ld(h, C), 0 if y is None else _ld(y, C), *ptrs[:3],
+                     mod_stride, *ptrs[3:], *out, *grads_in, *grads[:5], dmod_stride, *grads[5:])
+
+
+def _grn_fwd(cfg, h, y, mods, ws):
+    C = h.shape[-1]
+    h2, y2 = _rows2d(h, C), None if y is None else _rows2d(y, C)
+    mods, ms = _same_rows(mods)
+    ho = None if y is None and cfg["rs"] == 1.0 and cfg["pre"] else torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    xn = torch.empty(h.shape, dtype=cfg["ct"], device=h.device) if cfg["pre"] else None
+    if h.numel():
+        desc = _grn_desc(cfg, h2, y2, mods, ms, ws, (_lib.ptr(ho) or 0, _lib.ptr(xn) or 0))
+        with _On(h) as stream:
+            _lib.check(_lib.load().mdg_gate_res_norm(desc, stream), "mdg_gate_res_norm")
+    return h2, y2, mods, ms, ho, xn
+
+
+class _GrnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, h, y, gate, shift, scale, *ws):
+        h2, y2, mods, ms, ho, xn = _grn_fwd(cfg, h, y, [gate, shift, scale], ws)
+        ctx.save_for_backward(h2, y2, *mods, *ws)
+        ctx.cfg, ctx.ms, ctx.shape = cfg, ms, h.shape
+        ctx.passed = ho is None  # h itself goes on
+        ctx.set_materialize_grads(False)
+        return (h.view_as(h) if ho is None else ho), xn
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dho, dxn):
+        h, y, gate, shift, scale, *ws = ctx.saved_tensors
+        cfg, need = ctx.cfg, ctx.needs_input_grad[1:]
+        if dho is None and dxn is None:
+            return (None,) * (6 + len(ws))
+        C = h.shape[1]
+        dev = h.device
+        dho = None if dho is None else dho.contiguous()
+        dxn = None if dxn is None else dxn.contiguous()
+        dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if need[0] else None
+        dy = torch.empty(ctx.shape, dtype=y.dtype, device=dev) if need[1] else None
+        fresh = torch.empty if h.numel() else torch.zeros  # (no rows: sums of nothing)
+        par = []
+        for i, t in enumerate((gate, shift, scale, *ws)):
+            side = i in (1, 2, 5, 6)  # the pre norm's parameters
+            if t is None or not need[2 + i]:
+                par.append(None)
+            elif side and dxn is None:
+                par.append(torch.zeros(t.shape, device=dev))
+            else:
+                par.append(fresh(t.shape, device=dev))
+        if h.numel():
+            asked = [None if p is None or (i in (1, 2, 5, 6) and dxn is None) else p for i, p in enumerate(par)]
+            grads = [0 if t is None else t.data_ptr() for t in (dh, dy, *asked)]
+            ptr0 = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+            desc = _grn_desc(cfg, h, y, (gate, shift, scale), ctx.ms, ws, (0, 0), (ptr0(dho), ptr0(dxn)), grads, C)
+            lib = _lib.load()
+            nbytes = lib.mdg_gate_res_norm_bwd_workspace_bytes(desc)
+            if nbytes == _lib.SIZE_MAX:
+                _lib.check(1, "mdg_gate_res_norm_bwd_workspace_bytes")
+            wsp = _ws(nbytes, dev)
+            with _On(h) as stream:
+                _lib.check(lib.mdg_gate_res_norm_bwd(desc, _lib.ptr(wsp), nbytes, stream), "mdg_gate_res_norm_bwd")
+        return (None, dh, dy, *par)
+
+
+def gate_residual_norm(h, y=None, gate=None, shift=None, scale=None, resid_scale=1.0, post="none", pre="layer",
+                       post_w=None, post_b=None, pre_w=None, pre_b=None, eps=1e-6):
+    """(h_out, xn) with h_out = resid_scale h + gate u, u = post(y) post_w + post_b, and
+    xn = (pre(h_out) pre_w + pre_b) (1 + scale) + shift: the branch's own norm, its gated way back into the
+    residual stream and the next block's input in one pass.
+
+    h [..., C] fp32 or y's type; y [..., C] fp32 or bf16 (None: only the norm before a block; xn then has
+    h's type); post / pre "none", "rms" or "layer" (pre "none": xn is None).  gate / shift / scale fp32
+    [G, C], one row per run of rows (the rows' count is a multiple of G); weights fp32 [C].  C <= 8192.
+    Statistics and sums are fp32; xn is formed from h_out before its rounding."""
+    if h.dtype not in _DTYPES or h.dim() < 1:
+        raise TypeError(f"gate_residual_norm: h must be fp32 or bf16 [..., C], got {h.dtype} {tuple(h.shape)}")
+    C = h.shape[-1]
+    if not 1 <= C <= 8192:
+        raise ValueError(f"gate_residual_norm: C = {C}")
+    if post not in _NORMS or pre not in _NORMS:
+        raise ValueError(f"gate_residual_norm: post {post!r}, pre {pre!r} (one of {sorted(_NORMS)})")
+    if y is None:
+        if post != "none" or gate is not None:
+            raise ValueError("gate_residual_norm: a post norm or gate without y")
+        if pre == "none":
+            raise ValueError("gate_residual_norm: nothing to do without y and a pre norm")
+    elif y.shape != h.shape or y.dtype not in _DTYPES or h.dtype not in (torch.float32, y.dtype):
+        raise TypeError(f"gate_residual_norm: h {h.dtype} {tuple(h.shape)}, y {y.dtype} {tuple(y.shape)}")
+    if post == "none" and (post_w is not None or post_b is not None):
+        raise ValueError("gate_residual_norm: post weights without a post norm")
+    if pre == "none" and any(t is not None for t in (pre_w, pre_b, shift, scale)):
+        raise ValueError("gate_residual_norm: pre weights or modulation without a pre norm")
+    _check_device(h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
+    M, G = h.numel() // C, None
+    for n, t in (("gate", gate), ("shift", shift), ("scale", scale)):
+        if t is None:
+            continue
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != C or (G is not None and t.shape[0] != G):
+            raise ValueError(f"gate_residual_norm: {n} must be fp32 [G, {C}], got {t.dtype} {tuple(t.shape)}")
+        G = t.shape[0]
+    G = 1 if G is None else G
+    if G < 1 or M % G or (M == 0 and G > 1 and h.shape[0] != G):
+        raise ValueError(f"gate_residual_norm: {M} rows in {G} groups")
+    for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()):
+            raise ValueError(f"gate_residual_norm: {n} must be a contiguous fp32 [{C}], got {t.dtype} {tuple(t.shape)}")
+    eps, rs = float(eps), float(resid_scale)
+    if not (0.0 <= eps < math.inf and math.isfinite(rs)):
+        raise ValueError(f"gate_residual_norm: eps {eps}, resid_scale {rs}")
+    cfg = {"ct": h.dtype if y is None else y.dtype, "R": max(M // G, 1), "post": _NORMS[post], "pre": _NORMS[pre],
+           "rs": rs, "eps": eps}
+    ins = (h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
+        return _GrnFn.apply(cfg, *ins)
+    *_, ho, xn = _grn_fwd(cfg, h, y, [gate, shift, scale], ins[5:])
+    return (h if ho is None else ho), xn

@@ -129,6 +129,15 @@ void adam_table_build(int nt, int nc, const mdg_adam_tensor* t, void* table);
 size_t adam_ws_bytes(int nc);
 hipError_t adam_step_launch(int nt, int nc, const void* table, double lr, double b1, double b2, double eps, double wd,
                             int decoupled, double max_norm, float* gnorm, float* ws, hipStream_t s);
+// attn_cross.hip, rope_axes.hip, gate_res_norm.hip
+size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back);
+bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back);
+hipError_t attn_cross_launch(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s);
+bool rope_axes_grid_ok(const mdg_rope_axes_desc& d);
+hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s);
+size_t gate_res_norm_ws_bytes(const mdg_gate_res_norm_desc& d);
+hipError_t gate_res_norm_fwd_launch(const mdg_gate_res_norm_desc& d, hipStream_t s);
+hipError_t gate_res_norm_bwd_launch(const mdg_gate_res_norm_desc& d, void* ws, hipStream_t s);
 // linear_small.hip
 int seg_total(const mdg_seg_linear* s);
 bool seg_linear_shape_ok(int M, int K);
@@ -1622,6 +1631,151 @@ int mdg_seg_linear_bwd(int32_t M, int32_t K, const float* x, int32_t ldx, int32_
   if (need && (!ws || ws_bytes < need)) return fail(MDG_E_ARG, "seg_linear_bwd: workspace %zu < %zu bytes", ws_bytes, need);
   return hip_check(mdg::seg_linear_bwd_launch(M, K, x, ldx, in_act, s, dx, lddx, (float*)ws, (hipStream_t)stream),
                    "seg_linear_bwd");
+}
+
+// ---------------------------------------------------------------- a conditioned block's operators
+namespace {
+
+// bases and strides in whole elements (the kernels' element loads need no more), strides in range
+int check_heads(const char* who, const char* name, const mdg_heads& t, int e) {
+  if (!t.p) return fail(MDG_E_ARG, "%s: null %s", who, name);
+  if ((uintptr_t)t.p % e) return fail(MDG_E_ARG, "%s: %s is not aligned to its elements", who, name);
+  const int64_t lim = (int64_t)1 << 46;
+  if (t.sb < 0 || t.sn < 0 || t.sh < 0 || t.sb > lim || t.sn > lim || t.sh > lim)
+    return fail(MDG_E_SHAPE, "%s: strides of %s", who, name);
+  return MDG_OK;
+}
+
+int check_attn_cross(const mdg_attn_cross* a, bool back, bool pointers) {
+  const char* who = back ? "attn_cross_bwd" : "attn_cross_fwd";
+  if (!a) return fail(MDG_E_ARG, "%s: null descriptor", who);
+  if (a->dtype != MDG_F32 && a->dtype != MDG_BF16) return fail(MDG_E_DTYPE, "%s: dtype %d", who, a->dtype);
+  if (a->B <= 0 || a->Nq <= 0 || a->Nk < 0 || a->Hk <= 0 || a->H <= 0 || a->H % a->Hk || a->D <= 0 || a->D > 128)
+    return fail(MDG_E_SHAPE, "%s: B=%d Nq=%d Nk=%d H=%d Hk=%d D=%d", who, a->B, a->Nq, a->Nk, a->H, a->Hk, a->D);
+  if (!(a->scale >= 1e-18f && a->scale <= 1e18f)) return fail(MDG_E_ARG, "%s: scale %g", who, (double)a->scale);
+  if (a->mask_type < MDG_MASK_NONE || a->mask_type > MDG_MASK_F32 || (a->mask_type != MDG_MASK_NONE) != (a->mask != nullptr))
+    return fail(MDG_E_ARG, "%s: mask_type %d", who, a->mask_type);
+  if ((double)a->B * a->H * ((double)a->Nq + a->Nk) > 1e15 || !mdg::attn_cross_grid_ok(*a, back)) return fail(MDG_E_SHAPE, "%s: grid too large", who);
+  if (!pointers) return MDG_OK;
+  const int e = a->dtype == MDG_BF16 ? 2 : 4;
+  int rc;
+  if ((rc = check_heads(who, "q", a->q, e)) || (rc = check_heads(who, "o", a->o, e))) return rc;
+  if (a->Nk > 0 && ((rc = check_heads(who, "k", a->k, e)) || (rc = check_heads(who, "v", a->v, e)))) return rc;
+  if (a->o_lo.p && (a->dtype != MDG_BF16 || (rc = check_heads(who, "o_lo", a->o_lo, e))))
+    return fail(MDG_E_ARG, "%s: o_lo is bf16's rounding residual", who);
+  if (back) {
+    if (!a->lse) return fail(MDG_E_ARG, "%s: null lse", who);
+    if ((rc = check_heads(who, "dout", a->dout, e)) || (rc = check_heads(who, "dq", a->dq, e))) return rc;
+    if (!a->dk.p != !a->dv.p) return fail(MDG_E_ARG, "%s: dk and dv come together", who);
+    if (a->dk.p && ((rc = check_heads(who, "dk", a->dk, e)) || (rc = check_heads(who, "dv", a->dv, e)))) return rc;
+  }
+  return MDG_OK;
+}
+
+int check_grn(const mdg_gate_res_norm_desc* d, bool back, bool pointers) {
+  const char* who = back ? "gate_res_norm_bwd" : "gate_res_norm";
+  if (!d) return fail(MDG_E_ARG, "%s: null descriptor", who);
+  if (d->dtype != MDG_F32 && d->dtype != MDG_BF16) return fail(MDG_E_DTYPE, "%s: dtype %d", who, d->dtype);
+  if (d->res_dtype != MDG_F32 && d->res_dtype != d->dtype)
+    return fail(MDG_E_DTYPE, "%s: residual dtype %d with dtype %d", who, d->res_dtype, d->dtype);
+  if (d->M <= 0 || d->C <= 0 || d->C > 8192 || d->rows_per_mod <= 0)
+    return fail(MDG_E_SHAPE, "%s: M=%d C=%d rows_per_mod=%d", who, d->M, d->C, d->rows_per_mod);
+  if (d->post < MDG_NORM_NONE || d->post > MDG_NORM_LAYER || d->pre < MDG_NORM_NONE || d->pre > MDG_NORM_LAYER)
+    return fail(MDG_E_ARG, "%s: post %d pre %d", who, d->post, d->pre);
+  if (!(d->eps >= 0.f) || !std::isfinite(d->eps) || !std::isfinite(d->resid_scale))
+    return fail(MDG_E_ARG, "%s: eps %g resid_scale %g", who, (double)d->eps, (double)d->resid_scale);
+  if (!pointers) return MDG_OK;
+  if (!d->h || d->ldh < d->C) return fail(MDG_E_ARG, "%s: null h or ldh %lld", who, (long long)d->ldh);
+  if (d->y ? d->ldy < d->C : d->post != MDG_NORM_NONE || d->gate || d->dgate || d->dy)
+    return fail(MDG_E_ARG, "%s: a post norm, gate or their gradient without y, or ldy %lld", who, (long long)d->ldy);
+  if (d->post == MDG_NORM_NONE && (d->post_w || d->post_b || d->dpost_w || d->dpost_b))
+    return fail(MDG_E_ARG, "%s: post weights without a post norm", who);
+  if (d->pre == MDG_NORM_NONE && (d->pre_w || d->pre_b || d->shift || d->scale || d->xn || d->dxn || d->dpre_w || d->dpre_b ||
+                                  d->dshift || d->dscale))
+    return fail(MDG_E_ARG, "%s: pre weights, modulation or xn without a pre norm", who);
+  if ((d->gate || d->shift || d->scale) && d->mod_stride < d->C && d->M > d->rows_per_mod)
+    return fail(MDG_E_ARG, "%s: mod_stride %lld", who, (long long)d->mod_stride);
+  const uintptr_t re = d->res_dtype == MDG_BF16 ? 1 : 3, ce = d->dtype == MDG_BF16 ? 1 : 3;
+  if ((((uintptr_t)d->h | (uintptr_t)d->h_out | (uintptr_t)d->dh_out | (uintptr_t)d->dh) & re) ||
+      (((uintptr_t)d->y | (uintptr_t)d->xn | (uintptr_t)d->dxn | (uintptr_t)d->dy) & ce) ||
+      (((uintptr_t)d->gate | (uintptr_t)d->shift | (uintptr_t)d->scale | (uintptr_t)d->post_w | (uintptr_t)d->post_b |
+        (uintptr_t)d->pre_w | (uintptr_t)d->pre_b) & 3))
+    return fail(MDG_E_ARG, "%s: a tensor is not aligned to its elements", who);
+  if (!back) {
+    if (d->pre != MDG_NORM_NONE ? !d->xn : !d->h_out) return fail(MDG_E_ARG, "%s: no output", who);
+    if (d->h_out == d->h && d->ldh != d->C) return fail(MDG_E_ARG, "%s: in place needs contiguous rows", who);
+    return MDG_OK;
+  }
+  if (!d->dh_out && !d->dxn) return fail(MDG_E_ARG, "%s: no incoming gradient", who);
+  if ((d->dshift || d->dscale || d->dpre_w || d->dpre_b) && !d->dxn)
+    return fail(MDG_E_ARG, "%s: pre gradients without dxn", who);
+  if ((d->dgate || d->dshift || d->dscale) && d->dmod_stride < d->C && d->M > d->rows_per_mod)
+    return fail(MDG_E_ARG, "%s: dmod_stride %lld", who, (long long)d->dmod_stride);
+  return MDG_OK;
+}
+
+}  // namespace
+
+size_t mdg_attn_cross_workspace_bytes(const mdg_attn_cross* a, int32_t backward) {
+  return check_attn_cross(a, backward != 0, false) ? (size_t)-1 : mdg::attn_cross_ws_bytes(*a, backward != 0);
+}
+static int attn_cross_call(const mdg_attn_cross* a, bool back, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = check_attn_cross(a, back, true)) return rc;
+  const size_t need = mdg::attn_cross_ws_bytes(*a, back);
+  if (ws_bytes < need || (need && (!ws || (uintptr_t)ws % 16)))
+    return fail(MDG_E_ARG, "attn_cross: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+  return hip_check(mdg::attn_cross_launch(*a, back, ws, (hipStream_t)stream), back ? "attn_cross_bwd" : "attn_cross_fwd");
+}
+int mdg_attn_cross_fwd(const mdg_attn_cross* a, void* ws, size_t ws_bytes, void* stream) {
+  return attn_cross_call(a, false, ws, ws_bytes, stream);
+}
+int mdg_attn_cross_bwd(const mdg_attn_cross* a, void* ws, size_t ws_bytes, void* stream) {
+  return attn_cross_call(a, true, ws, ws_bytes, stream);
+}
+
+int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream) {
+  if (!d) return fail(MDG_E_ARG, "rope_axes: null descriptor");
+  if (d->dtype != MDG_F32 && d->dtype != MDG_BF16) return fail(MDG_E_DTYPE, "rope_axes: dtype %d", d->dtype);
+  if (d->B <= 0 || d->N <= 0 || d->D <= 0 || d->npairs <= 0 || d->npairs > d->D / 2 || d->naxes < 1 ||
+      d->naxes > MDG_ROPE_MAX_AXES || d->nseg < 1 || d->nseg > 2)
+    return fail(MDG_E_SHAPE, "rope_axes: B=%d N=%d D=%d npairs=%d naxes=%d nseg=%d", d->B, d->N, d->D, d->npairs, d->naxes, d->nseg);
+  if ((double)d->B * d->N * d->D > 1e15) return fail(MDG_E_SHAPE, "rope_axes: grid too large");
+  int sum = 0;
+  for (int a = 0; a < d->naxes; ++a) {
+    if (d->section[a] < 0 || d->section[a] > d->npairs) return fail(MDG_E_SHAPE, "rope_axes: section %d", d->section[a]);
+    sum += d->section[a];
+  }
+  if (sum != d->npairs) return fail(MDG_E_SHAPE, "rope_axes: the sections hold %d pairs of %d", sum, d->npairs);
+  if (d->pairs < MDG_ROPE_HALF || d->pairs > MDG_ROPE_AXIS) return fail(MDG_E_ARG, "rope_axes: pairs %d", d->pairs);
+  if (!d->pos || !d->turns || !d->axis || !d->cols) return fail(MDG_E_ARG, "rope_axes: null pos or table");
+  if (((uintptr_t)d->pos & (d->pos_i64 ? 7 : 3)) || ((uintptr_t)d->turns & 7) || (((uintptr_t)d->axis | (uintptr_t)d->cols) & 3))
+    return fail(MDG_E_ARG, "rope_axes: pos or a table is not aligned to its elements");
+  if (d->pos_sb < 0 || d->pos_sn < 0) return fail(MDG_E_SHAPE, "rope_axes: strides of pos");
+  for (int i = 0; i < d->nseg; ++i) {
+    if (d->H[i] <= 0 || d->H[i] > 1024) return fail(MDG_E_SHAPE, "rope_axes: H[%d]=%d", i, d->H[i]);
+    int rc;
+    const int e = d->dtype == MDG_BF16 ? 2 : 4;
+    if ((rc = check_heads("rope_axes", "x", d->x[i], e)) || (rc = check_heads("rope_axes", "out", d->out[i], e))) return rc;
+    if (d->x[i].p == d->out[i].p && (d->x[i].sb != d->out[i].sb || d->x[i].sn != d->out[i].sn || d->x[i].sh != d->out[i].sh))
+      return fail(MDG_E_ARG, "rope_axes: in place needs out's strides equal to x's");
+  }
+  if (!mdg::rope_axes_grid_ok(*d)) return fail(MDG_E_SHAPE, "rope_axes: grid too large");
+  return hip_check(mdg::rope_axes_launch(*d, (hipStream_t)stream), "rope_axes");
+}
+
+int mdg_gate_res_norm(const mdg_gate_res_norm_desc* d, void* stream) {
+  if (const int rc = check_grn(d, false, true)) return rc;
+  return hip_check(mdg::gate_res_norm_fwd_launch(*d, (hipStream_t)stream), "gate_res_norm");
+}
+size_t mdg_gate_res_norm_bwd_workspace_bytes(const mdg_gate_res_norm_desc* d) {
+  return check_grn(d, true, false) ? (size_t)-1 : mdg::gate_res_norm_ws_bytes(*d);
+}
+int mdg_gate_res_norm_bwd(const mdg_gate_res_norm_desc* d, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = check_grn(d, true, true)) return rc;
+  const size_t need = mdg::gate_res_norm_ws_bytes(*d);
+  if (ws_bytes < need || (need && (!ws || (uintptr_t)ws % 16)))
+    return fail(MDG_E_ARG, "gate_res_norm_bwd: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+  return hip_check(mdg::gate_res_norm_bwd_launch(*d, ws, (hipStream_t)stream), "gate_res_norm_bwd");
 }
 
 }  // extern "C"

@@ -1,0 +1,614 @@
+"""The conditioned block's operators on the GPU against plain implementations in 64 bits.
+
+Tolerances (u = half a rounding step relative to the value: bf16 2^-8, fp32 2^-24) are bounds on what
+the kernels round, element by element, from the magnitudes that enter each sum:
+  * an output of type t: u_t |value|;
+  * a sum of n fp32 products: n 2^-24 sum |terms|;
+  * bf16 attention: the probabilities (and dS) are rounded to bf16 before their product, u_bf16 of
+    sum |terms|; delta = do . (o + o_lo) carries o to 2^-16;
+  * scores are fp32 sums of D products: P changes by the factor exp of their error (and of the 2^-22
+    of exp2 and its argument's rounding at the scores met here, below 2^7)."""
+import functools
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32, U16 = 2.0 ** -24, 2.0 ** -8
+
+
+def X():
+    from mdgen_finetune_amd import cross_hip
+
+    return cross_hip
+
+
+def _gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def _near(got, want, tol, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), what
+    if not got.numel():
+        return
+    bad = (got - want).abs() - tol
+    assert bad.max().item() <= 0, (what, (got - want).abs().max().item(), bad.max().item())
+
+
+# ------------------------------------------------------------------------------------------ attention
+def _layout(x, store):
+    """The same values in another layout on the GPU."""
+    if store == "heads":
+        return x.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+    if store == "odd":  # rows that start off any 16-byte boundary
+        B, n, h, d = x.shape
+        buf = torch.full((B, n, h, d + 3), float("nan"), dtype=x.dtype, device="cuda")
+        buf[..., 1:d + 1] = x.cuda()
+        return buf[..., 1:d + 1]
+    if store == "dfirst":  # the head dim is not contiguous: the call copies
+        return x.cuda().permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0)
+    return x.cuda()
+
+
+def _attn_inputs(B, Nq, Nk, H, Hk, D, dt, pad, seed):
+    g = _gen(seed)
+    q, k, v, do = (torch.randn(B, n, h, D, generator=g).to(dt) for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
+    keep = torch.ones(B, Nk, dtype=torch.bool)
+    qkeep = torch.ones(B, Nq, dtype=torch.bool)
+    kw = {}
+    if "len" in pad:
+        ln = torch.randint(0, Nk + 1, (B,), generator=g, dtype=torch.int32)
+        ln[0] = Nk
+        keep &= torch.arange(Nk)[None] < ln[:, None]
+        kw["kv_len"] = ln
+    if "q" in pad:
+        ln = torch.randint(0, Nq + 1, (B,), generator=g, dtype=torch.int32)
+        qkeep &= torch.arange(Nq)[None] < ln[:, None]
+        kw["q_len"] = ln
+    if "mask" in pad:
+        m = torch.rand(B, Nk, generator=g) < 0.6
+        m[-1] = False  # a sequence whose mask leaves nothing
+        keep &= m
+        kw["mask"] = m if "bool" in pad else m.float()
+    # what lies at keys that are not there is garbage of the worst kind
+    if Nk:
+        k[~keep] = float("nan")
+        v[~keep] = float("inf")
+    return q, k, v, do, keep, qkeep, kw
+
+
+def _attn_oracle(q, k, v, do, keep, qkeep, scale, dt):
+    """o, dq, dk, dv and their tolerances, float64 on the CPU."""
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    G = H // Hk
+    z = lambda t: torch.where(keep[:, :, None, None], t.double(), 0.0)  # noqa: E731
+    qh = torch.where(qkeep[:, :, None, None], q.double(), 0.0).transpose(1, 2)
+    gh = torch.where(qkeep[:, :, None, None], do.double(), 0.0).transpose(1, 2)
+    kh, vh = (z(t).transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+    s = scale * (qh @ kh.transpose(-1, -2))
+    live = (keep[:, None, None, :] & qkeep[:, None, :, None]).expand(B, H, Nq, Nk)
+    s = s.masked_fill(~live, -math.inf)
+    m = s.amax(-1, keepdim=True) if Nk else torch.zeros(B, H, Nq, 1, dtype=torch.float64)
+    p = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
+    l = p.sum(-1, keepdim=True)
+    p = p / torch.where(l == 0, 1.0, l)
+    o = p @ vh
+    uo = U16 if dt == torch.bfloat16 else U32
+    up = U16 if dt == torch.bfloat16 else 0.0
+    # relative error of P: the scores' fp32 sums, exp2 and the normaliser's sum of Nk terms
+    smag = scale * (qh.abs() @ kh.abs().transpose(-1, -2))
+    ep = 2 * ((D + 4) * U32 * (smag.amax(-1, keepdim=True) if Nk else 0.0) + (Nk + 16) * U32 + 2.0 ** -20)
+    av = p @ vh.abs()
+    t_o = uo * o.abs() + (up + ep + (Nk + 8) * U32) * av
+    dv = p.transpose(-1, -2) @ gh
+    dvm = p.transpose(-1, -2) @ gh.abs()
+    t_dv = uo * dv.abs() + ((up + Nq * U32) * dvm + (p * ep).transpose(-1, -2) @ gh.abs())
+    dp = gh @ vh.transpose(-1, -2)
+    delta = (gh * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    # error of dS: P's, the fp32 sums of dp and delta, and o + o_lo (2^-16 of the rounded o, with its own P's error)
+    dpm = gh.abs() @ vh.abs().transpose(-1, -2)
+    dm = (gh.abs() * o.abs()).sum(-1, keepdim=True)
+    e_o = (gh.abs() * ((2.0 ** -16 if up else U32) * o.abs() + (up + ep + (Nk + 8) * U32) * av)).sum(-1, keepdim=True)
+    e_ds = up * ds.abs() + ep * ds.abs() + p * ((D + 4) * U32 * (dpm + dm) + e_o)
+    dq, t_dq = scale * (ds @ kh), scale * ((e_ds + Nk * U32 * ds.abs()) @ kh.abs())
+    dk = scale * (ds.transpose(-1, -2) @ qh)
+    t_dk = scale * ((e_ds + Nq * G * U32 * ds.abs()).transpose(-1, -2) @ qh.abs())
+    fold = lambda t: t.reshape(B, Hk, G, Nk, D).sum(2).transpose(1, 2)  # noqa: E731
+    dk, t_dk, dv, t_dv = fold(dk), fold(t_dk), fold(dv), fold(t_dv)
+    dq, t_dq, o, t_o = (t.transpose(1, 2) for t in (dq, t_dq, o, t_o))
+    tiny = 1e-30
+    return (o, dq, dk, dv), (t_o + tiny, t_dq + uo * dq.abs() + tiny, t_dk + uo * dk.abs() + tiny, t_dv + tiny)
+
+
+ATTN = [  # B, Nq, Nk, H, Hk, D, padding, layout
+    (1, 1, 1, 1, 1, 1, "", "tokens"),
+    (2, 1, 7, 4, 4, 24, "len", "tokens"),
+    (2, 1, 300, 8, 2, 128, "len", "heads"),
+    (3, 5, 33, 4, 2, 20, "mask", "odd"),
+    (2, 8, 64, 4, 1, 32, "q", "tokens"),        # exactly 32 packed rows
+    (2, 33, 65, 3, 3, 33, "mask bool", "dfirst"),
+    (1, 130, 31, 2, 1, 48, "len q", "heads"),
+    (2, 64, 129, 6, 3, 64, "mask len q", "tokens"),
+    (1, 257, 200, 2, 2, 96, "", "odd"),
+    (1, 40, 700, 2, 1, 128, "len", "tokens"),
+    (4, 3, 5, 2, 2, 16, "len mask q", "tokens"),
+    (1, 2, 0, 2, 1, 8, "", "tokens"),           # an encoder without states
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(str(x) for x in c))
+def test_cross_attention_forward_backward(case, dt):
+    B, Nq, Nk, H, Hk, D, pad, store = case
+    q, k, v, do, keep, qkeep, kw = _attn_inputs(B, Nq, Nk, H, Hk, D, dt, pad, 11)
+    scale = 0.7 * D ** -0.5
+    want, tol = _attn_oracle(q, k, v, do, keep, qkeep, scale, dt)
+    kw = {n: t.cuda() for n, t in kw.items()}
+    qc, kc, vc = (_layout(t, store) for t in (q, k, v))
+    with torch.no_grad():
+        _near(X().cross_attention(qc, kc, vc, scale=scale, **kw), want[0], tol[0], "o (inference)")
+    leaves = [t.detach().requires_grad_(True) for t in (qc, kc, vc)]
+    o = X().cross_attention(*leaves, scale=scale, **kw)
+    dout = do.cuda()
+    dout[~qkeep.cuda()] = float("nan")  # (not read)
+    grads = torch.autograd.grad(o, leaves, dout)
+    for n, got, w, t in zip(("o", "dq", "dk", "dv"), (o, *grads), want, tol):
+        _near(got, w, t, n)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("Nq,Nk,G", [(1, 5000, 4), (2, 20000, 1), (45, 6000, 1)])
+def test_cross_attention_splits_a_long_key_axis(Nq, Nk, G, dt):
+    """Few rows over many keys: the splits' partial softmaxes joined, ragged lengths (0 and 1 among them)."""
+    B, Hk, D = 3, 2, 40
+    q, k, v, do, keep, qkeep, _ = _attn_inputs(B, Nq, Nk, Hk * G, Hk, D, dt, "", 5)
+    ln = torch.tensor([Nk - 3, 0, 1], dtype=torch.int32)
+    keep = torch.arange(Nk)[None] < ln[:, None]
+    want, tol = _attn_oracle(q, k, v, do, keep, qkeep, D ** -0.5, dt)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = X().cross_attention(*leaves, kv_len=ln.cuda())
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    for n, got, w, t in zip(("o", "dq", "dk", "dv"), (o, *grads), want, tol):
+        _near(got, w, t, n)
+    with torch.no_grad():
+        assert torch.equal(X().cross_attention(*leaves, kv_len=ln.cuda()), o)
+
+
+def test_cross_attention_broadcast_inputs_and_frozen_encoder():
+    """k / v shared by the batch (stride 0): their gradient is the batch's sum; a frozen encoder gets none and
+    dq is the same bits."""
+    B, Nq, Nk, H, D = 3, 37, 50, 2, 24
+    q, k, v, do, *_ = _attn_inputs(B, Nq, Nk, H, H, D, torch.float32, "", 3)
+    k1, v1 = k[:1], v[:1]
+    ke, ve = k1.expand(B, -1, -1, -1), v1.expand(B, -1, -1, -1)
+    ones = torch.ones(B, Nk, dtype=torch.bool)
+    want, tol = _attn_oracle(q, ke, ve, do, ones, torch.ones(B, Nq, dtype=torch.bool), D ** -0.5, torch.float32)
+    ql, kl, vl = (t.cuda().requires_grad_(True) for t in (q, k1, v1))
+    o = X().cross_attention(ql, kl.expand(B, -1, -1, -1), vl.expand(B, -1, -1, -1))
+    dq, dk, dv = torch.autograd.grad(o, (ql, kl, vl), do.cuda())
+    _near(o, want[0], tol[0], "o")
+    _near(dk, want[2].sum(0, keepdim=True), tol[2].sum(0, keepdim=True) + 4 * U32 * want[2].abs().sum(0), "dk")
+    _near(dv, want[3].sum(0, keepdim=True), tol[3].sum(0, keepdim=True) + 4 * U32 * want[3].abs().sum(0), "dv")
+    of = X().cross_attention(ql, kl.detach().expand(B, -1, -1, -1), vl.detach().expand(B, -1, -1, -1))
+    (dqf,) = torch.autograd.grad(of, ql, do.cuda())
+    assert torch.equal(dqf, dq)
+    # a gradient that arrives expanded (as of a sum) and one in another order
+    (ds,) = torch.autograd.grad(X().cross_attention(ql, kl.detach().expand(B, -1, -1, -1), vl.detach().expand(B, -1, -1, -1)).sum(), ql)
+    assert torch.isfinite(ds).all()
+
+
+def test_cross_attention_gradient_against_differences():
+    B, Nq, Nk, H, D = 1, 3, 6, 2, 8
+    q, k, v, do, *_ = _attn_inputs(B, Nq, Nk, H, 1, D, torch.float32, "", 9)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(X().cross_attention(*leaves), leaves, do.cuda())
+    f = lambda xs: (X().cross_attention(*xs).double() * do.cuda().double()).sum().item()  # noqa: E731
+    eps = 2.0 ** -6
+    with torch.no_grad():
+        for which, at in ((0, (0, 1, 1, 3)), (1, (0, 4, 0, 2)), (2, (0, 2, 0, 7))):
+            hi, lo = ([t.detach().clone() for t in leaves] for _ in range(2))
+            hi[which][at] += eps
+            lo[which][at] -= eps
+            num = (f(hi) - f(lo)) / (2 * eps)
+            # the difference's own error: eps^2 / 6 of a third derivative below 8, and 48 fp32 outputs' rounding over 2 eps
+            assert abs(num - grads[which][at].item()) < eps * eps / 6 * 8 + 48 * 8 * U32 * 4 / eps
+
+
+def test_cross_attention_large_scores_and_ties():
+    """Scores far above and below zero (a raised maximum in later tiles), and equal scores."""
+    B, Nq, Nk, D = 1, 40, 300, 16
+    q = torch.ones(B, Nq, 1, D)
+    k = torch.zeros(B, Nk, 1, D)
+    k[0, :, 0, 0] = torch.linspace(-300, 300, Nk).round()
+    v = torch.randn(B, Nk, 1, D, generator=_gen(0))
+    one = torch.ones(B, Nk, dtype=torch.bool)
+    for dt in (torch.float32, torch.bfloat16):
+        args = [t.to(dt) for t in (q, k, v)]
+        want, tol = _attn_oracle(*args, args[0], one, torch.ones(B, Nq, dtype=torch.bool), 1.0, dt)
+        # exponents up to 600 * log2 e < 2^10: the argument of exp2 is rounded by 2^-14
+        _near(X().cross_attention(*(t.cuda() for t in args), scale=1.0), want[0], tol[0] + 2.0 ** -13 * 4, "o")
+        z = torch.zeros_like(args[1])
+        w2, t2 = _attn_oracle(args[0], z, args[2], args[0], one, torch.ones(B, Nq, dtype=torch.bool), 1.0, dt)
+        _near(X().cross_attention(args[0].cuda(), z.cuda(), args[2].cuda(), scale=1.0), w2[0], t2[0], "ties")
+    # a NaN among the keys that are there stays one
+    k[0, 7] = float("nan")
+    assert torch.isnan(X().cross_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)).all()
+    assert torch.isnan(X().cross_attention(q[:, :1].cuda(), k.cuda(), v.cuda(), scale=1.0)).all()
+
+
+def test_cross_attention_offsets_past_32_bits():
+    """A single token over a cache whose last keys lie past 2^31 elements, and lengths clamped to the cache."""
+    B, Nk, H, D = 1, 140000, 130, 128  # 2.3e9 elements each of k and v in bf16
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GiB")
+    kv = torch.zeros(Nk, H, D, dtype=torch.bfloat16, device="cuda")[None]
+    q = torch.ones(B, 1, H, D, dtype=torch.bfloat16, device="cuda")
+    kv[0, -1] = 4.0  # score 4 * 128 / sqrt(128) above the rest: the last key takes the whole softmax
+    o = X().cross_attention(q, kv, kv, kv_len=torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"))
+    assert (o - 4.0).abs().max().item() <= 4 * U16
+    o = X().cross_attention(q, kv, kv, kv_len=torch.tensor([Nk - 1], dtype=torch.int32, device="cuda"))
+    assert o.abs().max().item() == 0
+    o = X().cross_attention(q, kv, kv, kv_len=torch.tensor([-5], dtype=torch.int32, device="cuda"))
+    assert o.abs().max().item() == 0
+
+
+# ------------------------------------------------------------------------------------------ rotary
+def _rope_oracle(x, pos, sections, pairs, base, sign):
+    cols = X().RopeAxes(sections, pairs=pairs, device="cpu").cols.long()
+    n = sum(sections)
+    axis = torch.cat([torch.full((s,), a) for a, s in enumerate(sections)]).long()
+    freq = torch.tensor([base ** (-i / s) for s in sections for i in range(s)], dtype=torch.float64)
+    ang = (pos.double()[..., axis] * freq)[:, :, None]
+    out = x.double().clone()
+    a, b = x.double()[..., cols[:n]], x.double()[..., cols[n:]]
+    out[..., cols[:n]] = a * ang.cos() - sign * b * ang.sin()
+    out[..., cols[n:]] = b * ang.cos() + sign * a * ang.sin()
+    mag = out.abs().clone()
+    mag[..., cols[:n]] = mag[..., cols[n:]] = a.abs() + b.abs()
+    return out, mag
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("pairs", ["half", "interleaved", "axis"])
+@pytest.mark.parametrize("B,N,H,Hk,D,sections,store", [
+    (1, 1, 1, 1, 2, [1], "tokens"), (2, 5, 4, 2, 24, [6, 6], "tokens"), (3, 7, 2, 1, 64, [8, 8, 16], "heads"),
+    (2, 9, 3, 3, 33, [3, 5, 0, 7], "odd"), (1, 300, 12, 4, 128, [16, 24, 24], "tokens"), (2, 4, 40, 8, 48, [16], "dfirst"),
+    (1, 6001, 8, 8, 64, [16, 16], "tokens"),
+])
+def test_rope_axes_forward_backward(B, N, H, Hk, D, sections, store, pairs, dt):
+    g = _gen(2)
+    q, k, gq, gk = (torch.randn(B, N, h, D, generator=g).to(dt) for h in (H, Hk, H, Hk))
+    pos = torch.randint(-1000, 1_000_000, (B, N, len(sections)), generator=g)
+    plan = X().RopeAxes(sections, pairs=pairs, device="cuda")
+    u = U16 if dt == torch.bfloat16 else U32
+    # per output: its rounding, two fp32 products and their sum, and 2^-22 of cos / sin (the reduced angle in fp32)
+    lim = lambda o, m: u * o.abs() + (4 * U32 + 2.0 ** -22) * m + 1e-30  # noqa: E731
+    ql, kl = (_layout(t, store).detach().requires_grad_(True) for t in (q, k))
+    for p in (pos.to(torch.int32).cuda(), pos.cuda()):
+        qo, ko = X().rope_axes(plan, p, ql, kl)
+        for got, x in ((qo, q), (ko, k)):
+            w, m = _rope_oracle(x, pos, sections, pairs, 10000.0, 1.0)
+            _near(got, w, lim(w, m), "rotated")
+    dq, dk = torch.autograd.grad((qo, ko), (ql, kl), (gq.cuda(), gk.cuda()))
+    for got, x in ((dq, gq), (dk, gk)):
+        w, m = _rope_oracle(x, pos, sections, pairs, 10000.0, -1.0)
+        _near(got, w, lim(w, m), "gradient")
+    with torch.no_grad():  # one tensor, the inverse, in place, shared positions
+        one = X().rope_axes(plan, pos.cuda(), ql)
+        assert torch.equal(one, qo)
+        back = X().rope_axes(plan, pos.cuda(), gq.cuda(), inverse=True)
+        assert torch.equal(back, dq)
+        if store != "dfirst":
+            buf = _layout(q, store).clone(memory_format=torch.preserve_format)
+            kb = _layout(k, "tokens").clone()
+            r = X().rope_axes(plan, pos.cuda(), buf, kb, inplace=True)
+            assert r[0] is buf and torch.equal(buf, qo) and torch.equal(kb, ko)
+        sh = X().rope_axes(plan, pos[:1].cuda(), ql)
+        w, m = _rope_oracle(q, pos[:1].expand(B, -1, -1), sections, pairs, 10000.0, 1.0)
+        _near(sh, w, lim(w, m), "shared positions")
+
+
+def test_rope_axes_inplace_refusals():
+    plan = X().RopeAxes([4], device="cuda")
+    x = torch.zeros(1, 3, 2, 8, device="cuda")
+    pos = torch.zeros(3, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        X().rope_axes(plan, pos, x.requires_grad_(True), inplace=True)
+    with pytest.raises(ValueError):
+        X().rope_axes(plan, pos, x.detach()[:, :1].expand(1, 3, 2, 8), inplace=True)
+    with pytest.raises(TypeError):
+        X().rope_axes(plan, pos.float(), x.detach())
+    with pytest.raises(ValueError):
+        X().rope_axes(plan, pos[:2], x.detach())
+    with pytest.raises(ValueError):
+        X().rope_axes(plan, pos.cpu(), x.detach())
+    assert X().rope_axes(plan, pos[:0], x.detach()[:, :0]).shape == (1, 0, 2, 8)
+
+
+# ------------------------------------------------------------------------------------------ norms
+def _grn_oracle(t, G, post, pre, rs, eps, gh, gx):
+    """float64 autograd from the definition: outputs, gradients by name."""
+    leaf = {n: (None if x is None else x.double().requires_grad_(True)) for n, x in t.items()}
+    C = t["h"].shape[-1]
+    h, y = leaf["h"].reshape(G, -1, C), None if leaf["y"] is None else leaf["y"].reshape(G, -1, C)
+
+    def norm(x, kind, w, b):
+        if kind == "layer":
+            x = x - x.mean(-1, keepdim=True)
+        if kind != "none":
+            x = x / torch.sqrt((x ** 2).mean(-1, keepdim=True) + eps)
+        x = x if w is None else x * w
+        return x if b is None else x + b
+
+    row = lambda n: leaf[n][:, None]  # noqa: E731
+    ho = rs * h
+    if y is not None:
+        u = norm(y, post, leaf["post_w"], leaf["post_b"])
+        ho = ho + (u if leaf["gate"] is None else row("gate") * u)
+    outs, gs = [ho], [gh.double().reshape(G, -1, C)]
+    if pre != "none":
+        z = norm(ho, pre, leaf["pre_w"], leaf["pre_b"])
+        z = z if leaf["scale"] is None else z * (1 + row("scale"))
+        outs.append(z if leaf["shift"] is None else z + row("shift"))
+        gs.append(gx.double().reshape(G, -1, C))
+    names = [n for n, x in leaf.items() if x is not None]
+    grads = torch.autograd.grad(outs, [leaf[n] for n in names], gs, allow_unused=True)
+    return [o.detach().reshape(t["h"].shape) for o in outs], dict(zip(names, grads))
+
+
+GRN = [  # G, rows, C, post, pre, gate/mod/affine, type of h
+    (1, 1, 1, "none", "rms", "", "f32"),
+    (4, 1, 384, "rms", "layer", "gate mod", "f32"),
+    (2, 33, 64, "layer", "rms", "gate mod affine", "same"),
+    (3, 70, 24, "rms", "none", "gate", "f32"),
+    (2, 5, 129, "layer", "layer", "gate mod affine", "f32"),
+    (1, 9, 3001, "rms", "layer", "affine", "same"),
+    (5, 40, 1000, "rms", "rms", "mod", "same"),
+    (2, 3, 4096, "layer", "rms", "gate mod affine", "same"),
+    (1, 2, 8192, "none", "layer", "gate mod affine", "f32"),
+    (1, 300, 512, "layer", "layer", "", "f32"),
+    (1, 4, 2050, "rms", "rms", "gate mod affine", "same"),
+    (7, 1, 200, "noy", "layer", "mod affine", "same"),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", GRN, ids=lambda c: "-".join(str(x) for x in c))
+def test_gate_residual_norm_forward_backward(case, dt):
+    G, rows, C, post, pre, opts, res = case
+    rdt = torch.float32 if res == "f32" else dt
+    g = _gen(4)
+    rs, eps = 0.75, 1e-5
+    rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    noy = post == "noy"
+    post = "none" if noy else post
+    t = {"h": (2 * rnd(G, rows, C) + 0.5).to(rdt), "y": None if noy else (rnd(G, rows, C) - 0.2).to(dt)}
+    t["gate"] = rnd(G, C) if "gate" in opts else None
+    t["shift"], t["scale"] = (0.3 * rnd(G, C) if "mod" in opts else None for _ in range(2))
+    t["post_w"] = 1 + 0.2 * rnd(C) if "affine" in opts and post != "none" else None
+    t["post_b"] = 0.2 * rnd(C) if "affine" in opts and post == "layer" else None
+    t["pre_w"] = 1 + 0.2 * rnd(C) if "affine" in opts else None
+    t["pre_b"] = 0.2 * rnd(C) if "affine" in opts and pre == "layer" else None
+    xdt = rdt if noy else dt
+    gh, gx = rnd(G, rows, C).to(rdt), rnd(G, rows, C).to(xdt)
+    outs, grads = _grn_oracle(t, G, post, pre, rs, eps, gh, gx)
+    dev = {n: (None if x is None else x.cuda().requires_grad_(True)) for n, x in t.items()}
+    kw = {n: x for n, x in dev.items() if n not in ("h", "y")}
+    ho, xn = X().gate_residual_norm(dev["h"], dev["y"], resid_scale=rs, post=post, pre=pre, eps=eps, **kw)
+    got_o = [ho] if xn is None else [ho, xn]
+    names = [n for n, x in dev.items() if x is not None]
+    got_g = torch.autograd.grad(got_o, [dev[n] for n in names], [gh.cuda(), gx.cuda()][:len(got_o)])
+    u = lambda d: U16 if d == torch.bfloat16 else U32  # noqa: E731
+    # fp32 rows: sums of C terms (mean, variance) scale every value of the row, a few products follow; the
+    # magnitudes of the terms are bounded by the row's own largest ones
+    f32 = (C + 64) * U32
+    for n, o, w in zip(("h_out", "xn"), got_o, outs):
+        _near(o, w, u(o.dtype) * w.abs() + f32 * (4 + w.abs().amax(-1, keepdim=True)), n)
+    M = G * rows
+    for n, o in zip(names, got_g):
+        w = grads[n]
+        if n in ("h", "y"):
+            # C = 1 rows and rows of tiny variance: gradients of a norm scale with 1 / std
+            big = w.abs().amax(-1, keepdim=True) + 4
+            _near(o, w, u(o.dtype) * w.abs() + 4 * f32 * big, n)
+        else:  # column sums over the rows: terms up to 5 * 5 in magnitude, M of them, fp32
+            k = M if n in ("post_w", "post_b", "pre_w", "pre_b") else rows
+            _near(o, w, (k + C + 64) * U32 * 16 * math.sqrt(k) * 4, n)
+    with torch.no_grad():
+        h2, x2 = X().gate_residual_norm(dev["h"], dev["y"], resid_scale=rs, post=post, pre=pre, eps=eps, **kw)
+        assert torch.equal(h2, ho) and (xn is None or torch.equal(x2, xn))
+
+
+def test_gate_residual_norm_strided_rows_and_partial_gradients():
+    """h and y as column slices of wider rows, adaLN rows as chunks of one projection; gradients of some inputs only,
+    and of one output only."""
+    g = _gen(8)
+    G, R, C = 3, 11, 96
+    wide = torch.randn(G, R, 3 * C, generator=g).cuda()
+    mods = torch.randn(G, 3 * C, generator=g).cuda().requires_grad_(True)
+    h, y = wide[..., C:2 * C], wide[..., 2 * C:]
+    gate, shift, scale = mods.split(C, -1)
+    ho, xn = X().gate_residual_norm(h, y, gate=gate, shift=shift, scale=scale, post="rms")
+    hc, xc = X().gate_residual_norm(h.contiguous(), y.contiguous(), gate=gate.contiguous(), shift=shift.contiguous(),
+                                    scale=scale.contiguous(), post="rms")
+    assert torch.equal(ho, hc) and torch.equal(xn, xc)
+    (d1,) = torch.autograd.grad(xn.sum() + (ho * 2).sum(), mods, retain_graph=True)
+    (d2,) = torch.autograd.grad(xc.sum() + (hc * 2).sum(), mods)
+    assert torch.equal(d1, d2)
+    (dh_only,) = torch.autograd.grad(ho.sum(), mods, retain_graph=True)
+    assert dh_only[:, C:].abs().max().item() == 0 and dh_only[:, :C].abs().max().item() > 0
+    hl = h.detach().clone().requires_grad_(True)
+    _, x1 = X().gate_residual_norm(hl, pre="rms")
+    (gr,) = torch.autograd.grad(x1, hl, torch.ones_like(x1))
+    h64 = hl.detach().double().cpu().requires_grad_(True)
+    w = h64 / torch.sqrt((h64 ** 2).mean(-1, keepdim=True) + 1e-6)
+    (wg,) = torch.autograd.grad(w.sum(), h64)
+    _near(gr, wg, 4 * (C + 64) * U32 * (wg.abs().amax(-1, keepdim=True) + 4), "dh of a pre norm alone")
+
+
+def test_gate_residual_norm_empty_and_constant_rows():
+    e = torch.zeros(2, 0, 16, device="cuda", requires_grad=True)
+    ho, xn = X().gate_residual_norm(e, e.detach(), gate=torch.zeros(2, 16, device="cuda"))
+    assert ho.shape == xn.shape == (2, 0, 16)
+    c = torch.full((3, 48), 7.0, device="cuda")  # a layer norm of equal values: zeros, eps in the root
+    _, xn = X().gate_residual_norm(c, pre="layer")
+    assert xn.abs().max().item() <= 48 * U32 * 7 / 1e-3
+    _, xz = X().gate_residual_norm(torch.zeros(3, 48, device="cuda"), pre="rms")
+    assert xz.abs().max().item() == 0
+
+
+# ------------------------------------------------------------------------------------------ together
+def _block(x, states, mask, P, plan, pos, ops):
+    """A conditioned block: tokens on (frame, residue) axes attend to an encoder's states, then an MLP."""
+    B, N, C = x.shape
+    H, Hk = 4, 2
+    D = C // H
+    gate, shift, scale, gate2 = P["mods"].split(C, -1)
+    _, xn = ops.gate_residual_norm(x, pre="rms", pre_w=P["w0"], shift=shift, scale=scale)
+    q = (xn @ P["wq"]).reshape(B, N, H, D)
+    k, v = (states @ P["wkv"]).reshape(B, -1, 2, Hk, D).unbind(2)
+    q = ops.rope_axes(plan, pos, q)
+    y = ops.cross_attention(q, k, v, mask=mask).reshape(B, N, C) @ P["wo"]
+    x, xn = ops.gate_residual_norm(x, y, gate=gate, post="rms", post_w=P["w1"], pre="layer")
+    y = torch.nn.functional.gelu(xn @ P["w_up"]) @ P["w_dn"]
+    x, _ = ops.gate_residual_norm(x, y, gate=gate2, post="layer", pre="none")
+    return x
+
+
+class _Plain:
+    """The three operators in elementary 64-bit operations."""
+
+    @staticmethod
+    def gate_residual_norm(h, y=None, gate=None, shift=None, scale=None, post="none", pre="layer", post_w=None, pre_w=None):
+        def norm(x, kind, w):
+            if kind == "layer":
+                x = x - x.mean(-1, keepdim=True)
+            if kind != "none":
+                x = x / torch.sqrt((x ** 2).mean(-1, keepdim=True) + 1e-6)
+            return x if w is None else x * w
+
+        if y is not None:
+            u = norm(y, post, post_w)
+            h = h + (u if gate is None else gate[:, None] * u)
+        if pre == "none":
+            return h, None
+        xn = norm(h, pre, pre_w)
+        return h, xn if scale is None else xn * (1 + scale[:, None]) + shift[:, None]
+
+    @staticmethod
+    def rope_axes(plan, pos, x):
+        c, n = plan.cols.long().cpu(), plan.npairs
+        ang = (pos.double().cpu()[..., plan.axis.long().cpu()] * plan.turns.cpu() * 2 * math.pi)[:, :, None]
+        a, b = x[..., c[:n]], x[..., c[n:]]
+        out = x.clone()
+        out[..., c[:n]] = a * ang.cos() - b * ang.sin()
+        out[..., c[n:]] = b * ang.cos() + a * ang.sin()
+        return out
+
+    @staticmethod
+    def cross_attention(q, k, v, mask):
+        G = q.shape[2] // k.shape[2]
+        kh, vh = (t.transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+        s = q.transpose(1, 2) @ kh.transpose(-1, -2) * q.shape[-1] ** -0.5
+        p = torch.softmax(s.masked_fill(~mask.cpu().bool()[:, None, None], -math.inf), -1)
+        return (p @ vh).transpose(1, 2)
+
+
+def _block_case(seed=1):
+    g = _gen(seed)
+    B, T, L, C, S, Cs = 2, 9, 4, 96, 21, 40
+    x, states = torch.randn(B, T * L, C, generator=g), torch.randn(B, S, Cs, generator=g)
+    w = lambda i, o: torch.randn(i, o, generator=g) / math.sqrt(i)  # noqa: E731
+    P = {"mods": 0.5 * torch.randn(B, 4 * C, generator=g), "w0": 1 + 0.1 * torch.randn(C, generator=g),
+         "w1": 1 + 0.1 * torch.randn(C, generator=g), "wq": w(C, C), "wkv": w(Cs, 2 * 2 * (C // 4)), "wo": w(C, C),
+         "w_up": w(C, 2 * C), "w_dn": w(2 * C, C)}
+    mask = (torch.rand(B, S, generator=g) < 0.7).float()
+    n = torch.arange(T * L)
+    pos = torch.stack([n // L, n % L], -1)[None].to(torch.int32)
+    return x, states, P, mask, pos
+
+
+def test_conditioned_block_forward_and_gradients():
+    x, states, P, mask, pos = _block_case()
+    plan = X().RopeAxes([8, 4], device="cuda")
+
+    def run(dev, dt, ops):
+        leaf = {n: t.to(dev, dt).requires_grad_(True) for n, t in {"x": x, "states": states, **P}.items()}
+        out = _block(leaf["x"], leaf["states"], mask.to(dev), leaf, plan, pos.to(dev), ops)
+        go = torch.linspace(-1, 1, out.numel(), device=dev, dtype=dt).reshape(out.shape)
+        return out, dict(zip(leaf, torch.autograd.grad(out, list(leaf.values()), go)))
+
+    got, gg = run("cuda", torch.float32, X())
+    want, wg = run("cpu", torch.float64, _Plain)
+    # six products of up to 192 terms and four norms, each within (terms + 64) 2^-24 of its row's magnitude and
+    # amplified at most 4x by the next: 10 * 256 * 4 * 2^-24 of the largest value
+    lim = 10 * 256 * 4 * U32
+    _near(got, want.detach(), lim * want.abs().max().item(), "block")
+    for n in wg:
+        _near(gg[n], wg[n], 4 * lim * wg[n].abs().max().item(), "d" + n)
+
+
+def test_conditioned_block_captured_and_replayed():
+    """Forward and backward in one graph, replayed with new inputs between eager runs; every replay equals the
+    eager bits."""
+    x, states, P, mask, pos = _block_case()
+    plan = X().RopeAxes([8, 4], device="cuda")
+    mask, pos = mask.cuda(), pos.cuda()
+    static = {n: t.cuda().requires_grad_(True) for n, t in {"x": x, "states": states, **P}.items()}
+    go = torch.randn(x.shape, generator=_gen(6)).cuda()
+
+    def step(leaf):
+        out = _block(leaf["x"], leaf["states"], mask, leaf, plan, pos, X())
+        return (out.detach(), *torch.autograd.grad(out, list(leaf.values()), go))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for i in range(4):
+        fresh = {n: (t.detach() * (1 + 0.1 * i) + 0.01 * i) for n, t in static.items()} if i else None
+        if fresh:
+            with torch.no_grad():
+                for n in static:
+                    static[n].copy_(fresh[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step({n: t.detach().clone().requires_grad_(True) for n, t in static.items()})
+        for a, b in zip(outs, eager):
+            assert torch.equal(a, b), i
+
+
+def test_operators_on_another_stream_and_repeatable():
+    q, k, v, do, *_ = _attn_inputs(2, 150, 333, 4, 2, 48, torch.bfloat16, "", 21)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    do = do.cuda()
+
+    def once():
+        o = X().cross_attention(*leaves)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    base = once()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(base, once()))
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    res = []
+    for s in (s1, s2):  # two calls at once on streams of their own
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            res.append(once())
+    torch.cuda.synchronize()
+    for r in res:
+        assert all(torch.equal(a, b) for a, b in zip(base, r))
