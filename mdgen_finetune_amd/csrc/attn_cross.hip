@@ -22,6 +22,8 @@
 
 #include <cfloat>
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 namespace mdg {
 namespace {
@@ -49,7 +51,6 @@ struct CrossP {
   float* part;  // split partials
   float* part_ml;
   int nsplit;
-  int vec;      // 16-byte pieces: D a multiple of a piece, every base and stride 16-byte aligned
 };
 
 template <typename CT>
@@ -63,12 +64,29 @@ __device__ __forceinline__ f32x16 mma(const typename V8<CT>::T& a, const typenam
   }
 }
 
-// LDS row stride: 32 bytes of padding put 8 consecutive rows on different banks for 16-byte reads
+// LDS tiles are rows of DP elements without padding (what an asynchronous load can fill: a wave writes
+// 1024 consecutive bytes); the 16-byte chunk c of row r lies at chunk c ^ chunk_xor(r).  The XOR puts
+// the 8 rows that one pass of a 16-byte row read covers, and the 4 rows of a transposing read, on
+// different banks.
 template <typename CT, int DP>
-constexpr int lds_ld() { return DP + 32 / (int)sizeof(CT); }
+__device__ __forceinline__ int chunk_xor(int r) {
+  if constexpr (sizeof(CT) == 2) {
+    if constexpr (DP >= 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (DP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  } else {
+    if constexpr (DP >= 64) return (r & 3) | ((r & 4) << 1);
+    else return (r >> 1) & 7;
+  }
+}
+// element offset of chunk c of row r
+template <typename CT, int DP>
+__device__ __forceinline__ int lds_at(int r, int c) {
+  return r * DP + (c ^ chunk_xor<CT, DP>(r)) * (16 / (int)sizeof(CT));
+}
 
-// element j: tile[k0 + 8 (j >> 2) + 4h + (j & 3)][c0 + (lane & 31)] of a row-major LDS tile
-template <typename CT, int LD>
+// element j: tile[k0 + 8 (j >> 2) + 4h + (j & 3)][c0 + (lane & 31)]
+template <typename CT, int DP>
 __device__ __forceinline__ typename V8<CT>::T col_frag(const CT* tile, int k0, int c0, int lane) {
   typename V8<CT>::T r;
   const int h = lane >> 5;
@@ -76,31 +94,42 @@ __device__ __forceinline__ typename V8<CT>::T col_frag(const CT* tile, int k0, i
     // ds_read_b64_tr_b16: in each group of 16 lanes, lane 4q + p supplies columns 4p..4p+3 of row q and
     // receives column (lane & 15) of the four rows
     typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-    const CT* a = tile + (k0 + 4 * h + ((lane & 15) >> 2)) * LD + c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)a);
-    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(a + 8 * LD));
+    const int row = k0 + 4 * h + ((lane & 15) >> 2), c = c0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), e = 4 * (lane & 1);
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + lds_at<CT, DP>(row, c) + e));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + lds_at<CT, DP>(row + 8, c) + e));
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = lo[j], r[4 + j] = hi[j];
   } else {
-    const CT* a = tile + (k0 + 4 * h) * LD + c0 + (lane & 31);
+    const int c = (c0 + (lane & 31)) / 4, e = lane & 3;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = a[j * LD], r[4 + j] = a[(8 + j) * LD];
+    for (int j = 0; j < 8; ++j) r[j] = tile[lds_at<CT, DP>(k0 + 8 * (j >> 2) + 4 * h + (j & 3), c) + e];
   }
   return r;
 }
 
-template <typename CT, int LD>
+template <typename CT, int DP>
 __device__ __forceinline__ typename V8<CT>::T row_frag(const CT* tile, int row, int k0, int lane) {
-  return ld8<CT>(tile + row * LD + k0 + 8 * (lane >> 5));
+  const int c = (k0 + 8 * (lane >> 5)) * (int)sizeof(CT) / 16;
+  if constexpr (is_bf16<CT>()) {
+    return *reinterpret_cast<const bf16x8*>(tile + lds_at<CT, DP>(row, c));
+  } else {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(tile + lds_at<CT, DP>(row, c));
+    const f32x4 b = *reinterpret_cast<const f32x4*>(tile + lds_at<CT, DP>(row, c + 1));
+    f32x8 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = a[j], r[4 + j] = b[j];
+    return r;
+  }
 }
 
-// one 16-byte piece (columns c0 ..) of a row of D elements, zero past D
-template <typename CT>
-__device__ __forceinline__ uint4 ld_piece(const CT* row, int c0, int D, int vec) {
+// one 16-byte piece (columns c0 .., c0 < D) of a row of D elements, zero past D.  VEC: D is a multiple of a
+// piece and every base and stride is 16-byte aligned; otherwise element by element.
+template <typename CT, bool VEC>
+__device__ __forceinline__ uint4 ld_piece(const CT* row, int c0, int D) {
   constexpr int N = 16 / sizeof(CT);
   uint4 r = make_uint4(0, 0, 0, 0);
-  if (vec) {
-    if (c0 < D) r = *reinterpret_cast<const uint4*>(row + c0);
+  if constexpr (VEC) {
+    r = *reinterpret_cast<const uint4*>(row + c0);
   } else {
     CT e[N];
 #pragma unroll
@@ -109,13 +138,13 @@ __device__ __forceinline__ uint4 ld_piece(const CT* row, int c0, int D, int vec)
   }
   return r;
 }
-template <typename CT>
-__device__ __forceinline__ typename V8<CT>::T ld_frag(const CT* row, int c0, int D, int vec) {
+template <typename CT, bool VEC>
+__device__ __forceinline__ typename V8<CT>::T ld_frag(const CT* row, int c0, int D) {
   typename V8<CT>::T r;
   constexpr int N = 16 / sizeof(CT);
 #pragma unroll
   for (int j = 0; j < 8; j += N) {
-    const uint4 u = ld_piece<CT>(row, c0 + j, D, vec);
+    const uint4 u = c0 + j < D ? ld_piece<CT, VEC>(row, c0 + j, D) : make_uint4(0, 0, 0, 0);
     CT e[N];
     __builtin_memcpy(e, &u, 16);
 #pragma unroll
@@ -124,10 +153,10 @@ __device__ __forceinline__ typename V8<CT>::T ld_frag(const CT* row, int c0, int
   return r;
 }
 
-// four consecutive outputs d0 .. d0 + 3 of a row (vec: 8- / 16-byte stores, D a multiple of 4)
-template <typename CT>
-__device__ __forceinline__ void st_out(CT* row, int d0, int D, int vec, float a, float b, float c, float d) {
-  if (vec) {
+// four consecutive outputs d0 .. d0 + 3 of a row
+template <typename CT, bool VEC>
+__device__ __forceinline__ void st_out(CT* row, int d0, int D, float a, float b, float c, float d) {
+  if constexpr (VEC) {
     if (d0 < D) st4<CT>(row + d0, a, b, c, d);
   } else {
     if (d0 < D) row[d0] = (CT)a;
@@ -162,7 +191,9 @@ __device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32
 // The softmax of one 32-key tile: raises the lane's maximum when a score outgrows it by 2^8 (a lagging
 // maximum costs no precision: P is floating point and stays below 2^8, sums are fp32), turns the
 // scores into P and adds their sum.  s: raw scores, -inf where the key is masked.
-template <int NT, int DT>
+// DT counts every accumulator that carries the lane's scale; SUM: l is summed here (otherwise by a
+// product with ones, in the last of them).
+template <int NT, int DT, bool SUM>
 __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NT], f32x16 (&o)[DT], float& m, float& l, float c) {
   const float grow = 8.0f / c;
   float mx = s[0][0];
@@ -188,83 +219,189 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NT], f32x16 (&o)[DT], f
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -mc));
-      sum += s[t][i];
+      if constexpr (SUM) sum += s[t][i];
     }
-  l += sum;
+  if constexpr (SUM) l += sum;
 }
 
-// A tile of k / v rows on its way from memory to LDS through registers, by NT threads.
-template <typename CT, int DP, int ROWS, int NT>
-struct Stage {
-  static constexpr int LD = lds_ld<CT, DP>(), VEC = 16 / sizeof(CT), PPR = DP / VEC, P = ROWS * PPR / NT;
-  static_assert(ROWS * PPR % NT == 0, "whole pieces per thread");
-  uint4 r[P];
-  // rows key0 .. key0 + ROWS of one (b, kv head); keys >= end are zero
-  __device__ __forceinline__ void load(const CT* base, long long sn, int key0, int end, int D, int vec, int tid) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int idx = tid + i * NT, row = idx / PPR, cc = (idx % PPR) * VEC, key = key0 + row;
-      r[i] = key < end ? ld_piece<CT>(base + key * sn, cc, D, vec) : make_uint4(0, 0, 0, 0);
-    }
-  }
-  __device__ __forceinline__ void store(CT* tile, int tid) const {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int idx = tid + i * NT, row = idx / PPR, cc = (idx % PPR) * VEC;
-      *reinterpret_cast<uint4*>(tile + row * LD + cc) = r[i];
-    }
-  }
-};
+// Asynchronous loads, memory -> LDS, 16 bytes per lane at lds + 16 * lane.  Offsets outside the
+// resource's bytes read zeros, so a lane whose piece is not there is sent out of range.  (In assembly:
+// for the builtin the compiler waits for every such load before any later LDS read.  There is no
+// register result; async_wait below comes before the barrier after which the tile is read.)
+constexpr unsigned kNowhere = 0x80000000u;
+__device__ __forceinline__ u32x4 resource(uint64_t base, unsigned bytes) {
+  u32x4 r;
+  r[0] = (unsigned)base, r[1] = (unsigned)(base >> 32) & 0xffffu, r[2] = bytes, r[3] = 0x00020000u;
+  return r;
+}
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+  // (readfirstlane gives an int: the low word must not be widened with its sign)
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+// (m0 is written right before each use, by the compiler too.  Five wait states before the load, which
+// the compiler does not count into assembly: the vector unit may just have written the resource's
+// scalar registers.)
+__device__ __forceinline__ void async_load16(const u32x4& res, unsigned lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(res)
+               : "memory");
+}
+// all but this wave's N youngest loads have landed
+template <int N = 0>
+__device__ __forceinline__ void async_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// Masked keys' k / v rows are zero in LDS (what lies there, NaN too, never reaches a product) and their
-// scores start at -inf: kb holds 0 or -inf per key and is the product's initial accumulator.
-template <typename CT, int DP, int ROWS, int NT>
+// k and v tiles of ROWS keys of one (b, key head), by NT threads.  Masked keys' rows are zero in LDS (what
+// lies there, NaN too, never reaches a product) and their scores start at -inf: kb holds 0 or
+// -inf per key and is the products' initial accumulator; a tile whose keys are all there (flag 0) skips that.
+//   begin(key0): starts the tile (ASYNC: straight into LDS; else into registers)
+//   finish(...): completes it in LDS; the caller's barrier follows
+// Tiles come in order, `step` keys apart, init with the first.
+template <typename CT, int DP, int ROWS, int NT, bool VEC, bool ASYNC>
 struct KvStage {
-  Stage<CT, DP, ROWS, NT> k, v;
-  float keep[Stage<CT, DP, ROWS, NT>::P];
+  static constexpr int N = 16 / sizeof(CT), CPR = DP / N, P = ROWS * CPR / NT;
+  static_assert(ROWS * CPR % NT == 0 && ROWS <= 64, "whole pieces per thread");
+  uint4 k[ASYNC ? 1 : P], v[ASYNC ? 1 : P];
+  unsigned ko[ASYNC ? P : 1], vo[ASYNC ? P : 1];  // byte offsets of this thread's pieces in a tile
+  bool keep[P];  // ASYNC: of the tile to begin next; else of the begun one
   float kb;
-  __device__ __forceinline__ void load(const CrossP& p, const CT* kbase, const CT* vbase, int b, int key0, int end,
-                                       int tid) {
-    using S = Stage<CT, DP, ROWS, NT>;
-    k.load(kbase, p.k.sn, key0, end, p.D, p.vec, tid);
-    v.load(vbase, p.v.sn, key0, end, p.D, p.vec, tid);
-    if (p.mask) {
+  const CT *kp, *vp;           // the tile's first row
+  uint64_t ka, va;             // ASYNC: its address, and the strides from tile to tile, in bytes
+  int64_t kstep, vstep;
+  unsigned first;              // ASYNC: this wave's first slot in a tile, in bytes
+  // ASYNC: piece i is slot (wave * P + i) * 64 + lane of the tile's 16-byte slots; else i * NT + tid
+  __device__ __forceinline__ static int slot(int i, int tid) {
+    return ASYNC ? ((tid >> 6) * P + i) * 64 + (tid & 63) : i * NT + tid;
+  }
+  __device__ __forceinline__ void init(const CrossP& p, int b, int hk, int key0, int end, int step, int tid) {
+    kp = vrow<CT>(p.k, b, key0, hk);
+    vp = vrow<CT>(p.v, b, key0, hk);
+    if constexpr (ASYNC) {
+      ka = uniform64((uint64_t)kp), va = uniform64((uint64_t)vp);
+      kstep = step * p.k.sn * (int)sizeof(CT), vstep = step * p.v.sn * (int)sizeof(CT);
+      first = __builtin_amdgcn_readfirstlane(tid >> 6) * P * 1024;
 #pragma unroll
-      for (int i = 0; i < S::P; ++i) {
-        const int key = key0 + (tid + i * NT) / S::PPR;
-        keep[i] = key < end && key_kept(p, b, key) ? 1.f : 0.f;
+      for (int i = 0; i < P; ++i) {
+        const int row = slot(i, tid) / CPR, c = slot(i, tid) % CPR ^ chunk_xor<CT, DP>(row);
+        ko[i] = c * N < p.D ? (unsigned)(row * p.k.sn * sizeof(CT)) + c * 16 : kNowhere;
+        vo[i] = c * N < p.D ? (unsigned)(row * p.v.sn * sizeof(CT)) + c * 16 : kNowhere;
       }
     }
-    const int key = key0 + tid;
-    kb = tid < ROWS && key < end && key_kept(p, b, key) ? 0.f : -INFINITY;
+    if constexpr (ASYNC) look(p, b, key0, end, tid);
   }
-  // flag: some key of the tile is not there (one wave holds all of kb: ROWS <= 64)
-  __device__ __forceinline__ void store(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int tid) {
-    using S = Stage<CT, DP, ROWS, NT>;
-    if (p.mask) {
+  __device__ __forceinline__ void look(const CrossP& p, int b, int key0, int end, int tid) {
+    if (!p.mask) return;
 #pragma unroll
-      for (int i = 0; i < S::P; ++i)
-        if (keep[i] == 0.f) k.r[i] = v.r[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < P; ++i) {
+      const int key = key0 + slot(i, tid) / CPR;
+      keep[i] = key < end && key_kept(p, b, key);
     }
-    k.store(Ks, tid);
-    v.store(Vs, tid);
+  }
+  __device__ __forceinline__ void begin(const CrossP& p, CT* Ks, CT* Vs, int b, int key0, int end, int step, int tid) {
+    const int here = min(ROWS, end - key0);
+    if constexpr (ASYNC) {
+      const u32x4 kr = resource(ka, (unsigned)(((here - 1) * p.k.sn + p.D) * (int)sizeof(CT)));
+      const u32x4 vr = resource(va, (unsigned)(((here - 1) * p.v.sn + p.D) * (int)sizeof(CT)));
+      const unsigned kl = lds_address(Ks) + first, vl = lds_address(Vs) + first;
+      if (p.mask) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          async_load16(kr, kl + i * 1024, keep[i] ? ko[i] : kNowhere);
+          async_load16(vr, vl + i * 1024, keep[i] ? vo[i] : kNowhere);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          async_load16(kr, kl + i * 1024, ko[i]);
+          async_load16(vr, vl + i * 1024, vo[i]);
+        }
+      }
+      ka += kstep, va += vstep;
+    } else {
+      look(p, b, key0, end, tid);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int row = slot(i, tid) / CPR, cc = slot(i, tid) % CPR * N;
+        const bool in = row < here && cc < p.D;
+        k[i] = in ? ld_piece<CT, VEC>(kp + row * p.k.sn, cc, p.D) : make_uint4(0, 0, 0, 0);
+        v[i] = in ? ld_piece<CT, VEC>(vp + row * p.v.sn, cc, p.D) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    if constexpr (!ASYNC) kp += step * p.k.sn, vp += step * p.v.sn;
+    kb = 0.f;
+    if (p.mask || here < ROWS) {  // (uniform)
+      if (tid < ROWS) kb = tid < here && key_kept(p, b, key0 + tid) ? 0.f : -INFINITY;
+      if constexpr (ASYNC) look(p, b, key0 + step, end, tid);
+    }
+  }
+  __device__ __forceinline__ void finish_rows(const CrossP& p, CT* Ks, CT* Vs, int tid) {
+    if constexpr (!ASYNC) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int at = lds_at<CT, DP>(slot(i, tid) / CPR, slot(i, tid) % CPR);
+        const bool drop = p.mask && !keep[i];
+        *reinterpret_cast<uint4*>(Ks + at) = drop ? make_uint4(0, 0, 0, 0) : k[i];
+        *reinterpret_cast<uint4*>(Vs + at) = drop ? make_uint4(0, 0, 0, 0) : v[i];
+      }
+    }
+  }
+  __device__ __forceinline__ void finish_kb(float* kbs, int* flag, int tid) {
     if (tid < 64) {
       if (tid < ROWS) kbs[tid] = kb;
-      const bool any = __any(tid < ROWS && kb != 0.f);
+      const bool any = __any(kb != 0.f);
       if (tid == 0) *flag = any;
     }
   }
+  __device__ __forceinline__ void finish(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int tid) {
+    finish_rows(p, Ks, Vs, tid);
+    finish_kb(kbs, flag, tid);
+    if constexpr (ASYNC) async_wait();
+  }
 };
 
-// initial accumulator of a 32-key tile of S^T: the keys' kb, rows 8a + 4h + i
-__device__ __forceinline__ f32x16 kb_init(const float* kbs, int flag, int lane) {
+// initial accumulator of a 32-key tile of S^T with keys that are not there: their kb (rows 8a + 4h + i)
+__device__ __forceinline__ f32x16 kb_init(const float* kbs, int lane) {
   f32x16 s;
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const float4 t = flag ? *reinterpret_cast<const float4*>(kbs + 8 * a + 4 * (lane >> 5)) : make_float4(0, 0, 0, 0);
+    const float4 t = *reinterpret_cast<const float4*>(kbs + 8 * a + 4 * (lane >> 5));
     s[4 * a] = t.x, s[4 * a + 1] = t.y, s[4 * a + 2] = t.z, s[4 * a + 3] = t.w;
   }
   return s;
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.f;
+  return s;
+}
+
+// S^T of a tile of NT * 32 keys.  (The products stand in both branches: an accumulator that is one of two
+// things would be copied, one that starts at a literal zero is not.)
+template <typename CT, int DP, int NT>
+__device__ __forceinline__ void key_scores(f32x16 (&s)[NT], const CT* Kt, const typename V8<CT>::T (&qf)[DP / 16],
+                                           const float* kbs, bool holes, int lane) {
+  if (holes) {
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt) {
+      s[kt] = kb_init(kbs + 32 * kt, lane);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+        s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
+    }
+  } else {
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt) {
+      s[kt] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+        s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
+    }
+  }
 }
 
 template <typename CT>
@@ -303,76 +440,12 @@ __device__ __forceinline__ long long part_row(const CrossP& p, int sp, int b, in
   return ((long long)sp * p.B * p.Hk + (long long)b * p.Hk + hk) * rows + r;
 }
 
-// ------------------------------------------------------------------------------------------ forward
-// One block = 4 waves x 32 rows of one (b, key head); k / v tiles of KT keys go through LDS, double
-// buffered through registers, one barrier per tile.
-template <typename CT, int DP, int KT>
-__global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int tiles) {
-  constexpr int LD = lds_ld<CT, DP>(), DT = DP / 32, KS = DP / 16, NT = KT / 32;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  CT* Ks = reinterpret_cast<CT*>(smem);
-  CT* Vs = Ks + 2 * KT * LD;
-  float* kbs = reinterpret_cast<float*>(Vs + 2 * KT * LD);
-  int* flag = reinterpret_cast<int*>(kbs + 2 * KT);
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  const BlockId id = block_id(p, tiles);
-  const int rows = p.Nq * p.G, r = id.tile * 128 + wave * 32 + (lane & 31);
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
-  const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
-  const bool live = r < rows && n < qlen;
-
-  typename V8<CT>::T qf[KS];
-  const CT* qrow = vrow<CT>(p.q, id.b, live ? n : 0, live ? head : 0);
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT>(qrow, 16 * ks + 8 * h, p.D, p.vec) : zero8<CT>();
-
-  f32x16 o[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-  float m = kNoMax, l = 0.f;
-
-  int k0, k1;
-  split_range(klen, p.nsplit, id.split, k0, k1);
-  const CT* kbase = vrow<CT>(p.k, id.b, 0, id.hk);
-  const CT* vbase = vrow<CT>(p.v, id.b, 0, id.hk);
-  KvStage<CT, DP, KT, 256> st;
-  const int nt = (k1 - k0 + KT - 1) / KT;
-  if (nt > 0) {
-    st.load(p, kbase, vbase, id.b, k0, k1, tid);
-    st.store(p, Ks, Vs, kbs, flag, tid);
-  }
-  __syncthreads();
-  for (int t = 0; t < nt; ++t) {
-    const int cur = t & 1;
-    if (t + 1 < nt) st.load(p, kbase, vbase, id.b, k0 + (t + 1) * KT, k1, tid);
-    const CT* Kc = Ks + cur * KT * LD;
-    const CT* Vc = Vs + cur * KT * LD;
-    f32x16 s[NT];
-#pragma unroll
-    for (int kt = 0; kt < NT; ++kt) {
-      s[kt] = kb_init(kbs + cur * KT + 32 * kt, flag[cur], lane);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s[kt] = mma<CT>(row_frag<CT, LD>(Kc, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
-    }
-    softmax_tile<NT, DT>(s, o, m, l, p.c);
-#pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const typename V8<CT>::T pf = half_frag<CT>(s[kt], s2);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          o[dt] = mma<CT>(col_frag<CT, LD>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
-      }
-    if (t + 1 < nt) st.store(p, Ks + (cur ^ 1) * KT * LD, Vs + (cur ^ 1) * KT * LD, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
-    __syncthreads();
-  }
-
-  l = half_sum(l);
+// a lane's row of outputs, O^T rows 32 dt + 8a + 4h + i: normalised, or a split's partial
+template <typename CT, int DP, bool VEC>
+__device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, int r, int rows, bool live,
+                                           const f32x16* o, float m, float l, int lane) {
+  constexpr int DT = DP / 32;
+  const int h = lane >> 5;
   if (r >= rows) return;
   if (p.nsplit > 1) {
     const long long pr = part_row(p, id.split, id.b, id.hk, r);
@@ -388,6 +461,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
             make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
     return;
   }
+  const int n = r / p.G, head = id.hk * p.G + r % p.G;
   const bool some = live && l != 0.f;  // (a NaN among the keys that are there stays one)
   const float inv = some ? 1.0f / l : 0.f;
   if (p.lse && h == 0) p.lse[((long long)id.b * p.H + head) * p.Nq + n] = some ? m * p.c + log2f(l) : -INFINITY;
@@ -401,25 +475,176 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = some ? o[dt][4 * a + i] * inv : 0.f;
       const int d0 = 32 * dt + 8 * a + 4 * h;
-      st_out<CT>(orow, d0, p.D, p.vec, v[0], v[1], v[2], v[3]);
+      st_out<CT, VEC>(orow, d0, p.D, v[0], v[1], v[2], v[3]);
       if (lrow)  // the rounding residual of o, for an exact delta in the backward
-        st_out<CT>(lrow, d0, p.D, p.vec, v[0] - (float)(CT)v[0], v[1] - (float)(CT)v[1], v[2] - (float)(CT)v[2],
-                   v[3] - (float)(CT)v[3]);
+        st_out<CT, VEC>(lrow, d0, p.D, v[0] - (float)(CT)v[0], v[1] - (float)(CT)v[1], v[2] - (float)(CT)v[2],
+                        v[3] - (float)(CT)v[3]);
     }
 }
 
-// At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
-// the rows.  Each wave stages its own 32-key tiles (no block barrier in the loop: a wave's LDS
-// operations are in order), and the four partial softmaxes are joined in LDS at the end.
-template <typename CT, int DP>
-__global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tiles) {
-  constexpr int LD = lds_ld<CT, DP>(), DT = DP / 32, KS = DP / 16, LO = DP + 4;
+// ------------------------------------------------------------------------------------------ forward
+// One block = 4 waves x 32 rows of one (b, key head); k / v tiles of KT keys go through LDS, double
+// buffered through registers, one barrier per tile.
+template <typename CT, int DP, int KT, bool VEC>
+__global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int tiles) {
+  constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  CT* Ks = reinterpret_cast<CT*>(smem) + wave * 2 * 32 * LD;
-  CT* Vs = Ks + 32 * LD;
-  float* kbs = reinterpret_cast<float*>(reinterpret_cast<CT*>(smem) + 4 * 2 * 32 * LD) + wave * 32;
-  int* flag = reinterpret_cast<int*>(reinterpret_cast<float*>(reinterpret_cast<CT*>(smem) + 4 * 2 * 32 * LD) + 128) + wave;
+  CT* Ks = reinterpret_cast<CT*>(smem);
+  CT* Vs = Ks + 2 * TILE;
+  float* kbs = reinterpret_cast<float*>(Vs + 2 * TILE);
+  int* flag = reinterpret_cast<int*>(kbs + 2 * KT);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const BlockId id = block_id(p, tiles);
+  const int rows = p.Nq * p.G, r = id.tile * 128 + wave * 32 + (lane & 31);
+  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
+  const bool live = r < rows && n < qlen;
+
+  typename V8<CT>::T qf[KS];
+  const CT* qrow = vrow<CT>(p.q, id.b, live ? n : 0, live ? head : 0);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT, VEC>(qrow, 16 * ks + 8 * h, p.D) : zero8<CT>();
+
+  // narrow bf16 heads are bound by the vector unit: the row sums (of the rounded probabilities) then
+  // come from a product with ones, o[DT]
+  constexpr bool kOnes = sizeof(CT) == 2 && DP <= 64;
+  constexpr int NO = DT + (kOnes ? 1 : 0);
+  f32x16 o[NO];
+#pragma unroll
+  for (int t = 0; t < NO; ++t) o[t] = zero16();
+  typename V8<CT>::T ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (CT)1.f;
+  float m = kNoMax, l = 0.f;
+
+  int k0, k1;
+  split_range(klen, p.nsplit, id.split, k0, k1);
+  KvStage<CT, DP, KT, 256, VEC, VEC> st;
+  const int nt = (k1 - k0 + KT - 1) / KT;
+  if (nt > 0) {
+    st.init(p, id.b, id.hk, k0, k1, KT, tid);
+    st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
+    st.finish(p, Ks, Vs, kbs, flag, tid);
+  }
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const int cur = t & 1;
+    const int other = (cur ^ 1) * TILE;
+    if (t + 1 < nt) st.begin(p, Ks + other, Vs + other, id.b, k0 + (t + 1) * KT, k1, KT, tid);
+    const CT* Kc = Ks + cur * TILE;
+    const CT* Vc = Vs + cur * TILE;
+    f32x16 s[NT];
+    key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), lane);
+    softmax_tile<NT, NO, !kOnes>(s, o, m, l, p.c);
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const typename V8<CT>::T pf = half_frag<CT>(s[kt], s2);
+        if constexpr (kOnes) o[DT] = mma<CT>(ones, pf, o[DT]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
+      }
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
+    __syncthreads();
+  }
+
+  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, kOnes ? o[NO - 1][0] : half_sum(l), lane);
+}
+
+// The same with two groups of four waves (256 rows per block), one phase apart, each SIMD holding one wave
+// of either group: while one group's waves run their matrix products (M), the other's run their softmax
+// (V), and a barrier ends every phase.  (Left to themselves, waves of equal code drift into step and the
+// matrix cores and the vector unit take turns.)
+//   M(t): O += V(t-1)^T P(t-1), S = K(t) Q^T;   V(t): P(t) = softmax of S
+// Group 0 loads: K(t+1) and V(t+1) start at its M(t) and are awaited at the end of its V(t); K lies in two
+// buffers, V, read a phase later, in three.
+template <int DP, int KT>
+__global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, int tiles) {
+  using CT = bf16_t;
+  constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  CT* Ks = reinterpret_cast<CT*>(smem);
+  CT* Vs = Ks + 2 * TILE;
+  float* kbs = reinterpret_cast<float*>(Vs + 3 * TILE);
+  int* flag = reinterpret_cast<int*>(kbs + 2 * KT);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const bool second = wave >= 4;
+  const BlockId id = block_id(p, tiles);
+  const int rows = p.Nq * p.G, r = id.tile * 256 + wave * 32 + (lane & 31);
+  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
+  const bool live = r < rows && n < qlen;
+
+  bf16x8 qf[KS];
+  const CT* qrow = vrow<CT>(p.q, id.b, live ? n : 0, live ? head : 0);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT, true>(qrow, 16 * ks + 8 * h, p.D) : zero8<CT>();
+  f32x16 o[DT], s[NT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = zero16();
+  float m = kNoMax, l = 0.f;
+  bf16x8 pf[NT][2];
+
+  int k0, k1;
+  split_range(klen, p.nsplit, id.split, k0, k1);
+  KvStage<CT, DP, KT, 256, true, true> st;
+  const int nt = (k1 - k0 + KT - 1) / KT;
+  if (nt > 0 && !second) {
+    st.init(p, id.b, id.hk, k0, k1, KT, tid);
+    st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
+    st.finish(p, Ks, Vs, kbs, flag, tid);
+  }
+  __syncthreads();
+  if (second) __syncthreads();
+  int vprev = 0, vnext = 1;  // buffers of V(t-1) and V(t+1)
+  for (int t = 0; t <= nt; ++t) {
+    const bool loads = !second && t + 1 < nt;
+    if (loads) st.begin(p, Ks + ((t + 1) & 1) * TILE, Vs + vnext * TILE, id.b, k0 + (t + 1) * KT, k1, KT, tid);
+    if (t > 0) {
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            o[dt] = mma<CT>(col_frag<CT, DP>(Vs + vprev * TILE, 32 * kt + 16 * s2, 32 * dt, lane), pf[kt][s2], o[dt]);
+      vprev = vprev == 2 ? 0 : vprev + 1;
+    }
+    if (t < nt)
+      key_scores<CT, DP, NT>(s, Ks + (t & 1) * TILE, qf, kbs + (t & 1) * KT, __builtin_amdgcn_readfirstlane(flag[t & 1]), lane);
+    __syncthreads();
+    if (t < nt) {
+      softmax_tile<NT, DT, true>(s, o, m, l, p.c);
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) pf[kt][0] = half_frag<CT>(s[kt], 0), pf[kt][1] = half_frag<CT>(s[kt], 1);
+    }
+    if (loads) st.finish(p, Ks, Vs, kbs + ((t + 1) & 1) * KT, flag + ((t + 1) & 1), tid);
+    vnext = vnext == 2 ? 0 : vnext + 1;
+    __syncthreads();
+  }
+  if (!second) __syncthreads();
+  store_rows<CT, DP, true>(p, id, r, rows, live, o, m, half_sum(l), lane);
+}
+
+// At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
+// the rows.  Each wave stages its own 32-key tiles in two buffers of its own (no block barrier in the
+// loop: a wave's LDS operations are in order), and the four partial softmaxes are joined in LDS at the end.
+// (fp32 at 128 columns: two buffers per wave would not fit, it stages through registers)
+template <typename CT, int DP, bool VEC>
+constexpr bool few_async() { return VEC && sizeof(CT) * DP <= 256; }
+template <typename CT, int DP, bool VEC>
+__global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tiles) {
+  constexpr int TILE = 32 * DP, DT = DP / 32, KS = DP / 16, LO = DP + 4, BUFS = few_async<CT, DP, VEC>() ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  CT* Ks = reinterpret_cast<CT*>(smem) + wave * 2 * BUFS * TILE;
+  CT* Vs = Ks + BUFS * TILE;
+  float* kbs = reinterpret_cast<float*>(reinterpret_cast<CT*>(smem) + 4 * 2 * BUFS * TILE) + wave * 32;
+  int* flag = reinterpret_cast<int*>(reinterpret_cast<float*>(reinterpret_cast<CT*>(smem) + 4 * 2 * BUFS * TILE) + 128) + wave;
 
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = lane & 31;
@@ -427,42 +652,55 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const bool live = r < rows && n < qlen;
   typename V8<CT>::T qf[KS];
-  const CT* qrow = vrow<CT>(p.q, id.b, live ? n : 0, live ? head : 0);
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT>(qrow, 16 * ks + 8 * h, p.D, p.vec) : zero8<CT>();
   f32x16 o[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  for (int t = 0; t < DT; ++t) o[t] = zero16();
   float m = kNoMax, l = 0.f;
 
   int k0, k1;
   split_range(klen, p.nsplit, id.split, k0, k1);
-  const CT* kbase = vrow<CT>(p.k, id.b, 0, id.hk);
-  const CT* vbase = vrow<CT>(p.v, id.b, 0, id.hk);
-  KvStage<CT, DP, 32, 64> st;
-  int key = k0 + 32 * wave;
-  if (key < k1) st.load(p, kbase, vbase, id.b, key, k1, lane);
+  using S = KvStage<CT, DP, 32, 64, VEC, BUFS == 2>;
+  S st;
+  int key = k0 + 32 * wave, cur = 0;
+  if (key < k1) {
+    st.init(p, id.b, id.hk, key, k1, 128, lane);
+    st.begin(p, Ks, Vs, id.b, key, k1, 128, lane);
+  }
+  const CT* qrow = vrow<CT>(p.q, id.b, live ? n : 0, live ? head : 0);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT, VEC>(qrow, 16 * ks + 8 * h, p.D) : zero8<CT>();
   for (; key < k1; key += 128) {
-    st.store(p, Ks, Vs, kbs, flag, lane);
-    if (key + 128 < k1) st.load(p, kbase, vbase, id.b, key + 128, k1, lane);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    f32x16 s[1] = {kb_init(kbs, *flag, lane)};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s[0] = mma<CT>(row_frag<CT, LD>(Ks, lane & 31, 16 * ks, lane), qf[ks], s[0]);
-    softmax_tile<1, DT>(s, o, m, l, p.c);
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename V8<CT>::T pf = half_frag<CT>(s[0], s2);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = mma<CT>(col_frag<CT, LD>(Vs, 16 * s2, 32 * dt, lane), pf, o[dt]);
+    st.finish_kb(kbs, flag, lane);
+    const bool more = key + 128 < k1;
+    if constexpr (BUFS == 2) {
+      if (more) {
+        st.begin(p, Ks + (cur ^ 1) * TILE, Vs + (cur ^ 1) * TILE, id.b, key + 128, k1, 128, lane);
+        async_wait<2 * S::P>();  // this tile's loads, not the next one's
+      } else {
+        async_wait();
+      }
+    } else {
+      st.finish_rows(p, Ks, Vs, lane);
+      if (more) st.begin(p, Ks, Vs, id.b, key + 128, k1, 128, lane);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    f32x16 s[1];
+    key_scores<CT, DP, 1>(s, Ks + cur * TILE, qf, kbs, __builtin_amdgcn_readfirstlane(*flag), lane);
+    softmax_tile<1, DT, true>(s, o, m, l, p.c);
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const typename V8<CT>::T pf = half_frag<CT>(s[0], s2);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] = mma<CT>(col_frag<CT, DP>(Vs + cur * TILE, 16 * s2, 32 * dt, lane), pf, o[dt]);
+    }
+    // the next turn's loads overwrite this buffer: its reads are done before they start
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if constexpr (BUFS == 2) cur ^= 1;
   }
   l = half_sum(l);
 
@@ -516,58 +754,70 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
       const bool some = rn < qlen && Lr != 0.f;
       const float inv = some ? 1.0f / Lr : 0.f;
       v = some ? make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv) : make_float4(0, 0, 0, 0);
-      st_out<CT>(wrow<CT>(p.o, id.b, rn, rh), d0, p.D, p.vec, v.x, v.y, v.z, v.w);
+      st_out<CT, VEC>(wrow<CT>(p.o, id.b, rn, rh), d0, p.D, v.x, v.y, v.z, v.w);
       if (p.olo.p)
-        st_out<CT>(wrow<CT>(p.olo, id.b, rn, rh), d0, p.D, p.vec, v.x - (float)(CT)v.x, v.y - (float)(CT)v.y,
+        st_out<CT, VEC>(wrow<CT>(p.olo, id.b, rn, rh), d0, p.D, v.x - (float)(CT)v.x, v.y - (float)(CT)v.y,
                    v.z - (float)(CT)v.z, v.w - (float)(CT)v.w);
     }
   }
 }
 
-// Joins the splits' partial softmaxes: 32 lanes per row, fixed order over the splits.
-template <typename CT, int DP>
+// Joins the splits' partial softmaxes: 32 lanes per row.  A lane reads the statistics of the splits
+// lane, lane + 32, ...; then the lanes walk the splits in order, four columns each.
+template <typename CT, int DP, bool VEC>
 __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
   const long long rows = (long long)p.Nq * p.G, total = rows * p.B * p.Hk;
   const long long pr = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int d0 = (threadIdx.x & 31) * 4;
-  if (pr >= total) return;
-  float M = kNoMax, L = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, p.part_ml[2 * (s * total + pr)]);
+  const int sub = threadIdx.x & 31, d0 = sub * 4;
+  if (pr >= total) return;  // (all 32 lanes of the row)
+  float M = kNoMax;
+  for (int s = sub; s < p.nsplit; s += 32) M = fmaxf(M, p.part_ml[2 * (s * total + pr)]);
+#pragma unroll
+  for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+  float L = 0.f;
   float4 v = make_float4(0, 0, 0, 0);
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float ms = p.part_ml[2 * (s * total + pr)];
-    const float f = ms == kNoMax ? 1.f : __builtin_amdgcn_exp2f((ms - M) * p.c);  // (no keys: sums of 0)
-    L += f * p.part_ml[2 * (s * total + pr) + 1];
-    if (d0 < DP) {
-      const float4 t = *reinterpret_cast<const float4*>(p.part + (s * total + pr) * DP + d0);
-      v.x = fmaf(f, t.x, v.x), v.y = fmaf(f, t.y, v.y), v.z = fmaf(f, t.z, v.z), v.w = fmaf(f, t.w, v.w);
+  for (int s0 = 0; s0 < p.nsplit; s0 += 32) {
+    float f = 0.f, lf = 0.f;
+    if (s0 + sub < p.nsplit) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((s0 + sub) * total + pr));
+      f = ml.x == kNoMax ? 1.f : __builtin_amdgcn_exp2f((ml.x - M) * p.c);  // (no keys: sums of 0)
+      lf = f * ml.y;
+    }
+    const int n = min(32, p.nsplit - s0);
+    for (int s = 0; s < n; ++s) {
+      const float fs = __shfl(f, (threadIdx.x & 32) + s, 64);
+      L += __shfl(lf, (threadIdx.x & 32) + s, 64);
+      if (d0 < DP) {
+        const float4 t = *reinterpret_cast<const float4*>(p.part + ((s0 + s) * total + pr) * DP + d0);
+        v.x = fmaf(fs, t.x, v.x), v.y = fmaf(fs, t.y, v.y), v.z = fmaf(fs, t.z, v.z), v.w = fmaf(fs, t.w, v.w);
+      }
     }
   }
   const int bh = (int)(pr / rows), r = (int)(pr % rows), b = bh / p.Hk, n = r / p.G, head = (bh % p.Hk) * p.G + r % p.G;
   const bool some = n < clamp_len(p.qlen, b, p.Nq) && L != 0.f;
   const float inv = some ? 1.0f / L : 0.f;
   if (p.lse && d0 == 0) p.lse[((long long)b * p.H + head) * p.Nq + n] = some ? M * p.c + log2f(L) : -INFINITY;
-  if (d0 >= DP) return;
+  if (d0 >= p.D) return;
   v = some ? make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv) : make_float4(0, 0, 0, 0);
-  st_out<CT>(wrow<CT>(p.o, b, n, head), d0, p.D, p.vec, v.x, v.y, v.z, v.w);
+  st_out<CT, VEC>(wrow<CT>(p.o, b, n, head), d0, p.D, v.x, v.y, v.z, v.w);
   if (p.olo.p)
-    st_out<CT>(wrow<CT>(p.olo, b, n, head), d0, p.D, p.vec, v.x - (float)(CT)v.x, v.y - (float)(CT)v.y,
-               v.z - (float)(CT)v.z, v.w - (float)(CT)v.w);
+    st_out<CT, VEC>(wrow<CT>(p.olo, b, n, head), d0, p.D, v.x - (float)(CT)v.x, v.y - (float)(CT)v.y,
+                    v.z - (float)(CT)v.z, v.w - (float)(CT)v.w);
 }
 
 // ------------------------------------------------------------------------------------------ backward
 // dq: the forward's layout (one query per lane).  delta = do . (o + o_lo) is formed here from the
 // fragments in registers and left for the dk / dv pass.
-template <typename CT, int DP, int KT>
+template <typename CT, int DP, int KT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_kernel(const CrossP p, int tiles) {
-  constexpr int LD = lds_ld<CT, DP>(), DT = DP / 32, KS = DP / 16, NT = KT / 32;
+  constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   CT* Ks = reinterpret_cast<CT*>(smem);
-  CT* Vs = Ks + 2 * KT * LD;
-  float* kbs = reinterpret_cast<float*>(Vs + 2 * KT * LD);
+  CT* Vs = Ks + 2 * TILE;
+  float* kbs = reinterpret_cast<float*>(Vs + 2 * TILE);
   int* flag = reinterpret_cast<int*>(kbs + 2 * KT);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = id.tile * 128 + wave * 32 + (lane & 31);
   const int n = r / p.G, head = id.hk * p.G + r % p.G;
@@ -581,11 +831,11 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const int c0 = 16 * ks + 8 * h;
-    qf[ks] = live ? ld_frag<CT>(vrow<CT>(p.q, id.b, ln, lh), c0, p.D, p.vec) : zero8<CT>();
-    gf[ks] = live ? ld_frag<CT>(vrow<CT>(p.dout, id.b, ln, lh), c0, p.D, p.vec) : zero8<CT>();
-    const typename V8<CT>::T of = live ? ld_frag<CT>(vrow<CT>(p.o, id.b, ln, lh), c0, p.D, p.vec) : zero8<CT>();
+    qf[ks] = live ? ld_frag<CT, VEC>(vrow<CT>(p.q, id.b, ln, lh), c0, p.D) : zero8<CT>();
+    gf[ks] = live ? ld_frag<CT, VEC>(vrow<CT>(p.dout, id.b, ln, lh), c0, p.D) : zero8<CT>();
+    const typename V8<CT>::T of = live ? ld_frag<CT, VEC>(vrow<CT>(p.o, id.b, ln, lh), c0, p.D) : zero8<CT>();
     if (p.olo.p) {
-      const typename V8<CT>::T lo = live ? ld_frag<CT>(vrow<CT>(p.olo, id.b, ln, lh), c0, p.D, p.vec) : zero8<CT>();
+      const typename V8<CT>::T lo = live ? ld_frag<CT, VEC>(vrow<CT>(p.olo, id.b, ln, lh), c0, p.D) : zero8<CT>();
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[ks][j], (float)of[j] + (float)lo[j], delta);
     } else {
@@ -606,30 +856,29 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
 
   int k0, k1;
   split_range(klen, p.nsplit, id.split, k0, k1);
-  const CT* kbase = vrow<CT>(p.k, id.b, 0, id.hk);
-  const CT* vbase = vrow<CT>(p.v, id.b, 0, id.hk);
-  KvStage<CT, DP, KT, 256> st;
+  KvStage<CT, DP, KT, 256, VEC, VEC> st;
   const int nt = (k1 - k0 + KT - 1) / KT;
   if (nt > 0) {
-    st.load(p, kbase, vbase, id.b, k0, k1, tid);
-    st.store(p, Ks, Vs, kbs, flag, tid);
+    st.init(p, id.b, id.hk, k0, k1, KT, tid);
+    st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
+    st.finish(p, Ks, Vs, kbs, flag, tid);
   }
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const int cur = t & 1;
-    if (t + 1 < nt) st.load(p, kbase, vbase, id.b, k0 + (t + 1) * KT, k1, tid);
-    const CT* Kc = Ks + cur * KT * LD;
-    const CT* Vc = Vs + cur * KT * LD;
+    const int other = (cur ^ 1) * TILE;
+    if (t + 1 < nt) st.begin(p, Ks + other, Vs + other, id.b, k0 + (t + 1) * KT, k1, KT, tid);
+    const CT* Kc = Ks + cur * TILE;
+    const CT* Vc = Vs + cur * TILE;
+    const bool holes = __builtin_amdgcn_readfirstlane(flag[cur]);
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt) {
-      f32x16 s = kb_init(kbs + cur * KT + 32 * kt, flag[cur], lane), g;
+      f32x16 s1[1], g = zero16();
+      f32x16& s = s1[0];
+      key_scores<CT, DP, 1>(s1, Kc + 32 * kt * DP, qf, kbs + cur * KT + 32 * kt, holes, lane);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) g[i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = mma<CT>(row_frag<CT, LD>(Kc, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s);
-        g = mma<CT>(row_frag<CT, LD>(Vc, 32 * kt + (lane & 31), 16 * ks, lane), gf[ks], g);
-      }
+      for (int ks = 0; ks < KS; ++ks)
+        g = mma<CT>(row_frag<CT, DP>(Vc, 32 * kt + (lane & 31), 16 * ks, lane), gf[ks], g);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse)) * (g[i] - delta);
 #pragma unroll
@@ -637,10 +886,10 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
         const typename V8<CT>::T df = half_frag<CT>(s, s2);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          acc[dt] = mma<CT>(col_frag<CT, LD>(Kc, 32 * kt + 16 * s2, 32 * dt, lane), df, acc[dt]);
+          acc[dt] = mma<CT>(col_frag<CT, DP>(Kc, 32 * kt + 16 * s2, 32 * dt, lane), df, acc[dt]);
       }
     }
-    if (t + 1 < nt) st.store(p, Ks + (cur ^ 1) * KT * LD, Vs + (cur ^ 1) * KT * LD, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
     __syncthreads();
   }
   if (r >= rows) return;
@@ -659,25 +908,80 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int a = 0; a < 4; ++a)
-      st_out<CT>(row, 32 * dt + 8 * a + 4 * h, p.D, p.vec, acc[dt][4 * a] * p.scale, acc[dt][4 * a + 1] * p.scale,
+      st_out<CT, VEC>(row, 32 * dt + 8 * a + 4 * h, p.D, acc[dt][4 * a] * p.scale, acc[dt][4 * a + 1] * p.scale,
                  acc[dt][4 * a + 2] * p.scale, acc[dt][4 * a + 3] * p.scale);
 }
 
+// Packed rows of q and do, QT at a time, on their way to LDS (as KvStage), with their lse and delta.
+template <typename CT, int DP, int QT, bool VEC, bool ASYNC>
+struct RowStage {
+  static constexpr int N = 16 / sizeof(CT), CPR = DP / N, P = QT * CPR / 256;
+  static_assert(QT * CPR % 256 == 0 && QT <= 64, "whole pieces per thread");
+  uint4 q[ASYNC ? 1 : P], g[ASYNC ? 1 : P];
+  float lse, delta;
+  __device__ __forceinline__ static int slot(int i, int tid) {
+    return ASYNC ? ((tid >> 6) * P + i) * 64 + (tid & 63) : i * 256 + tid;
+  }
+  __device__ __forceinline__ void begin(const CrossP& p, CT* Qs, CT* Gs, int b, int hk, int row0, int end, int tid) {
+    const int n0 = row0 / p.G;
+    const CT* qb = vrow<CT>(p.q, b, n0, hk * p.G);
+    const CT* gb = vrow<CT>(p.dout, b, n0, hk * p.G);
+    u32x4 qr, gr;
+    if constexpr (ASYNC) qr = resource(uniform64((uint64_t)qb), 0x7fffffffu), gr = resource(uniform64((uint64_t)gb), 0x7fffffffu);
+    const unsigned first = __builtin_amdgcn_readfirstlane(tid >> 6) * P * 1024;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int lr = slot(i, tid) / CPR, row = row0 + lr, n = row / p.G, hd = row - n * p.G;
+      if constexpr (ASYNC) {
+        const int c = slot(i, tid) % CPR ^ chunk_xor<CT, DP>(lr);
+        const bool in = row < end && c * N < p.D;
+        const int dn = n - n0;
+        async_load16(qr, lds_address(Qs) + first + i * 1024,
+                     in ? (unsigned)((dn * p.q.sn + hd * p.q.sh) * sizeof(CT)) + c * 16 : kNowhere);
+        async_load16(gr, lds_address(Gs) + first + i * 1024,
+                     in ? (unsigned)((dn * p.dout.sn + hd * p.dout.sh) * sizeof(CT)) + c * 16 : kNowhere);
+      } else {
+        const int cc = slot(i, tid) % CPR * N;
+        const bool in = row < end && cc < p.D;
+        q[i] = in ? ld_piece<CT, VEC>(qb + (n - n0) * p.q.sn + hd * p.q.sh, cc, p.D) : make_uint4(0, 0, 0, 0);
+        g[i] = in ? ld_piece<CT, VEC>(gb + (n - n0) * p.dout.sn + hd * p.dout.sh, cc, p.D) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    lse = INFINITY, delta = 0.f;  // (every P of a row past the end, or without keys, is 0)
+    if (tid < QT && row0 + tid < end) {
+      const int row = row0 + tid, n = row / p.G, hd = hk * p.G + row % p.G;
+      const long long i = ((long long)b * p.H + hd) * p.Nq + n;
+      lse = p.lse[i], delta = p.delta[i];
+      if (lse == -INFINITY) lse = INFINITY;
+    }
+  }
+  __device__ __forceinline__ void finish(CT* Qs, CT* Gs, float* ls, float* ds, int tid) {
+    if constexpr (!ASYNC) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int at = lds_at<CT, DP>(slot(i, tid) / CPR, slot(i, tid) % CPR);
+        *reinterpret_cast<uint4*>(Qs + at) = q[i];
+        *reinterpret_cast<uint4*>(Gs + at) = g[i];
+      }
+    }
+    if (tid < QT) ls[tid] = lse, ds[tid] = delta;
+    if constexpr (ASYNC) async_wait();
+  }
+};
+
 // dk, dv: one key per lane; a block owns 4 x 32 keys of one (b, key head) and walks the rows in tiles
-// of 32 (q and do through LDS, double buffered); splits share the rows, their fp32 partials summed in
+// of QT (q and do through LDS, double buffered); splits share the rows, their fp32 partials summed in
 // order by cross_sum_kernel.
-template <typename CT, int DP>
+template <typename CT, int DP, int QT, bool VEC>
 __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tiles) {
-  constexpr int LD = lds_ld<CT, DP>(), DT = DP / 32, KS = DP / 16, QT = 32;
-  using S = Stage<CT, DP, QT, (QT * DP * (int)sizeof(CT) / 16 < 256 ? 128 : 256)>;
-  constexpr int SN = QT * DP * (int)sizeof(CT) / 16 < 256 ? 128 : 256;
+  constexpr int TILE = QT * DP, DT = DP / 32, KS = DP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   CT* Qs = reinterpret_cast<CT*>(smem);
-  CT* Gs = Qs + 2 * QT * LD;
-  float* ls = reinterpret_cast<float*>(Gs + 2 * QT * LD);  // [2][QT]
+  CT* Gs = Qs + 2 * TILE;
+  float* ls = reinterpret_cast<float*>(Gs + 2 * TILE);  // [2][QT]
   float* ds = ls + 2 * QT;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const BlockId id = block_id(p, tiles);
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const int rows = qlen * p.G;
@@ -688,93 +992,60 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const int c0 = 16 * ks + 8 * h;
-    kf[ks] = live ? ld_frag<CT>(vrow<CT>(p.k, id.b, key, id.hk), c0, p.D, p.vec) : zero8<CT>();
-    vf[ks] = live ? ld_frag<CT>(vrow<CT>(p.v, id.b, key, id.hk), c0, p.D, p.vec) : zero8<CT>();
+    kf[ks] = live ? ld_frag<CT, VEC>(vrow<CT>(p.k, id.b, key, id.hk), c0, p.D) : zero8<CT>();
+    vf[ks] = live ? ld_frag<CT, VEC>(vrow<CT>(p.v, id.b, key, id.hk), c0, p.D) : zero8<CT>();
   }
   f32x16 dk[DT], dv[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
+  for (int t = 0; t < DT; ++t) dk[t] = dv[t] = zero16();
 
   const int per = ((rows + p.nsplit - 1) / p.nsplit + QT - 1) / QT * QT;
   const int r0 = min(rows, id.split * per), r1 = min(rows, r0 + per);
-  const int nt = (r1 - r0 + QT - 1) / QT;
   // a block whose keys all lie past the sequence has nothing to sum
-  const int todo = id.tile * 128 < klen ? nt : 0;
+  const int todo = id.tile * 128 < klen ? (r1 - r0 + QT - 1) / QT : 0;
 
-  uint4 rq[S::P], rg[S::P];
-  float rl = INFINITY, rd = 0.f;
-  auto load = [&](int row0) {
-#pragma unroll
-    for (int i = 0; i < S::P; ++i) {
-      const int idx = tid + i * SN, row = row0 + idx / S::PPR, cc = (idx % S::PPR) * S::VEC;
-      rq[i] = rg[i] = make_uint4(0, 0, 0, 0);
-      if (tid < SN && row < r1) {
-        const int n = row / p.G, hd = id.hk * p.G + row % p.G;
-        rq[i] = ld_piece<CT>(vrow<CT>(p.q, id.b, n, hd), cc, p.D, p.vec);
-        rg[i] = ld_piece<CT>(vrow<CT>(p.dout, id.b, n, hd), cc, p.D, p.vec);
-      }
-    }
-    rl = INFINITY, rd = 0.f;
-    if (tid < QT && row0 + tid < r1) {
-      const int row = row0 + tid, n = row / p.G, hd = id.hk * p.G + row % p.G;
-      const long long i = ((long long)id.b * p.H + hd) * p.Nq + n;
-      rl = p.lse[i], rd = p.delta[i];
-      if (rl == -INFINITY) rl = INFINITY;
-    }
-  };
-  auto store = [&](int buf) {
-    if (tid < SN) {
-#pragma unroll
-      for (int i = 0; i < S::P; ++i) {
-        const int idx = tid + i * SN, row = idx / S::PPR, cc = (idx % S::PPR) * S::VEC;
-        *reinterpret_cast<uint4*>(Qs + buf * QT * LD + row * LD + cc) = rq[i];
-        *reinterpret_cast<uint4*>(Gs + buf * QT * LD + row * LD + cc) = rg[i];
-      }
-    }
-    if (tid < QT) ls[buf * QT + tid] = rl, ds[buf * QT + tid] = rd;
-  };
+  RowStage<CT, DP, QT, VEC, VEC> st;
   if (todo > 0) {
-    load(r0);
-    store(0);
+    st.begin(p, Qs, Gs, id.b, id.hk, r0, r1, tid);
+    st.finish(Qs, Gs, ls, ds, tid);
   }
   __syncthreads();
   for (int t = 0; t < todo; ++t) {
-    const int cur = t & 1;
-    if (t + 1 < todo) load(r0 + (t + 1) * QT);
-    const CT* Qc = Qs + cur * QT * LD;
-    const CT* Gc = Gs + cur * QT * LD;
-    f32x16 s, g;
+    const int cur = t & 1, other = (cur ^ 1) * TILE;
+    if (t + 1 < todo) st.begin(p, Qs + other, Gs + other, id.b, id.hk, r0 + (t + 1) * QT, r1, tid);
+    const CT* Qc = Qs + cur * TILE;
+    const CT* Gc = Gs + cur * TILE;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = g[i] = 0.f;
+    for (int qt = 0; qt < QT; qt += 32) {
+      f32x16 s = zero16(), g = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      s = mma<CT>(row_frag<CT, LD>(Qc, lane & 31, 16 * ks, lane), kf[ks], s);
-      g = mma<CT>(row_frag<CT, LD>(Gc, lane & 31, 16 * ks, lane), vf[ks], g);
-    }
+      for (int ks = 0; ks < KS; ++ks) {
+        s = mma<CT>(row_frag<CT, DP>(Qc, qt + (lane & 31), 16 * ks, lane), kf[ks], s);
+        g = mma<CT>(row_frag<CT, DP>(Gc, qt + (lane & 31), 16 * ks, lane), vf[ks], g);
+      }
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const float4 lv = *reinterpret_cast<const float4*>(ls + cur * QT + 8 * a + 4 * h);
-      const float4 dl = *reinterpret_cast<const float4*>(ds + cur * QT + 8 * a + 4 * h);
-      const float lw[4] = {lv.x, lv.y, lv.z, lv.w}, dw[4] = {dl.x, dl.y, dl.z, dl.w};
+      for (int a = 0; a < 4; ++a) {
+        const float4 lv = *reinterpret_cast<const float4*>(ls + cur * QT + qt + 8 * a + 4 * h);
+        const float4 dl = *reinterpret_cast<const float4*>(ds + cur * QT + qt + 8 * a + 4 * h);
+        const float lw[4] = {lv.x, lv.y, lv.z, lv.w}, dw[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * a + i], p.c, -lw[i]));
-        s[4 * a + i] = pr;
-        g[4 * a + i] = pr * (g[4 * a + i] - dw[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * a + i], p.c, -lw[i]));
+          s[4 * a + i] = pr;
+          g[4 * a + i] = pr * (g[4 * a + i] - dw[i]);
+        }
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const typename V8<CT>::T pf = half_frag<CT>(s, s2), df = half_frag<CT>(g, s2);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          dv[dt] = mma<CT>(col_frag<CT, DP>(Gc, qt + 16 * s2, 32 * dt, lane), pf, dv[dt]);
+          dk[dt] = mma<CT>(col_frag<CT, DP>(Qc, qt + 16 * s2, 32 * dt, lane), df, dk[dt]);
+        }
       }
     }
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename V8<CT>::T pf = half_frag<CT>(s, s2), df = half_frag<CT>(g, s2);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        dv[dt] = mma<CT>(col_frag<CT, LD>(Gc, 16 * s2, 32 * dt, lane), pf, dv[dt]);
-        dk[dt] = mma<CT>(col_frag<CT, LD>(Qc, 16 * s2, 32 * dt, lane), df, dk[dt]);
-      }
-    }
-    if (t + 1 < todo) store(cur ^ 1);
+    if (t + 1 < todo) st.finish(Qs + other, Gs + other, ls + (cur ^ 1) * QT, ds + (cur ^ 1) * QT, tid);
     __syncthreads();
   }
   if (key >= p.Nk) return;
@@ -792,15 +1063,15 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
         *reinterpret_cast<float4*>(p.part + pr) = make_float4(x[0], x[1], x[2], x[3]);
         *reinterpret_cast<float4*>(p.part + pr + total * DP) = make_float4(y[0], y[1], y[2], y[3]);
       } else {
-        st_out<CT>(wrow<CT>(p.dk, id.b, key, id.hk), d0, p.D, p.vec, x[0], x[1], x[2], x[3]);
-        st_out<CT>(wrow<CT>(p.dv, id.b, key, id.hk), d0, p.D, p.vec, y[0], y[1], y[2], y[3]);
+        st_out<CT, VEC>(wrow<CT>(p.dk, id.b, key, id.hk), d0, p.D, x[0], x[1], x[2], x[3]);
+        st_out<CT, VEC>(wrow<CT>(p.dv, id.b, key, id.hk), d0, p.D, y[0], y[1], y[2], y[3]);
       }
     }
 }
 
 // sums the splits' fp32 partials in order: nout planes [rows][DP] per split -> the strided outputs.
 // kv: rows (b, hk, key), planes dk | dv; else rows (b, hk, n * G + g), dq scaled here.
-template <typename CT, int DP>
+template <typename CT, int DP, bool VEC>
 __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossP p, int kv) {
   constexpr int Q = DP / 4;
   const long long rows = kv ? (long long)p.Nk : (long long)p.Nq * p.G, total = rows * p.B * p.Hk;
@@ -816,9 +1087,9 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossP p, int kv) 
   const long long r0 = row % total;
   const int bh = (int)(r0 / rows), r = (int)(r0 % rows), b = bh / p.Hk, hk = bh % p.Hk;
   if (kv) {
-    st_out<CT>(wrow<CT>(row < total ? p.dk : p.dv, b, r, hk), d0, p.D, p.vec, v.x, v.y, v.z, v.w);
+    st_out<CT, VEC>(wrow<CT>(row < total ? p.dk : p.dv, b, r, hk), d0, p.D, v.x, v.y, v.z, v.w);
   } else {
-    st_out<CT>(wrow<CT>(p.dq, b, r / p.G, hk * p.G + r % p.G), d0, p.D, p.vec, v.x * p.scale, v.y * p.scale,
+    st_out<CT, VEC>(wrow<CT>(p.dq, b, r / p.G, hk * p.G + r % p.G), d0, p.D, v.x * p.scale, v.y * p.scale,
                v.z * p.scale, v.w * p.scale);
   }
 }
@@ -846,7 +1117,7 @@ bool aligned16(const mdg_heads& t, int e) {
   return !t.p || ((reinterpret_cast<uintptr_t>(t.p) | (uintptr_t)(t.sb * e) | (uintptr_t)(t.sn * e) | (uintptr_t)(t.sh * e)) & 15) == 0;
 }
 
-CrossP params(const mdg_attn_cross& a, bool bwd) {
+CrossP params(const mdg_attn_cross& a) {
   CrossP p;
   p.q = view(a.q), p.k = view(a.k), p.v = view(a.v), p.o = view(a.o), p.olo = view(a.o_lo);
   p.dout = view(a.dout), p.dq = view(a.dq), p.dk = view(a.dk), p.dv = view(a.dv);
@@ -855,27 +1126,39 @@ CrossP params(const mdg_attn_cross& a, bool bwd) {
   p.B = a.B, p.Nq = a.Nq, p.Nk = a.Nk, p.H = a.H, p.Hk = a.Hk, p.G = a.H / a.Hk, p.D = a.D;
   p.c = a.scale * kLog2e, p.scale = a.scale, p.lse = a.lse;
   p.delta = nullptr, p.part = p.part_ml = nullptr, p.nsplit = 1;
-  const int e = a.dtype == MDG_BF16 ? 2 : 4;
-  p.vec = a.D % (16 / e) == 0 && aligned16(a.q, e) && aligned16(a.k, e) && aligned16(a.v, e) && aligned16(a.o, e) &&
-          aligned16(a.o_lo, e);
-  if (bwd) p.vec = p.vec && aligned16(a.dout, e) && aligned16(a.dq, e) && aligned16(a.dk, e) && aligned16(a.dv, e);
   return p;
 }
 
+// 16-byte pieces: the head dim a multiple of a piece, every base and stride 16-byte aligned; and a tile's
+// rows apart, within the 2^30 bytes that an asynchronous load's offset spans (64 keys, or 65 tokens)
+bool pieces(const mdg_attn_cross& a, bool bwd) {
+  const int e = a.dtype == MDG_BF16 ? 2 : 4;
+  const int64_t span = (int64_t)1 << 30;
+  bool ok = a.D % (16 / e) == 0;
+  for (const mdg_heads* t : {&a.q, &a.k, &a.v, &a.o, &a.o_lo}) ok = ok && aligned16(*t, e);
+  for (const mdg_heads* t : {&a.k, &a.v}) ok = ok && t->sn >= a.D && 64 * t->sn * e < span;
+  if (bwd) {
+    for (const mdg_heads* t : {&a.dout, &a.dq, &a.dk, &a.dv}) ok = ok && aligned16(*t, e);
+    for (const mdg_heads* t : {&a.q, &a.dout}) ok = ok && (65 * t->sn + a.H * t->sh) * e < span;
+  }
+  return ok;
+}
+
 struct Plan {
-  bool few;
+  bool few, pp;  // the single-token kernel; the two-phase kernel
   long long tiles;
   int split;
   size_t part, ml, bytes;  // byte offsets / total
 };
 size_t al(size_t n) { return (n + 255) / 256 * 256; }
 
-Plan fwd_plan(const mdg_attn_cross& a) {
+Plan fwd_plan(const mdg_attn_cross& a, bool vec) {
   Plan w;
   const long long rows = (long long)a.Nq * (a.H / a.Hk), bh = (long long)a.B * a.Hk;
   w.few = rows <= 32;
-  w.tiles = w.few ? 1 : (rows + 127) / 128;
-  w.split = pick_split(w.tiles * bh, a.Nk, w.few ? 256 : 512, w.few ? 1024 : 512);
+  w.pp = a.dtype == MDG_BF16 && vec && dp_of_head(a.D) == 128 && rows >= 256;
+  w.tiles = w.few ? 1 : w.pp ? (rows + 255) / 256 : (rows + 127) / 128;
+  w.split = pick_split(w.tiles * bh, a.Nk, a.dtype == MDG_F32 && !w.few ? 96 : 256, w.few ? 1024 : w.pp ? 256 : 512);
   w.part = 0, w.ml = w.bytes = 0;
   if (w.split > 1) {
     w.ml = al((size_t)w.split * rows * bh * dp_of_head(a.D) * 4);
@@ -893,8 +1176,8 @@ BwdPlan bwd_plan(const mdg_attn_cross& a) {
   BwdPlan w;
   const long long rows = (long long)a.Nq * (a.H / a.Hk), bh = (long long)a.B * a.Hk;
   w.qtiles = (rows + 127) / 128, w.ktiles = ((long long)a.Nk + 127) / 128;
-  w.qsplit = pick_split(w.qtiles * bh, a.Nk, 512, 512);
-  w.ksplit = pick_split(w.ktiles * bh, rows, 256, 512);
+  w.qsplit = pick_split(w.qtiles * bh, a.Nk, a.dtype == MDG_F32 ? 96 : 256, 512);
+  w.ksplit = pick_split(w.ktiles * bh, rows, a.dtype == MDG_F32 ? 96 : 256, 512);
   w.delta = 0;
   w.part = al((size_t)a.B * a.H * a.Nq * 4);
   const size_t dp = dp_of_head(a.D);
@@ -904,11 +1187,11 @@ BwdPlan bwd_plan(const mdg_attn_cross& a) {
   return w;
 }
 
-template <typename CT, int DP>
+template <typename CT, int DP, bool VEC>
 hipError_t fwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
-  constexpr int KT = sizeof(CT) == 2 ? 64 : 32, LD = lds_ld<CT, DP>();
-  const Plan w = fwd_plan(a);
-  CrossP p = params(a, false);
+  constexpr int KT = sizeof(CT) == 2 ? 64 : 32;
+  const Plan w = fwd_plan(a, VEC);
+  CrossP p = params(a);
   p.nsplit = w.split;
   if (w.split > 1) {
     p.part = reinterpret_cast<float*>(ws);
@@ -917,64 +1200,79 @@ hipError_t fwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
   const unsigned grid = (unsigned)(w.tiles * w.split * a.B * a.Hk);
   hipError_t e;
   if (w.few) {
-    const size_t stage = (size_t)4 * 2 * 32 * LD * sizeof(CT) + 4 * 32 * 4 + 16;
+    const size_t stage = (size_t)4 * 2 * (few_async<CT, DP, VEC>() ? 2 : 1) * 32 * DP * sizeof(CT) + 4 * 32 * 4 + 16;
     const size_t join = (size_t)(288 + 128 * (DP + 4)) * 4, sm = stage > join ? stage : join;
-    if ((e = allow_lds(cross_few_kernel<CT, DP>, sm)) != hipSuccess) return e;
-    hipLaunchKernelGGL((cross_few_kernel<CT, DP>), dim3(grid), dim3(256), sm, s, p, 1);
+    if ((e = allow_lds(cross_few_kernel<CT, DP, VEC>, sm)) != hipSuccess) return e;
+    hipLaunchKernelGGL((cross_few_kernel<CT, DP, VEC>), dim3(grid), dim3(256), sm, s, p, 1);
+  } else if (w.pp) {
+    if constexpr (VEC && sizeof(CT) == 2 && DP == 128) {
+      const size_t sm = (size_t)5 * KT * DP * sizeof(CT) + 2 * KT * 4 + 16;
+      if ((e = allow_lds(cross_fwd_pp_kernel<DP, KT>, sm)) != hipSuccess) return e;
+      hipLaunchKernelGGL((cross_fwd_pp_kernel<DP, KT>), dim3(grid), dim3(512), sm, s, p, (int)w.tiles);
+    }
   } else {
-    const size_t sm = (size_t)4 * KT * LD * sizeof(CT) + 2 * KT * 4 + 16;
-    if ((e = allow_lds(cross_fwd_kernel<CT, DP, KT>, sm)) != hipSuccess) return e;
-    hipLaunchKernelGGL((cross_fwd_kernel<CT, DP, KT>), dim3(grid), dim3(256), sm, s, p, (int)w.tiles);
+    const size_t sm = (size_t)4 * KT * DP * sizeof(CT) + 2 * KT * 4 + 16;
+    if ((e = allow_lds(cross_fwd_kernel<CT, DP, KT, VEC>, sm)) != hipSuccess) return e;
+    hipLaunchKernelGGL((cross_fwd_kernel<CT, DP, KT, VEC>), dim3(grid), dim3(256), sm, s, p, (int)w.tiles);
   }
   if (w.split > 1) {
     const long long total = (long long)a.B * a.H * a.Nq;
-    hipLaunchKernelGGL((cross_join_kernel<CT, DP>), dim3((unsigned)((total + 7) / 8)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((cross_join_kernel<CT, DP, VEC>), dim3((unsigned)((total + 7) / 8)), dim3(256), 0, s, p);
   }
   return hipGetLastError();
 }
 
-template <typename CT, int DP>
+template <typename CT, int DP, bool VEC>
 hipError_t bwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
-  constexpr int KT = sizeof(CT) == 2 ? 64 : 32, LD = lds_ld<CT, DP>(), QT = 32;
+  constexpr int KT = sizeof(CT) == 2 ? 64 : 32, QT = sizeof(CT) == 2 && DP <= 64 ? 64 : 32;
   const BwdPlan w = bwd_plan(a);
-  CrossP p = params(a, true);
+  CrossP p = params(a);
   p.delta = reinterpret_cast<float*>(static_cast<char*>(ws) + w.delta);
   p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);
   hipError_t e;
-  const size_t smq = (size_t)4 * KT * LD * sizeof(CT) + 2 * KT * 4 + 16;
-  const size_t smk = (size_t)4 * QT * LD * sizeof(CT) + 4 * QT * 4;
-  if ((e = allow_lds(cross_dq_kernel<CT, DP, KT>, smq)) != hipSuccess) return e;
-  if ((e = allow_lds(cross_dkv_kernel<CT, DP>, smk)) != hipSuccess) return e;
+  const size_t smq = (size_t)4 * KT * DP * sizeof(CT) + 2 * KT * 4 + 16;
+  const size_t smk = (size_t)4 * QT * DP * sizeof(CT) + 4 * QT * 4;
+  if ((e = allow_lds(cross_dq_kernel<CT, DP, KT, VEC>, smq)) != hipSuccess) return e;
+  if ((e = allow_lds(cross_dkv_kernel<CT, DP, QT, VEC>, smk)) != hipSuccess) return e;
   p.nsplit = w.qsplit;
-  hipLaunchKernelGGL((cross_dq_kernel<CT, DP, KT>), dim3((unsigned)(w.qtiles * w.qsplit * a.B * a.Hk)), dim3(256), smq, s, p,
+  hipLaunchKernelGGL((cross_dq_kernel<CT, DP, KT, VEC>), dim3((unsigned)(w.qtiles * w.qsplit * a.B * a.Hk)), dim3(256), smq, s, p,
                      (int)w.qtiles);
   if (w.qsplit > 1) {
     const long long n = (long long)a.B * a.H * a.Nq * (DP / 4);
-    hipLaunchKernelGGL((cross_sum_kernel<CT, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 0);
+    hipLaunchKernelGGL((cross_sum_kernel<CT, DP, VEC>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 0);
   }
   if (!a.dk.p || a.Nk == 0) return hipGetLastError();  // a frozen encoder, or none
   p.nsplit = w.ksplit;
-  hipLaunchKernelGGL((cross_dkv_kernel<CT, DP>), dim3((unsigned)(w.ktiles * w.ksplit * a.B * a.Hk)), dim3(256), smk, s, p,
+  hipLaunchKernelGGL((cross_dkv_kernel<CT, DP, QT, VEC>), dim3((unsigned)(w.ktiles * w.ksplit * a.B * a.Hk)), dim3(256), smk, s, p,
                      (int)w.ktiles);
   if (w.ksplit > 1) {
     const long long n = (long long)a.B * a.Hk * a.Nk * 2 * (DP / 4);
-    hipLaunchKernelGGL((cross_sum_kernel<CT, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 1);
+    hipLaunchKernelGGL((cross_sum_kernel<CT, DP, VEC>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 1);
   }
   return hipGetLastError();
 }
 
-template <typename CT>
+template <typename CT, bool VEC>
 hipError_t by_head(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s) {
   switch (dp_of_head(a.D)) {
-    case 32: return back ? bwd<CT, 32>(a, ws, s) : fwd<CT, 32>(a, ws, s);
-    case 64: return back ? bwd<CT, 64>(a, ws, s) : fwd<CT, 64>(a, ws, s);
-    default: return back ? bwd<CT, 128>(a, ws, s) : fwd<CT, 128>(a, ws, s);
+    case 32: return back ? bwd<CT, 32, VEC>(a, ws, s) : fwd<CT, 32, VEC>(a, ws, s);
+    case 64: return back ? bwd<CT, 64, VEC>(a, ws, s) : fwd<CT, 64, VEC>(a, ws, s);
+    default: return back ? bwd<CT, 128, VEC>(a, ws, s) : fwd<CT, 128, VEC>(a, ws, s);
   }
+}
+template <typename CT>
+hipError_t by_layout(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s) {
+  return pieces(a, back) ? by_head<CT, true>(a, back, ws, s) : by_head<CT, false>(a, back, ws, s);
 }
 
 }  // namespace
 
-size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back) { return back ? bwd_plan(a).bytes : fwd_plan(a).bytes; }
+// (for either layout: a size query need not know the tensors)
+size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back) {
+  if (back) return bwd_plan(a).bytes;
+  const size_t x = fwd_plan(a, false).bytes, y = fwd_plan(a, true).bytes;
+  return x > y ? x : y;
+}
 
 // grid sizes of every launch, for the host-side check (each must stay below 2^31)
 bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back) {
@@ -982,7 +1280,7 @@ bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back) {
   const long long rows = (long long)a.Nq * (a.H / a.Hk);
   if (rows > lim || rows * bh > lim || (long long)a.Nk * bh > lim) return false;
   if (!back) {
-    const Plan w = fwd_plan(a);
+    const Plan w = fwd_plan(a, false);  // (the other has half the tiles)
     return w.tiles * w.split * bh <= lim;
   }
   const BwdPlan w = bwd_plan(a);
@@ -991,7 +1289,7 @@ bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back) {
 }
 
 hipError_t attn_cross_launch(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s) {
-  return a.dtype == MDG_BF16 ? by_head<bf16_t>(a, back, ws, s) : by_head<float>(a, back, ws, s);
+  return a.dtype == MDG_BF16 ? by_layout<bf16_t>(a, back, ws, s) : by_layout<float>(a, back, ws, s);
 }
 
 }  // namespace mdg

@@ -141,6 +141,11 @@ ATTN = [  # B, Nq, Nk, H, Hk, D, padding, layout
     (1, 40, 700, 2, 1, 128, "len", "tokens"),
     (4, 3, 5, 2, 2, 16, "len mask q", "tokens"),
     (1, 2, 0, 2, 1, 8, "", "tokens"),           # an encoder without states
+    # enough rows for the wide blocks of each head width
+    (8, 300, 100, 16, 16, 24, "mask", "tokens"),
+    (4, 520, 161, 32, 16, 64, "len q", "heads"),
+    (4, 260, 133, 32, 32, 128, "mask len", "tokens"),
+    (16, 257, 31, 16, 16, 40, "", "tokens"),
 ]
 
 
