@@ -42,29 +42,45 @@ _NO_HEADS = (0, 0, 0, 0)
 
 
 def _check_device(t, *others):
-    if not t.is_cuda:
-        raise RuntimeError("mdgen_finetune_amd.cross_hip runs on a ROCm device; got a tensor on " + str(t.device))
+    dev = t.device
+    if dev.type != "cuda":
+        raise RuntimeError("mdgen_finetune_amd.cross_hip runs on a ROCm device; got a tensor on " + str(dev))
     for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
+        if o is not None and o.device != dev:
+            raise ValueError(f"tensors on {dev} and {o.device}")
 
 
-class _On:
-    """The tensors' device made current for the launch, where it is not."""
-    __slots__ = ("prev", "idx")
+def _stream(dev):
+    """(the device index to go back to, or -1; the current stream of the tensors' device, which is current now)."""
+    idx, cur = dev.index, torch._C._cuda_getDevice()
+    if cur == idx:
+        return -1, torch._C._cuda_getCurrentRawStream(idx)
+    torch._C._cuda_setDevice(idx)
+    return cur, torch._C._cuda_getCurrentRawStream(idx)
 
-    def __init__(self, t):
-        self.idx = t.device.index
 
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-        return torch.cuda.current_stream(self.idx).cuda_stream
+def _done(back, rc, what):
+    if back >= 0:
+        torch._C._cuda_setDevice(back)
+    if rc != 0:
+        _lib.check(rc, what)
 
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
+
+def _launch(fn, what, dev, *args):
+    """One library call on the current stream of dev (made current for it where it is not)."""
+    back, stream = _stream(dev)
+    _done(back, fn(*args, stream), what)
+
+
+def _twice(backward):
+    """Autograd formula of a Function whose backward has no derivative of its own: once_differentiable's
+    wrapping only where a caller asks for a graph of the backward (create_graph)."""
+    once = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(call)
 
 
 def _unit(t):
@@ -73,11 +89,22 @@ def _unit(t):
 
 
 def _heads(t):
-    return (t.data_ptr(), *t.stride()[:3])
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1], s[2]
 
 
 def _ws(nbytes, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+_LIB = None
+
+
+def _library():
+    global _LIB
+    if _LIB is None:
+        _LIB = _lib.load()
+    return _LIB
 
 
 # ------------------------------------------------------------------------------------------
@@ -85,67 +112,75 @@ def _ws(nbytes, dev):
 
 @functools.lru_cache(maxsize=512)
 def _cross_ws_bytes(dtype, B, Nq, Nk, H, Hk, D, backward):
-    n = _lib.load().mdg_attn_cross_workspace_bytes(_CROSS.pack(dtype, B, Nq, Nk, H, Hk, D, 0, 1.0, *([0] * 42)), backward)
+    n = _library().mdg_attn_cross_workspace_bytes(_CROSS.pack(dtype, B, Nq, Nk, H, Hk, D, 0, 1.0, *([0] * 42)), backward)
     if n == _lib.SIZE_MAX:
         _lib.check(1, "mdg_attn_cross_workspace_bytes")
     return n
 
 
-def _cross_call(backward, q, k, v, o, o_lo, lse, mask, q_len, kv_len, scale, dout=None, dq=None, dk=None, dv=None):
+def _cross_desc(q, k, v, o, side, mask, q_len, kv_len, scale, grads=_NO_HEADS * 4):
+    """side: (o_lo address or 0, lse address or 0); both contiguous as o [B, Nq, H, D] and [B, H, Nq]."""
     B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    dt = _DTYPES[q.dtype]
-    nbytes = _cross_ws_bytes(dt, B, Nq, Nk, H, Hk, D, backward)
+    o_lo, lse = side
+    return _CROSS.pack(_DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, 0 if mask is None else _MASKS[mask.dtype], scale,
+                       *_heads(q), *_heads(k), *_heads(v), *_heads(o), o_lo, Nq * H * D, H * D, D, *grads,
+                       0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(),
+                       *((0, 0, 0) if mask is None else (mask.data_ptr(), *mask.stride())), lse)
+
+
+def _cross_fwd(q, k, v, o, side, mask, q_len, kv_len, scale):
+    B, Nq, H, D = q.shape
+    nbytes = _cross_ws_bytes(_DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, 0)
     ws = _ws(nbytes, q.device)
-    grads = (_NO_HEADS * 4 if dout is None else
-             (*_heads(dout), *_heads(dq), *(_heads(dk) if dk is not None else _NO_HEADS),
-              *(_heads(dv) if dv is not None else _NO_HEADS)))
-    desc = _CROSS.pack(dt, B, Nq, Nk, H, Hk, D, 0 if mask is None else _MASKS[mask.dtype], scale,
-                       *_heads(q), *_heads(k), *_heads(v), *_heads(o), *(_heads(o_lo) if o_lo is not None else _NO_HEADS),
-                       *grads, 0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(),
-                       *((0, 0, 0) if mask is None else (mask.data_ptr(), *mask.stride())),
-                       0 if lse is None else lse.data_ptr())
-    lib = _lib.load()
-    with _On(q) as stream:
-        if backward:
-            _lib.check(lib.mdg_attn_cross_bwd(desc, _lib.ptr(ws), nbytes, stream), "mdg_attn_cross_bwd")
-        else:
-            _lib.check(lib.mdg_attn_cross_fwd(desc, _lib.ptr(ws), nbytes, stream), "mdg_attn_cross_fwd")
+    _launch(_library().mdg_attn_cross_fwd, "mdg_attn_cross_fwd", q.device,
+            _cross_desc(q, k, v, o, side, mask, q_len, kv_len, scale), _lib.ptr(ws), nbytes)
 
 
 class _CrossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, q_len, kv_len, scale):
         q, k, v = _unit(q), _unit(k), _unit(v)
-        B, Nq, H, _ = q.shape
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        o_lo = torch.empty_like(o) if q.dtype == torch.bfloat16 else None
-        lse = torch.empty(B, H, Nq, device=q.device)
-        if o.numel():
-            _cross_call(0, q, k, v, o, o_lo, lse, mask, q_len, kv_len, scale)
-        ctx.save_for_backward(q, k, v, o, o_lo, lse, mask, q_len, kv_len)
-        ctx.scale = scale
+        n, dev = q.numel(), q.device
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        # what the backward reads beside o, one allocation: lse [B, H, Nq] fp32, then bf16's o_lo as o
+        low = q.dtype == torch.bfloat16
+        rows = (n // q.shape[3] + 3) // 4 * 16  # bytes of lse, o_lo aligned behind it
+        side = torch.empty(rows + (2 * n if low else 0), dtype=torch.uint8, device=dev)
+        if n:
+            at = side.data_ptr()
+            _cross_fwd(q, k, v, o, (at + rows if low else 0, at), mask, q_len, kv_len, scale)
+        ctx.save_for_backward(q, k, v, o, mask, q_len, kv_len)
+        ctx.rest = side, rows if low else -1, scale
         return o
 
-    @staticmethod
-    @once_differentiable
+    @_twice
     def backward(ctx, dout):
-        q, k, v, o, o_lo, lse, mask, q_len, kv_len = ctx.saved_tensors
+        q, k, v, o, mask, q_len, kv_len = ctx.saved_tensors
+        side, low, scale = ctx.rest
         need = ctx.needs_input_grad
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dev = q.device
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
         dk = dv = None
         if need[1] or need[2]:  # (a frozen encoder leaves the key side's pass out)
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+            dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+            dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
         if q.numel():
-            _cross_call(1, q, k, v, o, o_lo, lse, mask, q_len, kv_len, ctx.scale, _unit(dout), dq, dk, dv)
+            dout = _unit(dout)
+            B, Nq, H, D = q.shape
+            nbytes = _cross_ws_bytes(_DTYPES[q.dtype], B, Nq, k.shape[1], H, k.shape[2], D, 1)
+            ws = _ws(nbytes, dev)
+            keys = _NO_HEADS * 2 if dk is None else (*_heads(dk), *_heads(dv))
+            at = side.data_ptr()
+            desc = _cross_desc(q, k, v, o, (at + low if low >= 0 else 0, at), mask, q_len, kv_len, scale,
+                               (*_heads(dout), *_heads(dq), *keys))
+            _launch(_library().mdg_attn_cross_bwd, "mdg_attn_cross_bwd", dev, desc, _lib.ptr(ws), nbytes)
         elif dk is not None:
             dk.zero_(), dv.zero_()
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def _check_len(name, t, B):
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
         raise ValueError(f"cross_attention: {name} must be a contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
 
 
@@ -158,23 +193,26 @@ def cross_attention(q, k, v, mask=None, q_len=None, kv_len=None, scale=None):
     too) and has gradient 0; a row without keys gives 0, and so do query rows past q_len.  scale
     defaults to D ** -0.5.  Accumulation and the softmax are fp32; with bf16 inputs the probabilities
     are rounded to bf16 before their product with v."""
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"cross_attention: {n} must be [B, N, heads, D], got {tuple(t.shape)}")
+    if not q.dim() == k.dim() == v.dim() == 4:
+        raise ValueError(f"cross_attention: q, k, v must be [B, N, heads, D], got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"cross_attention: q, k, v must be fp32 or bf16 of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hk == 0 or H % Hk or not 1 <= D <= 128:
+    kB, Nk, Hk, kD = k.shape
+    if k.shape != v.shape or kB != B or kD != D or Hk == 0 or H % Hk or not 1 <= D <= 128:
         raise ValueError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     _check_device(q, k, v, mask, q_len, kv_len)
     if mask is not None:
         if mask.dtype not in _MASKS or mask.dim() != 2 or mask.shape[1] != Nk or mask.shape[0] not in (1, B):
             raise ValueError(f"cross_attention: mask must be bool, uint8 or fp32 [{B} or 1, {Nk}], got {mask.dtype} "
                              f"{tuple(mask.shape)}")
-        mask = mask.expand(B, Nk)
-    _check_len("q_len", q_len, B)
-    _check_len("kv_len", kv_len, B)
+        if mask.shape[0] != B:
+            mask = mask.expand(B, Nk)
+    if q_len is not None:
+        _check_len("q_len", q_len, B)
+    if kv_len is not None:
+        _check_len("kv_len", kv_len, B)
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-18 <= scale <= 1e18:
         raise ValueError(f"cross_attention: scale {scale}")
@@ -183,7 +221,7 @@ def cross_attention(q, k, v, mask=None, q_len=None, kv_len=None, scale=None):
     q, k, v = _unit(q), _unit(k), _unit(v)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if o.numel():
-        _cross_call(0, q, k, v, o, None, None, mask, q_len, kv_len, scale)
+        _cross_fwd(q, k, v, o, (0, 0), mask, q_len, kv_len, scale)
     return o
 
 
@@ -234,8 +272,7 @@ def _rope_call(plan, pos, xs, outs, inverse):
                       inverse, xs[0].shape[2], xs[1].shape[2] if len(xs) > 1 else 0, *plan._sections8,
                       pos.data_ptr(), 0 if pos.shape[0] == 1 else pos.stride(0), pos.stride(1), plan.turns.data_ptr(),
                       plan.axis.data_ptr(), plan.cols.data_ptr(), *x[0], *x[1], *y[0], *y[1])
-    with _On(xs[0]) as stream:
-        _lib.check(_lib.load().mdg_rope_axes(desc, stream), "mdg_rope_axes")
+    _launch(_library().mdg_rope_axes, "mdg_rope_axes", xs[0].device, desc)
 
 
 def _rope_new(plan, pos, xs, inverse):
@@ -253,8 +290,7 @@ class _RopeFn(torch.autograd.Function):
         ctx.save_for_backward(pos)
         return tuple(_rope_new(plan, pos, xs, inverse))
 
-    @staticmethod
-    @once_differentiable
+    @_twice
     def backward(ctx, *gs):  # the rotation's transpose is the rotation by the negative angle
         (pos,) = ctx.saved_tensors
         return (None, None, None, *_rope_new(ctx.plan, pos, gs, 1 - ctx.inverse))
@@ -338,8 +374,7 @@ def _grn_fwd(cfg, h, y, mods, ws):
     xn = torch.empty(h.shape, dtype=cfg["ct"], device=h.device) if cfg["pre"] else None
     if h.numel():
         desc = _grn_desc(cfg, h2, y2, mods, ms, ws, (_lib.ptr(ho) or 0, _lib.ptr(xn) or 0))
-        with _On(h) as stream:
-            _lib.check(_lib.load().mdg_gate_res_norm(desc, stream), "mdg_gate_res_norm")
+        _launch(_library().mdg_gate_res_norm, "mdg_gate_res_norm", h.device, desc)
     return h2, y2, mods, ms, ho, xn
 
 
@@ -353,8 +388,7 @@ class _GrnFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return (h.view_as(h) if ho is None else ho), xn
 
-    @staticmethod
-    @once_differentiable
+    @_twice
     def backward(ctx, dho, dxn):
         h, y, gate, shift, scale, *ws = ctx.saved_tensors
         cfg, need = ctx.cfg, ctx.needs_input_grad[1:]
@@ -366,28 +400,25 @@ class _GrnFn(torch.autograd.Function):
         dxn = None if dxn is None else dxn.contiguous()
         dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if need[0] else None
         dy = torch.empty(ctx.shape, dtype=y.dtype, device=dev) if need[1] else None
-        fresh = torch.empty if h.numel() else torch.zeros  # (no rows: sums of nothing)
-        par = []
-        for i, t in enumerate((gate, shift, scale, *ws)):
-            side = i in (1, 2, 5, 6)  # the pre norm's parameters
-            if t is None or not need[2 + i]:
-                par.append(None)
-            elif side and dxn is None:
-                par.append(torch.zeros(t.shape, device=dev))
-            else:
-                par.append(fresh(t.shape, device=dev))
+        ins = (gate, shift, scale, *ws)
+        pre = (False, True, True, False, False, True, True)  # the pre norm's parameters: none without dxn
+        live = [need[2 + i] and not (pre[i] and dxn is None) and h.numel() > 0 for i in range(7)]
+        par = [None if live[i] or not need[2 + i] else torch.zeros(ins[i].shape, device=dev) for i in range(7)]
+        for part in (range(3), range(3, 7)):  # the rows' gradients in one allocation, the weights' in another
+            at = [i for i in part if live[i]]
+            if at:
+                for i, t in zip(at, torch.empty((len(at), *ins[at[0]].shape), device=dev).unbind(0)):
+                    par[i] = t
         if h.numel():
-            asked = [None if p is None or (i in (1, 2, 5, 6) and dxn is None) else p for i, p in enumerate(par)]
-            grads = [0 if t is None else t.data_ptr() for t in (dh, dy, *asked)]
+            grads = [0 if t is None else t.data_ptr() for t in (dh, dy)] + [par[i].data_ptr() if live[i] else 0 for i in range(7)]
             ptr0 = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
             desc = _grn_desc(cfg, h, y, (gate, shift, scale), ctx.ms, ws, (0, 0), (ptr0(dho), ptr0(dxn)), grads, C)
-            lib = _lib.load()
+            lib = _library()
             nbytes = lib.mdg_gate_res_norm_bwd_workspace_bytes(desc)
             if nbytes == _lib.SIZE_MAX:
                 _lib.check(1, "mdg_gate_res_norm_bwd_workspace_bytes")
             wsp = _ws(nbytes, dev)
-            with _On(h) as stream:
-                _lib.check(lib.mdg_gate_res_norm_bwd(desc, _lib.ptr(wsp), nbytes, stream), "mdg_gate_res_norm_bwd")
+            _launch(lib.mdg_gate_res_norm_bwd, "mdg_gate_res_norm_bwd", dev, desc, _lib.ptr(wsp), nbytes)
         return (None, dh, dy, *par)
 
 
