@@ -156,6 +156,7 @@ class _CrossFn(torch.autograd.Function):
     @_twice
     def backward(ctx, dout):
         q, k, v, o, mask, q_len, kv_len = ctx.saved_tensors
+        q, k, v, o = _unit(q), _unit(k), _unit(v), _unit(o)
         side, low, scale = ctx.rest
         need = ctx.needs_input_grad
         dev = q.device
@@ -260,19 +261,22 @@ class RopeAxes:
         self.turns = (freq / (2.0 * math.pi)).to(device)
         self.axis = torch.tensor([a for a, s in enumerate(sections) for _ in range(s)], dtype=torch.int32).to(device)
         self.cols = torch.tensor(first + second, dtype=torch.int32).to(device)
-        self._head = (n, len(sections))
+        self._code = _PAIRS[pairs]
         self._sections8 = tuple(sections + [0] * (_lib.MDG_ROPE_MAX_AXES - len(sections)))
 
 
 def _rope_call(plan, pos, xs, outs, inverse):
-    B, N, _, D = xs[0].shape
-    x = [_heads(t) for t in xs] + [_NO_HEADS] * (2 - len(xs))
-    y = [_heads(t) for t in outs] + [_NO_HEADS] * (2 - len(xs))
-    desc = _ROPE.pack(_DTYPES[xs[0].dtype], _PAIRS[plan.pairs], len(xs), B, N, D, *plan._head, pos.dtype == torch.int64,
-                      inverse, xs[0].shape[2], xs[1].shape[2] if len(xs) > 1 else 0, *plan._sections8,
-                      pos.data_ptr(), 0 if pos.shape[0] == 1 else pos.stride(0), pos.stride(1), plan.turns.data_ptr(),
-                      plan.axis.data_ptr(), plan.cols.data_ptr(), *x[0], *x[1], *y[0], *y[1])
-    _launch(_library().mdg_rope_axes, "mdg_rope_axes", xs[0].device, desc)
+    q, o = xs[0], outs[0]
+    B, N, H, D = q.shape
+    if len(xs) == 2:
+        H2, k2, o2 = xs[1].shape[2], _heads(xs[1]), _heads(outs[1])
+    else:
+        H2, k2, o2 = 0, _NO_HEADS, _NO_HEADS
+    ps = pos.stride()
+    desc = _ROPE.pack(_DTYPES[q.dtype], plan._code, len(xs), B, N, D, plan.npairs, len(plan.sections), pos.dtype == torch.int64,
+                      inverse, H, H2, *plan._sections8, pos.data_ptr(), 0 if pos.shape[0] == 1 else ps[0], ps[1],
+                      plan.turns.data_ptr(), plan.axis.data_ptr(), plan.cols.data_ptr(), *_heads(q), *k2, *_heads(o), *o2)
+    _launch(_library().mdg_rope_axes, "mdg_rope_axes", q.device, desc)
 
 
 def _rope_new(plan, pos, xs, inverse):
@@ -305,8 +309,9 @@ def rope_axes(plan, pos, q, k=None, inverse=False, inplace=False):
         if t.dim() != 4 or t.dtype not in _DTYPES or t.dtype != q.dtype:
             raise TypeError(f"rope_axes: tensors must be fp32 or bf16 [B, N, heads, D] of one type, got {t.dtype} "
                             f"{tuple(t.shape)}")
-        if t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3] or not 1 <= t.shape[2] <= 1024:
-            raise ValueError(f"rope_axes: q {tuple(q.shape)}, k {tuple(t.shape)}")
+        s = t.shape
+        if s[0] != q.shape[0] or s[1] != q.shape[1] or s[3] != q.shape[3] or not 1 <= s[2] <= 1024:
+            raise ValueError(f"rope_axes: q {tuple(q.shape)}, k {tuple(s)}")
     B, N, _, D = q.shape
     if 2 * plan.npairs > D:
         raise ValueError(f"rope_axes: {plan.npairs} pairs in a head of {D}")
@@ -315,8 +320,8 @@ def rope_axes(plan, pos, q, k=None, inverse=False, inplace=False):
         raise TypeError(f"rope_axes: pos must be int32 or int64, got {pos.dtype}")
     if pos.dim() == 2:
         pos = pos[None]
-    if pos.dim() != 3 or pos.shape[0] not in (1, B) or tuple(pos.shape[1:]) != (N, plan._head[1]):
-        raise ValueError(f"rope_axes: pos {tuple(pos.shape)} for tokens [{B}, {N}] on {plan._head[1]} axes")
+    if pos.dim() != 3 or pos.shape[0] not in (1, B) or pos.shape[1] != N or pos.shape[2] != len(plan.sections):
+        raise ValueError(f"rope_axes: pos {tuple(pos.shape)} for tokens [{B}, {N}] on {len(plan.sections)} axes")
     pos = _unit(pos)
     inverse = int(bool(inverse))
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in xs)
@@ -338,64 +343,69 @@ def rope_axes(plan, pos, q, k=None, inverse=False, inplace=False):
 # the norms around a block, its gate and residual scale
 
 def _rows2d(t, C):
+    """(t as rows [M, C] with a contiguous last dim, their stride)."""
+    if t.is_contiguous():
+        return t, C
     t = t.reshape(-1, C)
-    return t if (t.stride(1) == 1 or C == 1) and (t.stride(0) >= C or t.shape[0] == 1) else t.contiguous()
+    if (t.stride(1) == 1 or C == 1) and (t.stride(0) >= C or t.shape[0] == 1):
+        return t, (t.stride(0) if t.shape[0] > 1 else C)
+    return t.contiguous(), C
 
 
-def _ld(t, C):
-    return t.stride(0) if t.shape[0] > 1 else C
+def _same_rows(gate, shift, scale):
+    """gate / shift / scale with one common row stride (copied where they differ), and that stride."""
+    some = gate if gate is not None else shift if shift is not None else scale
+    if some is None:
+        return gate, shift, scale, 0
+    st, C = some.stride(), some.shape[1]
+    if (st[1] == 1 or C == 1) and st[0] >= C and (shift is None or shift.stride() == st) and (
+            scale is None or scale.stride() == st):
+        return gate, shift, scale, st[0]
+    return (*(None if t is None else t.contiguous() for t in (gate, shift, scale)), C)
 
 
-def _same_rows(mods):
-    """gate / shift / scale with one common row stride (copied where they differ)."""
-    have = [t for t in mods if t is not None]
-    if not have:
-        return mods, 0
-    ok = all((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) == have[0].stride(0) >= t.shape[1] for t in have)
-    if not ok:
-        mods = [None if t is None else t.contiguous() for t in mods]
-        have = [t for t in mods if t is not None]
-    return mods, (have[0].stride(0) if have[0].shape[0] > 1 else have[0].shape[1])
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
-def _grn_desc(cfg, h, y, mods, mod_stride, ws, out, grads_in=(0, 0), grads=(0,) * 9, dmod_stride=0):
-    M, C = h.shape
-    ptrs = [0 if t is None else t.data_ptr() for t in (*mods, *ws)]
-    return _GRN.pack(_DTYPES[cfg["ct"]], _DTYPES[h.dtype], M, C, cfg["R"], cfg["post"], cfg["pre"], cfg["rs"], cfg["eps"],
-                     h.data_ptr(), 0 if y is None else y.data_ptr(), _ld(h, C), 0 if y is None else _ld(y, C), *ptrs[:3],
-                     mod_stride, *ptrs[3:], *out, *grads_in, *grads[:5], dmod_stride, *grads[5:])
-
-
-def _grn_fwd(cfg, h, y, mods, ws):
+def _grn_ins(cfg, h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b):
+    """The inputs' part of the descriptor, and the tensors that it points into.  cfg: (dtype code of y, of h,
+    rows per group, post, pre, resid_scale, eps, type of xn)."""
     C = h.shape[-1]
-    h2, y2 = _rows2d(h, C), None if y is None else _rows2d(y, C)
-    mods, ms = _same_rows(mods)
-    ho = None if y is None and cfg["rs"] == 1.0 and cfg["pre"] else torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    xn = torch.empty(h.shape, dtype=cfg["ct"], device=h.device) if cfg["pre"] else None
+    h, ldh = _rows2d(h, C)
+    y, ldy = (None, 0) if y is None else _rows2d(y, C)
+    gate, shift, scale, ms = _same_rows(gate, shift, scale)
+    return (cfg[0], cfg[1], h.numel() // C, C, *cfg[2:7], h.data_ptr(), _ptr(y), ldh, ldy, _ptr(gate), _ptr(shift), _ptr(scale),
+            ms, _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b)), (h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
+
+
+def _grn_fwd(cfg, h, y, *par):
+    head, ins = _grn_ins(cfg, h, y, *par)
+    ho = None if y is None and cfg[5] == 1.0 and cfg[4] else torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    xn = torch.empty(h.shape, dtype=cfg[7], device=h.device) if cfg[4] else None
     if h.numel():
-        desc = _grn_desc(cfg, h2, y2, mods, ms, ws, (_lib.ptr(ho) or 0, _lib.ptr(xn) or 0))
+        desc = _GRN.pack(*head, _ptr(ho), _ptr(xn), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         _launch(_library().mdg_gate_res_norm, "mdg_gate_res_norm", h.device, desc)
-    return h2, y2, mods, ms, ho, xn
+    return ins, ho, xn
 
 
 class _GrnFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, cfg, h, y, gate, shift, scale, *ws):
-        h2, y2, mods, ms, ho, xn = _grn_fwd(cfg, h, y, [gate, shift, scale], ws)
-        ctx.save_for_backward(h2, y2, *mods, *ws)
-        ctx.cfg, ctx.ms, ctx.shape = cfg, ms, h.shape
-        ctx.passed = ho is None  # h itself goes on
+    def forward(ctx, cfg, h, y, *par):
+        ins, ho, xn = _grn_fwd(cfg, h, y, *par)
+        ctx.save_for_backward(*ins)
+        ctx.cfg, ctx.shape = cfg, h.shape
         ctx.set_materialize_grads(False)
-        return (h.view_as(h) if ho is None else ho), xn
+        return (h.view_as(h) if ho is None else ho), xn  # (without y, h itself goes on)
 
     @_twice
     def backward(ctx, dho, dxn):
-        h, y, gate, shift, scale, *ws = ctx.saved_tensors
-        cfg, need = ctx.cfg, ctx.needs_input_grad[1:]
+        need = ctx.needs_input_grad[1:]
         if dho is None and dxn is None:
-            return (None,) * (6 + len(ws))
-        C = h.shape[1]
-        dev = h.device
+            return (None,) * 10
+        head, saved = _grn_ins(ctx.cfg, *ctx.saved_tensors)
+        h, y, gate, shift, scale, *ws = saved
+        C, dev = h.shape[-1], h.device
         dho = None if dho is None else dho.contiguous()
         dxn = None if dxn is None else dxn.contiguous()
         dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if need[0] else None
@@ -410,9 +420,8 @@ class _GrnFn(torch.autograd.Function):
                 for i, t in zip(at, torch.empty((len(at), *ins[at[0]].shape), device=dev).unbind(0)):
                     par[i] = t
         if h.numel():
-            grads = [0 if t is None else t.data_ptr() for t in (dh, dy)] + [par[i].data_ptr() if live[i] else 0 for i in range(7)]
-            ptr0 = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-            desc = _grn_desc(cfg, h, y, (gate, shift, scale), ctx.ms, ws, (0, 0), (ptr0(dho), ptr0(dxn)), grads, C)
+            at = [par[i].data_ptr() if live[i] else 0 for i in range(7)]
+            desc = _GRN.pack(*head, 0, 0, _ptr(dho), _ptr(dxn), _ptr(dh), _ptr(dy), *at[:3], C, *at[3:])
             lib = _library()
             nbytes = lib.mdg_gate_res_norm_bwd_workspace_bytes(desc)
             if nbytes == _lib.SIZE_MAX:
@@ -451,26 +460,29 @@ def gate_residual_norm(h, y=None, gate=None, shift=None, scale=None, resid_scale
     if pre == "none" and any(t is not None for t in (pre_w, pre_b, shift, scale)):
         raise ValueError("gate_residual_norm: pre weights or modulation without a pre norm")
     _check_device(h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
-    M, G = h.numel() // C, None
-    for n, t in (("gate", gate), ("shift", shift), ("scale", scale)):
-        if t is None:
-            continue
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != C or (G is not None and t.shape[0] != G):
-            raise ValueError(f"gate_residual_norm: {n} must be fp32 [G, {C}], got {t.dtype} {tuple(t.shape)}")
-        G = t.shape[0]
-    G = 1 if G is None else G
-    if G < 1 or M % G or (M == 0 and G > 1 and h.shape[0] != G):
+    M, G = h.numel() // C, 0
+    for t in (gate, shift, scale):
+        if t is not None:
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != C or (G and t.shape[0] != G):
+                raise ValueError(f"gate_residual_norm: gate, shift and scale must be fp32 [G, {C}], got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+            G = t.shape[0]
+            if not G:
+                raise ValueError("gate_residual_norm: gate, shift or scale without rows")
+    G = G or 1
+    if M % G or (M == 0 and G > 1 and h.shape[0] != G):
         raise ValueError(f"gate_residual_norm: {M} rows in {G} groups")
-    for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()):
-            raise ValueError(f"gate_residual_norm: {n} must be a contiguous fp32 [{C}], got {t.dtype} {tuple(t.shape)}")
+    for t in (post_w, post_b, pre_w, pre_b):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != C or not t.is_contiguous()):
+            raise ValueError(f"gate_residual_norm: weights must be contiguous fp32 [{C}], got {t.dtype} {tuple(t.shape)}")
     eps, rs = float(eps), float(resid_scale)
     if not (0.0 <= eps < math.inf and math.isfinite(rs)):
         raise ValueError(f"gate_residual_norm: eps {eps}, resid_scale {rs}")
-    cfg = {"ct": h.dtype if y is None else y.dtype, "R": max(M // G, 1), "post": _NORMS[post], "pre": _NORMS[pre],
-           "rs": rs, "eps": eps}
-    ins = (h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
-        return _GrnFn.apply(cfg, *ins)
-    *_, ho, xn = _grn_fwd(cfg, h, y, [gate, shift, scale], ins[5:])
+    ct = h.dtype if y is None else y.dtype
+    cfg = (_DTYPES[ct], _DTYPES[h.dtype], M // G or 1, _NORMS[post], _NORMS[pre], rs, eps, ct)
+    if torch.is_grad_enabled():
+        for t in (h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b):
+            if t is not None and t.requires_grad:
+                return _GrnFn.apply(cfg, h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
+    _, ho, xn = _grn_fwd(cfg, h, y, gate, shift, scale, post_w, post_b, pre_w, pre_b)
     return (h if ho is None else ho), xn
