@@ -700,7 +700,7 @@ int mdg_attn_cross_bwd(const mdg_attn_cross* a, void* ws, size_t ws_bytes, void*
    MDG_ROPE_AXIS (halves within each axis's own section; section[a] = that axis's pairs, their sum
    npairs).  cols, axis and turns are device tables [2 npairs], [npairs], [npairs].  pos: int32 or int64
    (pos_i64) [B][N][naxes], element strides pos_sb (0: shared) and pos_sn.  nseg 1 or 2 tensors x[i]
-   [B][N][H[i]][D] -> out[i] (may be x[i] itself).  inverse 1: the transposed rotation, the backward. */
+   [B][N][H[i]][D] -> out[i] (may be x[i] itself), D <= 1024, H[i] <= 1024, B N < 2^31.  inverse 1: the transposed rotation, the backward. */
 enum { MDG_ROPE_HALF = 0, MDG_ROPE_INTERLEAVED = 1, MDG_ROPE_AXIS = 2 };
 #define MDG_ROPE_MAX_AXES 8
 typedef struct {

@@ -313,7 +313,7 @@ def rope_axes(plan, pos, q, k=None, inverse=False, inplace=False):
         if s[0] != q.shape[0] or s[1] != q.shape[1] or s[3] != q.shape[3] or not 1 <= s[2] <= 1024:
             raise ValueError(f"rope_axes: q {tuple(q.shape)}, k {tuple(s)}")
     B, N, _, D = q.shape
-    if 2 * plan.npairs > D:
+    if 2 * plan.npairs > D or D > 1024:
         raise ValueError(f"rope_axes: {plan.npairs} pairs in a head of {D}")
     _check_device(q, k, pos, plan.turns)
     if pos.dtype not in (torch.int32, torch.int64):

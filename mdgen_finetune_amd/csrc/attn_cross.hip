@@ -185,8 +185,6 @@ __device__ __forceinline__ bool key_kept(const CrossP& p, int b, int key) {
                     : reinterpret_cast<const unsigned char*>(p.mask)[i] != 0;
 }
 
-__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 
 // The softmax of one 32-key tile: raises the lane's maximum when a score outgrows it by 2^8 (a lagging
 // maximum costs no precision: P is floating point and stays below 2^8, sums are fp32), turns the
@@ -201,7 +199,7 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NT], f32x16 (&o)[DT], f
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-  mx = half_max(mx);
+  mx = other_half_max(mx);
   if (__any(mx > m + grow)) {
     const float nm = mx > m + grow ? mx : m;
     const float alpha = m == kNoMax ? 0.f : __builtin_amdgcn_exp2f((m - nm) * c);
@@ -551,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     __syncthreads();
   }
 
-  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, kOnes ? o[NO - 1][0] : half_sum(l), lane);
+  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, kOnes ? o[NO - 1][0] : other_half_sum(l), lane);
 }
 
 // The same with two groups of four waves (256 rows per block), one phase apart, each SIMD holding one wave
@@ -627,7 +625,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
     __syncthreads();
   }
   if (!second) __syncthreads();
-  store_rows<CT, DP, true>(p, id, r, rows, live, o, m, half_sum(l), lane);
+  store_rows<CT, DP, true>(p, id, r, rows, live, o, m, other_half_sum(l), lane);
 }
 
 // At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
@@ -702,10 +700,12 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if constexpr (BUFS == 2) cur ^= 1;
   }
-  l = half_sum(l);
+  l = other_half_sum(l);
 
   // join: [4][32] maxima and sums, then the rescaled outputs [4][32][DP + 4] over the staging area
-  __syncthreads();
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last tile's reads are done
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   float* jm = reinterpret_cast<float*>(smem);
   float* jl = jm + 128;
   float* js = jl + 128;  // [32] the rows' joined sums
@@ -843,7 +843,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
       for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[ks][j], (float)of[j], delta);
     }
   }
-  delta = half_sum(delta);
+  delta = other_half_sum(delta);
   float lse = live ? p.lse[srow] : -INFINITY;
   if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every P is 0
   if (p.delta && id.split == 0 && r < rows && h == 0) p.delta[((long long)id.b * p.H + head) * p.Nq + n] = delta;

@@ -133,7 +133,6 @@ hipError_t adam_step_launch(int nt, int nc, const void* table, double lr, double
 size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back);
 bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back);
 hipError_t attn_cross_launch(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s);
-bool rope_axes_grid_ok(const mdg_rope_axes_desc& d);
 hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s);
 size_t gate_res_norm_ws_bytes(const mdg_gate_res_norm_desc& d);
 hipError_t gate_res_norm_fwd_launch(const mdg_gate_res_norm_desc& d, hipStream_t s);
@@ -1739,7 +1738,8 @@ int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream) {
   if (d->B <= 0 || d->N <= 0 || d->D <= 0 || d->npairs <= 0 || d->npairs > d->D / 2 || d->naxes < 1 ||
       d->naxes > MDG_ROPE_MAX_AXES || d->nseg < 1 || d->nseg > 2)
     return fail(MDG_E_SHAPE, "rope_axes: B=%d N=%d D=%d npairs=%d naxes=%d nseg=%d", d->B, d->N, d->D, d->npairs, d->naxes, d->nseg);
-  if ((double)d->B * d->N * d->D > 1e15) return fail(MDG_E_SHAPE, "rope_axes: grid too large");
+  if ((int64_t)d->B * d->N > INT32_MAX || d->D > 1024)
+    return fail(MDG_E_SHAPE, "rope_axes: D=%d (at most 1024) or grid too large", d->D);
   int sum = 0;
   for (int a = 0; a < d->naxes; ++a) {
     if (d->section[a] < 0 || d->section[a] > d->npairs) return fail(MDG_E_SHAPE, "rope_axes: section %d", d->section[a]);
@@ -1759,7 +1759,6 @@ int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream) {
     if (d->x[i].p == d->out[i].p && (d->x[i].sb != d->out[i].sb || d->x[i].sn != d->out[i].sn || d->x[i].sh != d->out[i].sh))
       return fail(MDG_E_ARG, "rope_axes: in place needs out's strides equal to x's");
   }
-  if (!mdg::rope_axes_grid_ok(*d)) return fail(MDG_E_SHAPE, "rope_axes: grid too large");
   return hip_check(mdg::rope_axes_launch(*d, (hipStream_t)stream), "rope_axes");
 }
 

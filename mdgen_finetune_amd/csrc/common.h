@@ -108,6 +108,49 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// Sum over every aligned group of W = 16, 32 or 64 lanes, in each of them, on the vector unit alone
+// (lane permutations within rows of 16, then swaps of rows and halves; wave_sum's shuffles go
+// through LDS, ~100 cycles a step).  The group's lanes must all be active.
+template <int CTRL>
+__device__ __forceinline__ float row_perm(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// (x, y) with the odd rows of 16 lanes (or the wave's upper half) of x and the even rows (the lower half)
+// of y exchanged, for x = y = v.  In assembly: this compiler's builtins return the first register
+// twice.  Two wait states cover the inputs' writes.
+__device__ __forceinline__ float2 swap_rows(float v) {
+  float x = v, y = v;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return make_float2(x, y);
+}
+__device__ __forceinline__ float2 swap_halves(float v) {
+  float x = v, y = v;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return make_float2(x, y);
+}
+// of lane l and lane l ^ 32
+__device__ __forceinline__ float other_half_sum(float v) {
+  const float2 r = swap_halves(v);
+  return r.x + r.y;
+}
+__device__ __forceinline__ float other_half_max(float v) {
+  const float2 r = swap_halves(v);
+  return fmaxf(r.x, r.y);
+}
+template <int W>
+__device__ __forceinline__ float lane_sum(float v) {
+  v += row_perm<0xB1>(v);   // lane ^ 1
+  v += row_perm<0x4E>(v);   // lane ^ 2
+  v += row_perm<0x141>(v);  // mirrored within 8
+  v += row_perm<0x140>(v);  // mirrored within 16
+  if constexpr (W >= 32) {
+    const float2 r = swap_rows(v);
+    v = r.x + r.y;
+  }
+  if constexpr (W >= 64) v = other_half_sum(v);
+  return v;
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));

@@ -87,9 +87,7 @@ struct Red {
 template <int TPR, int N>
 __device__ __forceinline__ void team_sum(float (&v)[N], Red& rd) {
 #pragma unroll
-  for (int o = (TPR < 64 ? TPR : 64) / 2; o >= 1; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  for (int i = 0; i < N; ++i) v[i] = lane_sum<(TPR < 64 ? TPR : 64)>(v[i]);
   if constexpr (TPR >= 256) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float* red = rd.at + rd.turn * 32;
@@ -107,35 +105,47 @@ __device__ __forceinline__ void team_sum(float (&v)[N], Red& rd) {
   }
 }
 
-// x <- normalised x; returns 1 / std.  Columns past C hold 0 and stay 0.
-template <int TPR, int NV, int V>
-__device__ __forceinline__ float normalise(float (&x)[NV][V], int kind, float eps, float invC, const bool (&in)[NV],
-                                           Red& red) {
+// ROWS rows of a team at once: x <- normalised x, r <- 1 / std.  Columns past C hold 0 and stay 0.
+template <int TPR, int ROWS, int NV, int V>
+__device__ __forceinline__ void normalise(float (&x)[ROWS][NV][V], float (&r)[ROWS], int kind, float eps, float invC,
+                                          const bool (&in)[NV], Red& red) {
   if (kind == MDG_NORM_LAYER) {
-    float s[1] = {0.f};
+    float s[ROWS];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int w = 0; w < ROWS; ++w) {
+      s[w] = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += x[k][i];
-    team_sum<TPR, 1>(s, red);
-    const float mean = s[0] * invC;
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+        for (int i = 0; i < V; ++i) s[w] += x[w][k][i];
+    }
+    team_sum<TPR, ROWS>(s, red);
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = in[k] ? x[k][i] - mean : 0.f;
+    for (int w = 0; w < ROWS; ++w) {
+      const float mean = s[w] * invC;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[w][k][i] = in[k] ? x[w][k][i] - mean : 0.f;
+    }
   }
-  float q[1] = {0.f};
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int w = 0; w < ROWS; ++w) {
+    r[w] = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) q[0] = fmaf(x[k][i], x[k][i], q[0]);
-  team_sum<TPR, 1>(q, red);
-  const float r = 1.0f / sqrtf(fmaf(q[0], invC, eps));
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+      for (int i = 0; i < V; ++i) r[w] = fmaf(x[w][k][i], x[w][k][i], r[w]);
+  }
+  team_sum<TPR, ROWS>(r, red);
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[k][i] *= r;
-  return r;
+  for (int w = 0; w < ROWS; ++w) {
+    r[w] = 1.0f / sqrtf(fmaf(r[w], invC, eps));
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[w][k][i] *= r[w];
+  }
 }
 
 // g <- r (g - [mean(g)] - n mean(g n)): the gradient of the row before its norm.  Columns past C stay 0.
@@ -165,60 +175,78 @@ __device__ __forceinline__ void ldopt(const float* p, long long at, float dflt, 
   }
 }
 
-template <typename RT, typename CT, int V, int TPR, int NV>
+// ROWS consecutive rows per team: the parameters' rows (up to seven of them, fp32, from L2) are read
+// once for all that share them, which bounds wide rows, and a block's sums share their barriers.
+template <typename RT, typename CT, int V, int TPR, int NV, int ROWS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void grn_fwd_kernel(const GrnP p) {
   __shared__ float red_[64];
   Red red{red_, 0};
   constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
   const int team = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const int row = blockIdx.x * TEAMS + team;
-  if (TPR < 256 && row >= p.M) return;
-  const long long mo = (long long)(row / p.R) * p.mod_stride;
-  float h[NV][V], y[NV][V];
+  const int row0 = (blockIdx.x * TEAMS + team) * ROWS;
+  if (TPR < 256 && row0 >= p.M) return;
+  float h[ROWS][NV][V], y[ROWS][NV][V], r[ROWS];
+  long long mo[ROWS];
   bool in[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (t + k * TPR) * V;
-    in[k] = c < p.C;
+  for (int k = 0; k < NV; ++k) in[k] = (t + k * TPR) * V < p.C;
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[k][i] = y[k][i] = 0.f;
-    if (in[k]) {
-      ldv<RT, V>(reinterpret_cast<const RT*>(p.h) + row * p.ldh + c, h[k]);
-      if (p.y) ldv<CT, V>(reinterpret_cast<const CT*>(p.y) + row * p.ldy + c, y[k]);
+  for (int w = 0; w < ROWS; ++w) {
+    const int row = min(row0 + w, p.M - 1);  // (past the last row: the last one, not stored)
+    mo[w] = (long long)(row / p.R) * p.mod_stride;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (t + k * TPR) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[w][k][i] = y[w][k][i] = 0.f;
+      if (in[k]) {
+        ldv<RT, V>(reinterpret_cast<const RT*>(p.h) + row * p.ldh + c, h[w][k]);
+        if (p.y) ldv<CT, V>(reinterpret_cast<const CT*>(p.y) + row * p.ldy + c, y[w][k]);
+      }
     }
   }
-  if (p.post != MDG_NORM_NONE) normalise<TPR, NV, V>(y, p.post, p.eps, p.invC, in, red);
+  if (p.post != MDG_NORM_NONE) normalise<TPR, ROWS, NV, V>(y, r, p.post, p.eps, p.invC, in, red);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (t + k * TPR) * V;
     if (!in[k]) continue;
+    float wt[V], b[V], g[V];
     if (p.y) {
-      float w[V], b[V], g[V];
-      ldopt<V>(p.w1, c, 1.f, w);
+      ldopt<V>(p.w1, c, 1.f, wt);
       ldopt<V>(p.b1, c, 0.f, b);
-      ldopt<V>(p.gate, mo + c, 1.f, g);
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = fmaf(g[i], fmaf(y[k][i], w[i], b[i]), p.rs * h[k][i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] *= p.rs;
     }
-    if (p.ho) stv<RT, V>(reinterpret_cast<RT*>(p.ho) + (long long)row * p.C + c, h[k]);
+#pragma unroll
+    for (int w = 0; w < ROWS; ++w) {
+      if (p.y) {
+        if (w == 0 || mo[w] != mo[w - 1]) ldopt<V>(p.gate, mo[w] + c, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[w][k][i] = fmaf(g[i], fmaf(y[w][k][i], wt[i], b[i]), p.rs * h[w][k][i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[w][k][i] *= p.rs;
+      }
+      if (p.ho && row0 + w < p.M) stv<RT, V>(reinterpret_cast<RT*>(p.ho) + (long long)(row0 + w) * p.C + c, h[w][k]);
+    }
   }
   if (p.pre == MDG_NORM_NONE) return;
-  normalise<TPR, NV, V>(h, p.pre, p.eps, p.invC, in, red);
+  normalise<TPR, ROWS, NV, V>(h, r, p.pre, p.eps, p.invC, in, red);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (t + k * TPR) * V;
     if (!in[k]) continue;
-    float w[V], b[V], sc[V], sh[V], o[V];
-    ldopt<V>(p.w2, c, 1.f, w);
+    float wt[V], b[V], sc[V], sh[V], o[V];
+    ldopt<V>(p.w2, c, 1.f, wt);
     ldopt<V>(p.b2, c, 0.f, b);
-    ldopt<V>(p.scale, mo + c, 0.f, sc);
-    ldopt<V>(p.shift, mo + c, 0.f, sh);
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = fmaf(fmaf(h[k][i], w[i], b[i]), 1.0f + sc[i], sh[i]);
-    stv<CT, V>(reinterpret_cast<CT*>(p.xn) + (long long)row * p.C + c, o);
+    for (int w = 0; w < ROWS; ++w) {
+      if (w == 0 || mo[w] != mo[w - 1]) {
+        ldopt<V>(p.scale, mo[w] + c, 0.f, sc);
+        ldopt<V>(p.shift, mo[w] + c, 0.f, sh);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fmaf(fmaf(h[w][k][i], wt[i], b[i]), 1.0f + sc[i], sh[i]);
+      if (row0 + w < p.M) stv<CT, V>(reinterpret_cast<CT*>(p.xn) + (long long)(row0 + w) * p.C + c, o);
+    }
   }
 }
 
@@ -242,62 +270,61 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void grn_bwd_kernel(const Gr
 #pragma unroll
       for (int i = 0; i < V; ++i) S[s][k][i] = 0.f;
   bool in[NV];
+  // the group's rows of parameters: gate w1, gate b1, (1 + scale) w2
+  float gw[NV][V], gb[NV][V], sw[NV][V];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) in[k] = (t + k * TPR) * V < p.C;
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t + k * TPR) * V;
+    in[k] = c < p.C;
+#pragma unroll
+    for (int i = 0; i < V; ++i) gw[k][i] = gb[k][i] = sw[k][i] = 0.f;
+    if (in[k]) {
+      float g[V], w2[V], sc[V];
+      ldopt<V>(p.gate, mo + c, 1.f, g);
+      ldopt<V>(p.w1, c, 1.f, gw[k]);
+      ldopt<V>(p.b1, c, 0.f, gb[k]);
+      ldopt<V>(p.w2, c, 1.f, w2);
+      ldopt<V>(p.scale, mo + c, 0.f, sc);
+#pragma unroll
+      for (int i = 0; i < V; ++i) gw[k][i] *= g[i], gb[k][i] *= g[i], sw[k][i] = (1.0f + sc[i]) * w2[i];
+    }
+  }
 
   // every team of the block makes the same number of turns (the sums of a whole block hold barriers)
   for (int rb = r0; rb < r1; rb += TEAMS) {
     const int row = rb + team;
     if (TPR < 256 && row >= r1) break;
-    float h[NV][V], y[NV][V], g[NV][V];
+    float h[1][NV][V], y[1][NV][V], g[NV][V], a[NV][V], r1y[1], r2[1];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (t + k * TPR) * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = y[k][i] = g[k][i] = 0.f;
+      for (int i = 0; i < V; ++i) h[0][k][i] = y[0][k][i] = g[k][i] = a[k][i] = 0.f;
       if (in[k]) {
-        if (p.dxn) ldv<RT, V>(reinterpret_cast<const RT*>(p.h) + row * p.ldh + c, h[k]);
-        if (p.y) ldv<CT, V>(reinterpret_cast<const CT*>(p.y) + row * p.ldy + c, y[k]);
+        if (p.dxn) ldv<RT, V>(reinterpret_cast<const RT*>(p.h) + row * p.ldh + c, h[0][k]);
+        if (p.y) ldv<CT, V>(reinterpret_cast<const CT*>(p.y) + row * p.ldy + c, y[0][k]);
+        if (p.dxn) ldv<CT, V>(reinterpret_cast<const CT*>(p.dxn) + (long long)row * p.C + c, a[k]);
         if (p.dho) ldv<RT, V>(reinterpret_cast<const RT*>(p.dho) + (long long)row * p.C + c, g[k]);
       }
     }
-    float r1y = 1.f;
-    if (p.post != MDG_NORM_NONE) r1y = normalise<TPR, NV, V>(y, p.post, p.eps, p.invC, in, red);  // y is n1
+    r1y[0] = 1.f;
+    if (p.post != MDG_NORM_NONE) normalise<TPR, 1, NV, V>(y, r1y, p.post, p.eps, p.invC, in, red);  // y is n1
     if (p.dxn) {
-      float a[NV][V];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (t + k * TPR) * V;
-        if (!in[k]) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) a[k][i] = 0.f;
-          continue;
-        }
-        float w[V], b[V], gt[V];
-        ldopt<V>(p.w1, c, 1.f, w);
-        ldopt<V>(p.b1, c, 0.f, b);
-        ldopt<V>(p.gate, mo + c, 1.f, gt);
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          h[k][i] = p.y ? fmaf(gt[i], fmaf(y[k][i], w[i], b[i]), p.rs * h[k][i]) : p.rs * h[k][i];
-        ldv<CT, V>(reinterpret_cast<const CT*>(p.dxn) + (long long)row * p.C + c, a[k]);
-      }
-      const float r2 = normalise<TPR, NV, V>(h, p.pre, p.eps, p.invC, in, red);  // h is n2
+          h[0][k][i] = p.y ? fmaf(y[0][k][i], gw[k][i], fmaf(p.rs, h[0][k][i], gb[k][i])) : p.rs * h[0][k][i];
+      normalise<TPR, 1, NV, V>(h, r2, p.pre, p.eps, p.invC, in, red);  // h is n2
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (t + k * TPR) * V;
-        if (!in[k]) continue;
-        float w[V], sc[V];
-        ldopt<V>(p.w2, c, 1.f, w);
-        ldopt<V>(p.scale, mo + c, 0.f, sc);
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           S[0][k][i] += a[k][i];
-          S[1][k][i] = fmaf(a[k][i], h[k][i], S[1][k][i]);
-          a[k][i] *= (1.0f + sc[i]) * w[i];
+          S[1][k][i] = fmaf(a[k][i], h[0][k][i], S[1][k][i]);
+          a[k][i] *= sw[k][i];
         }
-      }
-      normalise_bwd<TPR, NV, V>(a, h, r2, p.pre, p.invC, in, red);
+      normalise_bwd<TPR, NV, V>(a, h[0], r2[0], p.pre, p.invC, in, red);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -315,21 +342,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void grn_bwd_kernel(const Gr
     }
     if (!p.y) continue;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (t + k * TPR) * V;
-      if (!in[k]) continue;
-      float w[V], gt[V];
-      ldopt<V>(p.w1, c, 1.f, w);
-      ldopt<V>(p.gate, mo + c, 1.f, gt);
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         S[2][k][i] += g[k][i];
-        S[3][k][i] = fmaf(g[k][i], y[k][i], S[3][k][i]);
-        g[k][i] *= gt[i] * w[i];
+        S[3][k][i] = fmaf(g[k][i], y[0][k][i], S[3][k][i]);
+        g[k][i] *= gw[k][i];
       }
-    }
     if (!p.dy) continue;
-    if (p.post != MDG_NORM_NONE) normalise_bwd<TPR, NV, V>(g, y, r1y, p.post, p.invC, in, red);
+    if (p.post != MDG_NORM_NONE) normalise_bwd<TPR, NV, V>(g, y[0], r1y[0], p.post, p.invC, in, red);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (in[k]) stv<CT, V>(reinterpret_cast<CT*>(p.dy) + (long long)row * p.C + (t + k * TPR) * V, g[k]);
@@ -362,57 +383,68 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void grn_bwd_kernel(const Gr
   }
 }
 
-// Column sums of the blocks' partials: one block = 64 columns of one group, 16 chunk lanes; then the
-// group's modulation gradients, and the groups' sums S [G][4][C] over the first chunk's partials
-// (kept for grn_weights_kernel).
+// Column sums of the blocks' partials: one block = 64 columns of one group and one norm (blockIdx.z 0: the
+// pre norm's S1, S2; 1: the post norm's S3, S4), 16 lanes along the chunks; then the group's modulation
+// gradients, and its sums S [G][4][C] for grn_weights_kernel.
 __global__ __launch_bounds__(1024) void grn_cols_kernel(const GrnP p, float* sums, float* dgate, float* dshift, float* dscale,
                                                         long long dmod_stride) {
-  __shared__ float red[16][64];
-  const int c = blockIdx.y * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6, grp = blockIdx.x;
-  const float* base = p.part + (long long)grp * p.chunks * 4 * p.C;
-  float S[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    float v = 0.f;
-    if (c < p.C && (s < 2 ? p.want_x_sums : p.want_y_sums))
-      for (int k = lane; k < p.chunks; k += 16) v += base[((long long)k * 4 + s) * p.C + c];
-    red[lane][threadIdx.x & 63] = v;
-    __syncthreads();
-    float a = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) a += red[k][threadIdx.x & 63];
-    S[s] = a;
-    __syncthreads();
+  __shared__ float red[2][16][64];
+  const int x = threadIdx.x & 63, c = blockIdx.y * 64 + x, lane = threadIdx.x >> 6, grp = blockIdx.x, half = blockIdx.z;
+  if (half ? !p.want_y_sums : !p.want_x_sums) return;
+  const float* base = p.part + ((long long)grp * p.chunks * 4 + 2 * half) * p.C + c;
+  float u = 0.f, v = 0.f;
+  if (c < p.C) {
+#pragma unroll 4
+    for (int k = lane; k < p.chunks; k += 16) {
+      u += base[(long long)k * 4 * p.C];
+      v += base[((long long)k * 4 + 1) * p.C];
+    }
   }
+  red[0][lane][x] = u, red[1][lane][x] = v;
+  __syncthreads();
   if (lane != 0 || c >= p.C) return;
+  u = v = 0.f;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) sums[((long long)grp * 4 + s) * p.C + c] = S[s];
+  for (int k = 0; k < 16; ++k) u += red[0][k][x], v += red[1][k][x];
+  sums[((long long)grp * 4 + 2 * half) * p.C + c] = u;
+  sums[((long long)grp * 4 + 2 * half + 1) * p.C + c] = v;
   const long long at = (long long)grp * dmod_stride + c;
-  if (dshift) dshift[at] = S[0];
-  if (dscale) dscale[at] = (p.w2 ? p.w2[c] : 1.f) * S[1] + (p.b2 ? p.b2[c] * S[0] : 0.f);
-  if (dgate) dgate[at] = (p.w1 ? p.w1[c] : 1.f) * S[3] + (p.b1 ? p.b1[c] * S[2] : 0.f);
+  if (half) {
+    if (dgate) dgate[at] = (p.w1 ? p.w1[c] : 1.f) * v + (p.b1 ? p.b1[c] * u : 0.f);
+  } else {
+    if (dshift) dshift[at] = u;
+    if (dscale) dscale[at] = (p.w2 ? p.w2[c] : 1.f) * v + (p.b2 ? p.b2[c] * u : 0.f);
+  }
 }
 
-__global__ __launch_bounds__(256) void grn_weights_kernel(const GrnP p, const float* sums, int G, float* dw1, float* db1,
-                                                          float* dw2, float* db2) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= p.C) return;
-  float a = 0.f, b = 0.f, d = 0.f, e = 0.f;
-  for (int g = 0; g < G; ++g) {
-    const float* s = sums + (long long)g * 4 * p.C + c;
-    if (p.want_x_sums) {
-      const float sc = 1.0f + (p.scale ? p.scale[g * p.mod_stride + c] : 0.f);
-      e = fmaf(sc, s[0], e), d = fmaf(sc, s[p.C], d);
-    }
-    if (p.want_y_sums) {
-      const float gt = p.gate ? p.gate[g * p.mod_stride + c] : 1.f;
-      b = fmaf(gt, s[2 * p.C], b), a = fmaf(gt, s[3 * (long long)p.C], a);
+// The weights' gradients: one block = 64 columns, 16 lanes along the groups.
+__global__ __launch_bounds__(1024) void grn_weights_kernel(const GrnP p, const float* sums, int G, float* dw1, float* db1,
+                                                           float* dw2, float* db2) {
+  __shared__ float red[4][16][64];
+  const int x = threadIdx.x & 63, c = blockIdx.x * 64 + x, lane = threadIdx.x >> 6;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};  // db2, dw2, db1, dw1
+  if (c < p.C) {
+    for (int g = lane; g < G; g += 16) {
+      const float* s = sums + (long long)g * 4 * p.C + c;
+      if (p.want_x_sums) {
+        const float sc = 1.0f + (p.scale ? p.scale[g * p.mod_stride + c] : 0.f);
+        a[0] = fmaf(sc, s[0], a[0]), a[1] = fmaf(sc, s[p.C], a[1]);
+      }
+      if (p.want_y_sums) {
+        const float gt = p.gate ? p.gate[g * p.mod_stride + c] : 1.f;
+        a[2] = fmaf(gt, s[2 * (long long)p.C], a[2]), a[3] = fmaf(gt, s[3 * (long long)p.C], a[3]);
+      }
     }
   }
-  if (dw1) dw1[c] = a;
-  if (db1) db1[c] = b;
-  if (dw2) dw2[c] = d;
-  if (db2) db2[c] = e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[i][lane][x] = a[i];
+  __syncthreads();
+  if (lane >= 4 || c >= p.C) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v += red[lane][k][x];
+  float* out = lane == 0 ? db2 : lane == 1 ? dw2 : lane == 2 ? db1 : dw1;
+  if (out) out[c] = v;
 }
 
 GrnP grn_params(const mdg_gate_res_norm_desc& d) {
@@ -462,9 +494,13 @@ Shape grn_shape(int C, int V) {
 
 template <typename RT, typename CT, int V, int TPR, int NV>
 void grn_go(const GrnP& p, bool back, int G, hipStream_t s) {
-  constexpr int BD = TPR < 256 ? 256 : TPR, TEAMS = BD / TPR;
-  if (back) hipLaunchKernelGGL((grn_bwd_kernel<RT, CT, V, TPR, NV>), dim3((unsigned)(G * p.chunks)), dim3(BD), 0, s, p);
-  else hipLaunchKernelGGL((grn_fwd_kernel<RT, CT, V, TPR, NV>), dim3((unsigned)((p.M + TEAMS - 1) / TEAMS)), dim3(BD), 0, s, p);
+  constexpr int BD = TPR < 256 ? 256 : TPR, TEAMS = BD / TPR, ROWS = TPR == 256 ? 2 : 1;
+  if (back) {
+    if constexpr (V <= 4) hipLaunchKernelGGL((grn_bwd_kernel<RT, CT, V, TPR, NV>), dim3((unsigned)(G * p.chunks)), dim3(BD), 0, s, p);
+    return;
+  }
+  hipLaunchKernelGGL((grn_fwd_kernel<RT, CT, V, TPR, NV, ROWS>), dim3((unsigned)((p.M + TEAMS * ROWS - 1) / (TEAMS * ROWS))),
+                          dim3(BD), 0, s, p);
 }
 
 template <typename RT, typename CT, int V>
@@ -494,7 +530,8 @@ void grn_by_shape(const GrnP& p, bool back, int G, hipStream_t s) {
 }
 
 void grn_dispatch(const mdg_gate_res_norm_desc& d, const GrnP& p, bool back, int G, hipStream_t s) {
-  const int v = grn_vec(d);
+  // (the backward's rows, sums and parameters fill the registers at 4 columns per vector)
+  const int v = back ? (grn_vec(d) < 4 ? 1 : 4) : grn_vec(d);
   if (d.res_dtype == MDG_BF16) {
     if (v == 8) grn_by_shape<bf16_t, bf16_t, 8>(p, back, G, s);
     else if (v == 4) grn_by_shape<bf16_t, bf16_t, 4>(p, back, G, s);
@@ -512,10 +549,10 @@ bool want_y(const mdg_gate_res_norm_desc& d) { return d.dgate || d.dpost_w || d.
 bool want_x(const mdg_gate_res_norm_desc& d) { return d.dshift || d.dscale || d.dpre_w || d.dpre_b; }
 int groups(const mdg_gate_res_norm_desc& d) { return (int)(((long long)d.M + d.rows_per_mod - 1) / d.rows_per_mod); }
 
-// Chunks of a group's rows: about 1024 blocks in all, each with 32 rows or more
+// Chunks of a group's rows: about 768 blocks in all (three per CU), each with 32 rows or more
 int grn_chunks(const mdg_gate_res_norm_desc& d) {
   const int G = groups(d);
-  const int want = (1024 + G - 1) / G, most = (d.rows_per_mod + 31) / 32;
+  const int want = (768 + G - 1) / G, most = (d.rows_per_mod + 31) / 32;
   return want < most ? want : most;
 }
 
@@ -545,10 +582,10 @@ hipError_t gate_res_norm_bwd_launch(const mdg_gate_res_norm_desc& d, void* ws, h
   }
   grn_dispatch(d, p, true, G, s);
   if (sums) {
-    hipLaunchKernelGGL(grn_cols_kernel, dim3(G, (d.C + 63) / 64), dim3(1024), 0, s, p, S, d.dgate, d.dshift, d.dscale,
+    hipLaunchKernelGGL(grn_cols_kernel, dim3(G, (d.C + 63) / 64, 2), dim3(1024), 0, s, p, S, d.dgate, d.dshift, d.dscale,
                        (long long)d.dmod_stride);
     if (d.dpost_w || d.dpost_b || d.dpre_w || d.dpre_b)
-      hipLaunchKernelGGL(grn_weights_kernel, dim3((d.C + 255) / 256), dim3(256), 0, s, p, (const float*)S, G, d.dpost_w, d.dpost_b,
+      hipLaunchKernelGGL(grn_weights_kernel, dim3((d.C + 63) / 64), dim3(1024), 0, s, p, (const float*)S, G, d.dpost_w, d.dpost_b,
                          d.dpre_w, d.dpre_b);
   }
   return hipGetLastError();

@@ -1,10 +1,10 @@
 // Rotary positions with several axes: pair p of a head's rotated columns belongs to one axis (frame,
 // residue, height, ...) and turns by pos[token][axis[p]] * freq[p]; columns past the pairs pass through.
 //   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin      (inverse: -sin; it is the backward)
-// Bound by memory: every element is read and written once.  The angle is formed in double as a number
-// of turns and reduced there (a position of 10^6 in fp32 would lose the angle), then cos / sin in
-// fp32, once per (token, pair) and thread for all the heads that thread walks.  q and k go in one
-// launch: their heads are one list.
+// Bound by memory: every element is read and written once.  A block takes a few tokens: first their cos /
+// sin per pair into LDS, once for all heads (the angle is formed in double as a number of turns and
+// reduced there: a position of 10^6 in fp32 would lose it), then a sweep over the tokens' rows in
+// memory order.  q and k go in one launch: their heads are one list.
 #include "../../include/mdgen_hip.h"
 #include "common.h"
 
@@ -19,18 +19,25 @@ struct RopeSeg {
 struct RopeP {
   RopeSeg seg[2];
   int H0, HT;  // heads of the first tensor, of both
-  int N, D, np, pairs;
-  long long tokens;  // B * N
+  int N, D, np;
+  unsigned tokens;  // B * N
   const void* pos;
   long long pb, pn;
   const double* turns;
   const int* axis;
   const int* cols;  // first columns of the pairs, then second columns
   int inverse, i64;
-  int rot_tasks, tasks;  // per head row: rotations of V pairs, then copies of 2V (or V) columns
+  int rot_tasks, tasks;  // per head row: rotations of V pairs, then copies of copy_w columns (2V or V)
   int copy_w;
-  int hpt, hs;  // heads per thread, threads along the heads
+  int T;  // tokens per block
+  float inv_np, inv_tasks, inv_row;  // 1 / pairs, tasks, tasks of a token
 };
+
+constexpr int kRopeLds = 2048;  // (token, pair) entries of a block
+
+// i / d for 0 <= i < 2^21 and d < 2^21: (i + 1/2) / d is at least 1 / (2 d) from a whole number, well
+// beyond the products' rounding there
+__device__ __forceinline__ int small_div(int i, float inv_d) { return (int)(((float)i + 0.5f) * inv_d); }
 
 template <typename CT, int W> struct Pack { CT v[W]; };
 template <typename CT, int W>
@@ -75,65 +82,63 @@ __device__ __forceinline__ void stw(CT* p, const Pack<CT, W>& r) {
   }
 }
 
-// V pairs per thread and head.  INTER: the pair's columns are neighbours (one run of 2V columns);
-// otherwise two runs of V columns, cols[p] .. and cols[np + p] ..  (the host picks V so that no run
-// crosses a section and every run is aligned to its bytes).
+// V pairs per item.  INTER: the pair's columns are neighbours (one run of 2V columns); otherwise two runs
+// of V columns, cols[p] .. and cols[np + p] ..  (the host picks V so that no run crosses a section
+// and every run is aligned to its bytes).  Items run over (token, head, task), task fastest.
 template <typename CT, int V, bool INTER>
 __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeP p) {
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int task = (int)(id % p.tasks);
-  const long long rest = id / p.tasks;
-  const int hslot = (int)(rest % p.hs);
-  const long long tok = rest / p.hs;
-  if (tok >= p.tokens) return;
-  const long long b = tok / p.N, n = tok % p.N;
-
-  const bool rot = task < p.rot_tasks;
-  float cs[V], sn[V];
-  int c1, c2;
-  if (rot) {
-    const int p0 = task * V;
-    c1 = INTER ? 2 * p0 : p.cols[p0];
-    c2 = INTER ? 2 * p0 : p.cols[p.np + p0];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const long long at = b * p.pb + n * p.pn + p.axis[p0 + i];
-      const double ps = p.i64 ? (double)reinterpret_cast<const long long*>(p.pos)[at]
-                              : (double)reinterpret_cast<const int*>(p.pos)[at];
-      const double t = ps * p.turns[p0 + i];
-      const float f = 2.0f * (float)(t - rint(t));  // half turns in [-1, 1]
-      sincospif(f, &sn[i], &cs[i]);
-      if (p.inverse) sn[i] = -sn[i];
-    }
-  } else {
-    c1 = c2 = 2 * p.np + (task - p.rot_tasks) * p.copy_w;
+  __shared__ __attribute__((aligned(16))) float cs[kRopeLds], sn[kRopeLds];
+  const int tid = threadIdx.x;
+  const unsigned t0 = blockIdx.x * (unsigned)p.T;
+  const int T = (int)min((unsigned)p.T, p.tokens - t0);
+  for (int i = tid; i < T * p.np; i += 256) {
+    const int t = small_div(i, p.inv_np), pr = i - t * p.np;
+    const unsigned b = (t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
+    const long long at = b * p.pb + n * p.pn + p.axis[pr];
+    const double ps = p.i64 ? (double)reinterpret_cast<const long long*>(p.pos)[at]
+                            : (double)reinterpret_cast<const int*>(p.pos)[at];
+    const double turn = ps * p.turns[pr];
+    float s, c;
+    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);  // half turns in [-1, 1]
+    cs[i] = c, sn[i] = p.inverse ? -s : s;
   }
-  for (int j = 0; j < p.hpt; ++j) {
-    const int hd = j * p.hs + hslot;
-    if (hd >= p.HT) break;
+  __syncthreads();
+  constexpr int W = INTER ? 2 * V : V;
+  const int per = p.HT * p.tasks, items = T * per;
+#pragma unroll 2
+  for (int i = tid; i < items; i += 256) {
+    const int t = small_div(i, p.inv_row), j = i - t * per, hd = small_div(j, p.inv_tasks), task = j - hd * p.tasks;
+    const unsigned b = (t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
     const RopeSeg& g = p.seg[hd >= p.H0];
     const int h = hd >= p.H0 ? hd - p.H0 : hd;
     const CT* x = reinterpret_cast<const CT*>(g.x) + b * g.xb + n * g.xn + h * g.xh;
     CT* y = reinterpret_cast<CT*>(g.y) + b * g.yb + n * g.yn + h * g.yh;
-    if (!rot) {
-      for (int i = 0; i < p.copy_w; i += V) stw<CT, V>(y + c1 + i, ldw<CT, V>(x + c1 + i));
-    } else if constexpr (INTER) {
-      Pack<CT, 2 * V> a = ldw<CT, 2 * V>(x + c1), r;
+    if (task >= p.rot_tasks) {
+      const int c = 2 * p.np + (task - p.rot_tasks) * p.copy_w;
+      for (int k = 0; k < p.copy_w; k += V) stw<CT, V>(y + c + k, ldw<CT, V>(x + c + k));
+      continue;
+    }
+    const int p0 = task * V, at = t * p.np + p0;
+    const int c1 = INTER ? 2 * p0 : p.cols[p0], c2 = INTER ? 0 : p.cols[p.np + p0];
+    const Pack<float, V> c = ldw<float, V>(cs + at), s = ldw<float, V>(sn + at);
+    if constexpr (INTER) {
+      const Pack<CT, W> a = ldw<CT, W>(x + c1);
+      Pack<CT, W> r;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float u = (float)a.v[2 * i], w = (float)a.v[2 * i + 1];
-        r.v[2 * i] = (CT)(u * cs[i] - w * sn[i]);
-        r.v[2 * i + 1] = (CT)(w * cs[i] + u * sn[i]);
+      for (int k = 0; k < V; ++k) {
+        const float v = (float)a.v[2 * k], w = (float)a.v[2 * k + 1];
+        r.v[2 * k] = (CT)(v * c.v[k] - w * s.v[k]);
+        r.v[2 * k + 1] = (CT)(w * c.v[k] + v * s.v[k]);
       }
-      stw<CT, 2 * V>(y + c1, r);
+      stw<CT, W>(y + c1, r);
     } else {
-      const Pack<CT, V> a = ldw<CT, V>(x + c1), c = ldw<CT, V>(x + c2);
+      const Pack<CT, V> a = ldw<CT, V>(x + c1), d = ldw<CT, V>(x + c2);
       Pack<CT, V> r, q;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float u = (float)a.v[i], w = (float)c.v[i];
-        r.v[i] = (CT)(u * cs[i] - w * sn[i]);
-        q.v[i] = (CT)(w * cs[i] + u * sn[i]);
+      for (int k = 0; k < V; ++k) {
+        const float v = (float)a.v[k], w = (float)d.v[k];
+        r.v[k] = (CT)(v * c.v[k] - w * s.v[k]);
+        q.v[k] = (CT)(w * c.v[k] + v * s.v[k]);
       }
       stw<CT, V>(y + c1, r);
       stw<CT, V>(y + c2, q);
@@ -174,24 +179,22 @@ static RopeP rope_params(const mdg_rope_axes_desc& d, int& V) {
     p.HT += d.H[i];
   }
   if (d.nseg == 1) p.seg[1] = p.seg[0];
-  p.H0 = d.H[0], p.N = d.N, p.D = d.D, p.np = d.npairs, p.pairs = d.pairs;
-  p.tokens = (long long)d.B * d.N;
+  p.H0 = d.H[0], p.N = d.N, p.D = d.D, p.np = d.npairs;
+  p.tokens = (unsigned)d.B * (unsigned)d.N;
   p.pos = d.pos, p.pb = d.pos_sb, p.pn = d.pos_sn, p.i64 = d.pos_i64;
   p.turns = d.turns, p.axis = d.axis, p.cols = d.cols, p.inverse = d.inverse;
   const int tail = d.D - 2 * d.npairs;
   p.rot_tasks = d.npairs / V;
   p.copy_w = tail % (2 * V) == 0 ? 2 * V : V;
   p.tasks = p.rot_tasks + tail / p.copy_w;
-  // heads per thread: 8 share one set of cos / sin once the launch fills the chip without that
-  p.hpt = p.tokens * p.tasks * p.HT >= 256LL * 2048 * 4 ? (p.HT < 8 ? p.HT : 8) : 1;
-  p.hs = (p.HT + p.hpt - 1) / p.hpt;
+  // tokens per block: about 2048 items, and 1024 blocks where there are that many tokens
+  const int row = p.HT * p.tasks;
+  int T = 2048 / row, few = (int)((p.tokens + 1023) / 1024);
+  if (T > few) T = few;
+  if (T * p.np > kRopeLds) T = kRopeLds / p.np;
+  p.T = T < 1 ? 1 : T;
+  p.inv_np = 1.0f / p.np, p.inv_tasks = 1.0f / p.tasks, p.inv_row = 1.0f / row;
   return p;
-}
-
-bool rope_axes_grid_ok(const mdg_rope_axes_desc& d) {
-  int V;
-  const RopeP p = rope_params(d, V);
-  return (p.tokens * p.tasks * p.hs + 255) / 256 < (1LL << 31);
 }
 
 // whether one interleaved pair can be read as a run of two elements
@@ -206,14 +209,9 @@ bool rope_axes_pair_aligned(const mdg_rope_axes_desc& d) {
   return true;
 }
 
-hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s) {
-  int V;
-  const RopeP p = rope_params(d, V);
-  // (interleaved pairs that do not lie on a word of two elements take the two-run kernel: V is 1 then)
-  const bool inter = d.pairs == MDG_ROPE_INTERLEAVED && rope_axes_pair_aligned(d);
-  const unsigned grid = (unsigned)((p.tokens * p.tasks * p.hs + 255) / 256);
+static void rope_go(const RopeP& p, int dtype, int V, bool inter, unsigned grid, hipStream_t s) {
 #define ROPE_GO(CT, V_, I) hipLaunchKernelGGL((rope_axes_kernel<CT, V_, I>), dim3(grid), dim3(256), 0, s, p)
-  if (d.dtype == MDG_BF16) {
+  if (dtype == MDG_BF16) {
     if (inter) {
       if (V == 4) ROPE_GO(bf16_t, 4, true);
       else if (V == 2) ROPE_GO(bf16_t, 2, true);
@@ -235,6 +233,14 @@ hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s) {
     }
   }
 #undef ROPE_GO
+}
+
+hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s) {
+  int V;
+  const RopeP p = rope_params(d, V);
+  // (interleaved pairs that do not lie on a word of two elements take the two-run kernel: V is 1 then)
+  const bool inter = d.pairs == MDG_ROPE_INTERLEAVED && rope_axes_pair_aligned(d);
+  rope_go(p, d.dtype, V, inter, (p.tokens + p.T - 1) / p.T, s);
   return hipGetLastError();
 }
 
