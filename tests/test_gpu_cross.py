@@ -617,3 +617,99 @@ def test_operators_on_another_stream_and_repeatable():
     torch.cuda.synchronize()
     for r in res:
         assert all(torch.equal(a, b) for a, b in zip(base, r))
+
+
+# ------------------------------------------------------------------------------------------ autograd's corners
+def _small(seed=2):
+    g = _gen(seed)
+    q, k, v = (torch.randn(2, n, 2, 16, generator=g).cuda() for n in (5, 9, 9))
+    h, y = torch.randn(2, 5, 32, generator=g).cuda(), torch.randn(2, 5, 32, generator=g).cuda()
+    gate = torch.randn(2, 32, generator=g).cuda()
+    plan = X().RopeAxes([4, 4], device="cuda")
+    pos = torch.randint(0, 50, (5, 2), generator=g).cuda()
+    return [(lambda q, k, v: X().cross_attention(q, k, v), (q, k, v)),
+            (lambda q: X().rope_axes(plan, pos, q), (q,)),
+            (lambda h, y, gate: sum(X().gate_residual_norm(h, y, gate=gate, post="rms")), (h, y, gate))]
+
+
+@pytest.mark.parametrize("which", range(3), ids=["attention", "rope", "norms"])
+def test_once_differentiable(which):
+    """create_graph returns the same gradients; differentiating them raises, and so does a second backward."""
+    f, ins = _small()[which]
+    leaves = [t.clone().requires_grad_(True) for t in ins]
+    base = torch.autograd.grad(f(*leaves).sum(), leaves)
+    again = torch.autograd.grad(f(*leaves).sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(base, again))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(sum(a.sum() for a in again), leaves)
+    out = f(*leaves)
+    out.sum().backward()
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("which", range(3), ids=["attention", "rope", "norms"])
+def test_saved_tensors_moved_to_the_host(which):
+    """Saved tensors that come back at other addresses (offloaded to the host between the passes)."""
+    f, ins = _small()[which]
+    leaves = [t.clone().requires_grad_(True) for t in ins]
+    base = torch.autograd.grad(f(*leaves).sum(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        out = f(*leaves)
+    junk = [torch.full_like(t, float("nan")) for t in ins]
+    assert all(torch.equal(a, b) for a, b in zip(base, torch.autograd.grad(out.sum(), leaves)))
+    del junk
+
+
+def test_a_changed_input_is_noticed():
+    f, ins = _small()[0]
+    leaves = [t.clone().requires_grad_(True) for t in ins]
+    mask = torch.ones(2, 9, device="cuda")
+    out = X().cross_attention(*leaves, mask=mask)
+    mask[0, 3] = 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_rope_plan_copies_and_gradient_of_one_output():
+    import copy
+    import pickle
+
+    plan = X().RopeAxes([3, 5], pairs="axis", device="cuda")
+    x = torch.randn(1, 7, 2, 16, device="cuda")
+    pos = torch.randint(0, 99, (7, 2), device="cuda", dtype=torch.int32)
+    want = X().rope_axes(plan, pos, x)
+    for p in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        assert torch.equal(X().rope_axes(p, pos, x), want)
+    q, k = (x.clone().requires_grad_(True) for _ in range(2))
+    qo, ko = X().rope_axes(plan, pos, q, k)
+    dq, dk = torch.autograd.grad(ko.sum(), (q, k), allow_unused=True)
+    assert dq is None and torch.isfinite(dk).all()
+    with torch.inference_mode():
+        y = x.clone()
+        X().rope_axes(plan, pos, y, inplace=True)
+        assert torch.equal(y, want)
+
+
+def test_refusals_on_the_gpu():
+    x = torch.zeros(2, 3, 4, 8, device="cuda")
+    for kw in (dict(mask=torch.ones(2, 4, device="cuda")), dict(mask=torch.ones(2, 3, device="cuda").half()),
+               dict(kv_len=torch.ones(2, device="cuda")), dict(q_len=torch.ones(3, dtype=torch.int32, device="cuda")),
+               dict(mask=torch.ones(2, 3)), dict(scale=0.0), dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            X().cross_attention(x, x, x, **kw)
+    h = torch.zeros(6, 8, device="cuda")
+    for kw in (dict(gate=torch.ones(4, 8, device="cuda")), dict(gate=torch.ones(2, 7, device="cuda")), dict(pre_w=torch.ones(9, device="cuda")),
+               dict(gate=torch.ones(2, 8, device="cuda"), shift=torch.ones(3, 8, device="cuda")), dict(eps=-1.0),
+               dict(resid_scale=float("inf")), dict(scale=torch.ones(2, 8, device="cuda").half())):
+        with pytest.raises(ValueError):
+            X().gate_residual_norm(h, h, **kw)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_operators_on_a_device_that_is_not_current():
+    f, ins = _small()[0]
+    torch.cuda.set_device(0)
+    with torch.cuda.device(1):
+        other = [t.to("cuda:1") for t in ins]
+    assert torch.equal(f(*other).cpu(), f(*ins).cpu()) and torch.cuda.current_device() == 0
