@@ -37,6 +37,18 @@ struct View {  // element strides of batch, token, head; the head dim is contigu
   const void* p;
   long long sb, sn, sh;
 };
+// n / d for 0 <= n < 2^31 by one multiplication (d >= 1): mul = floor(2^32 (2^shift - d) / d) + 1 with
+// shift = ceil(log2 d); the sum below stays under 2^32
+struct Divisor {
+  unsigned mul, shift;
+};
+inline Divisor divisor(long long d) {
+  unsigned s = 0;
+  while ((1LL << s) < d) ++s;
+  return Divisor{(unsigned)((((1ULL << s) - (unsigned long long)d) << 32) / (unsigned long long)d + 1), s};
+}
+__device__ __forceinline__ int quot(int n, const Divisor& d) { return (int)((__umulhi((unsigned)n, d.mul) + (unsigned)n) >> d.shift); }
+
 struct CrossP {
   View q, k, v, o, olo, dout, dq, dk, dv;
   const int *qlen, *klen;
@@ -51,6 +63,7 @@ struct CrossP {
   float* part;  // split partials
   float* part_ml;
   int nsplit;
+  Divisor by_g, by_hk, by_split, by_tiles, by_rows;
 };
 
 template <typename CT>
@@ -378,18 +391,25 @@ __device__ __forceinline__ f32x16 zero16() {
   return s;
 }
 
+// A product's steps of 16 past D are zeros.  fp32, eight MFMA of 64 cycles each, leaves them out; for bf16,
+// one of 32 cycles, the branches would cost more than they save.
+template <typename CT, int DP>
+__device__ __forceinline__ bool step_there(int ks, int D) {
+  return is_bf16<CT>() || 32 * ks < DP || 16 * ks < D;  // (D > DP / 2, or DP is 32 and D > 0)
+}
+
 // S^T of a tile of NT * 32 keys.  (The products stand in both branches: an accumulator that is one of two
 // things would be copied, one that starts at a literal zero is not.)
 template <typename CT, int DP, int NT>
 __device__ __forceinline__ void key_scores(f32x16 (&s)[NT], const CT* Kt, const typename V8<CT>::T (&qf)[DP / 16],
-                                           const float* kbs, bool holes, int lane) {
+                                           const float* kbs, bool holes, int D, int lane) {
   if (holes) {
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt) {
       s[kt] = kb_init(kbs + 32 * kt, lane);
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
-        s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
+        if (step_there<CT, DP>(ks, D)) s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
     }
   } else {
 #pragma unroll
@@ -397,7 +417,7 @@ __device__ __forceinline__ void key_scores(f32x16 (&s)[NT], const CT* Kt, const 
       s[kt] = zero16();
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
-        s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
+        if (step_there<CT, DP>(ks, D)) s[kt] = mma<CT>(row_frag<CT, DP>(Kt, 32 * kt + (lane & 31), 16 * ks, lane), qf[ks], s[kt]);
     }
   }
 }
@@ -411,8 +431,8 @@ __device__ __forceinline__ typename V8<CT>::T half_frag(const f32x16& s, int s2)
 }
 
 // keys [k0, k1) of split `sp`: the sequence's own length shared out in multiples of 32
-__device__ __forceinline__ void split_range(int klen, int nsplit, int sp, int& k0, int& k1) {
-  const int per = ((klen + nsplit - 1) / nsplit + 31) / 32 * 32;
+__device__ __forceinline__ void split_range(const CrossP& p, int klen, int sp, int& k0, int& k1) {
+  const int per = (quot(klen + p.nsplit - 1, p.by_split) + 31) / 32 * 32;
   k0 = min(klen, sp * per);
   k1 = min(klen, k0 + per);
 }
@@ -422,14 +442,21 @@ struct BlockId {
 };
 __device__ __forceinline__ BlockId block_id(const CrossP& p, int tiles) {
   BlockId r;
-  int id = blockIdx.x;
-  r.tile = id % tiles;
-  id /= tiles;
-  r.split = id % p.nsplit;
-  id /= p.nsplit;
-  r.hk = id % p.Hk;
-  r.b = id / p.Hk;
+  int id = blockIdx.x, q = quot(id, p.by_tiles);
+  r.tile = id - q * tiles;
+  id = q, q = quot(id, p.by_split);
+  r.split = id - q * p.nsplit;
+  r.b = quot(q, p.by_hk);
+  r.hk = q - r.b * p.Hk;
   return r;
+}
+// packed row r: token n, query head g of the key head's G
+struct PackedRow {
+  int n, g;
+};
+__device__ __forceinline__ PackedRow packed(const CrossP& p, int r) {
+  const int n = quot(r, p.by_g);
+  return PackedRow{n, r - n * p.G};
 }
 
 // rows of partial `sp`: ((b * Hk + hk) * rows + r), rows = Nq * G
@@ -459,7 +486,8 @@ __device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, i
             make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
     return;
   }
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const PackedRow pk = packed(p, r);
+  const int n = pk.n, head = id.hk * p.G + pk.g;
   const bool some = live && l != 0.f;  // (a NaN among the keys that are there stays one)
   const float inv = some ? 1.0f / l : 0.f;
   if (p.lse && h == 0) p.lse[((long long)id.b * p.H + head) * p.Nq + n] = some ? m * p.c + log2f(l) : -INFINITY;
@@ -495,7 +523,8 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = id.tile * 128 + wave * 32 + (lane & 31);
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const PackedRow pk = packed(p, r);
+  const int n = pk.n, head = id.hk * p.G + pk.g;
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const bool live = r < rows && n < qlen;
 
@@ -517,7 +546,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
   float m = kNoMax, l = 0.f;
 
   int k0, k1;
-  split_range(klen, p.nsplit, id.split, k0, k1);
+  split_range(p, klen, id.split, k0, k1);
   KvStage<CT, DP, KT, 256, VEC, VEC> st;
   const int nt = (k1 - k0 + KT - 1) / KT;
   if (nt > 0) {
@@ -533,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     const CT* Kc = Ks + cur * TILE;
     const CT* Vc = Vs + cur * TILE;
     f32x16 s[NT];
-    key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), lane);
+    key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), p.D, lane);
     softmax_tile<NT, NO, !kOnes>(s, o, m, l, p.c);
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
@@ -573,7 +602,8 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
   const bool second = wave >= 4;
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = id.tile * 256 + wave * 32 + (lane & 31);
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const PackedRow pk = packed(p, r);
+  const int n = pk.n, head = id.hk * p.G + pk.g;
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const bool live = r < rows && n < qlen;
 
@@ -588,7 +618,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
   bf16x8 pf[NT][2];
 
   int k0, k1;
-  split_range(klen, p.nsplit, id.split, k0, k1);
+  split_range(p, klen, id.split, k0, k1);
   KvStage<CT, DP, KT, 256, true, true> st;
   const int nt = (k1 - k0 + KT - 1) / KT;
   if (nt > 0 && !second) {
@@ -613,7 +643,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
       vprev = vprev == 2 ? 0 : vprev + 1;
     }
     if (t < nt)
-      key_scores<CT, DP, NT>(s, Ks + (t & 1) * TILE, qf, kbs + (t & 1) * KT, __builtin_amdgcn_readfirstlane(flag[t & 1]), lane);
+      key_scores<CT, DP, NT>(s, Ks + (t & 1) * TILE, qf, kbs + (t & 1) * KT, __builtin_amdgcn_readfirstlane(flag[t & 1]), p.D, lane);
     __syncthreads();
     if (t < nt) {
       softmax_tile<NT, DT, true>(s, o, m, l, p.c);
@@ -646,7 +676,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
 
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = lane & 31;
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const PackedRow pk = packed(p, r);
+  const int n = pk.n, head = id.hk * p.G + pk.g;
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const bool live = r < rows && n < qlen;
   typename V8<CT>::T qf[KS];
@@ -656,7 +687,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
   float m = kNoMax, l = 0.f;
 
   int k0, k1;
-  split_range(klen, p.nsplit, id.split, k0, k1);
+  split_range(p, klen, id.split, k0, k1);
   using S = KvStage<CT, DP, 32, 64, VEC, BUFS == 2>;
   S st;
   int key = k0 + 32 * wave, cur = 0;
@@ -685,7 +716,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     f32x16 s[1];
-    key_scores<CT, DP, 1>(s, Ks + cur * TILE, qf, kbs, __builtin_amdgcn_readfirstlane(*flag), lane);
+    key_scores<CT, DP, 1>(s, Ks + cur * TILE, qf, kbs, __builtin_amdgcn_readfirstlane(*flag), p.D, lane);
     softmax_tile<1, DT, true>(s, o, m, l, p.c);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
@@ -749,7 +780,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     if (p.nsplit > 1) {
       *reinterpret_cast<float4*>(p.part + part_row(p, id.split, id.b, id.hk, row) * DP + d0) = v;
     } else {
-      const int rn = row / p.G, rh = id.hk * p.G + row % p.G;
+      const PackedRow pr = packed(p, row);
+      const int rn = pr.n, rh = id.hk * p.G + pr.g;
       const float Lr = js[row];
       const bool some = rn < qlen && Lr != 0.f;
       const float inv = some ? 1.0f / Lr : 0.f;
@@ -767,7 +799,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
 template <typename CT, int DP, bool VEC>
 __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
   const long long rows = (long long)p.Nq * p.G, total = rows * p.B * p.Hk;
-  const long long pr = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int pr = (int)min(blockIdx.x * 8LL + (threadIdx.x >> 5), total);  // (total < 2^31)
   const int sub = threadIdx.x & 31, d0 = sub * 4;
   if (pr >= total) return;  // (all 32 lanes of the row)
   float M = kNoMax;
@@ -793,7 +825,9 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
       }
     }
   }
-  const int bh = (int)(pr / rows), r = (int)(pr % rows), b = bh / p.Hk, n = r / p.G, head = (bh % p.Hk) * p.G + r % p.G;
+  const int bh = quot(pr, p.by_rows), b = quot(bh, p.by_hk);
+  const PackedRow pk = packed(p, pr - bh * (int)rows);
+  const int n = pk.n, head = (bh - b * p.Hk) * p.G + pk.g;
   const bool some = n < clamp_len(p.qlen, b, p.Nq) && L != 0.f;
   const float inv = some ? 1.0f / L : 0.f;
   if (p.lse && d0 == 0) p.lse[((long long)b * p.H + head) * p.Nq + n] = some ? M * p.c + log2f(L) : -INFINITY;
@@ -820,12 +854,21 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const BlockId id = block_id(p, tiles);
   const int rows = p.Nq * p.G, r = id.tile * 128 + wave * 32 + (lane & 31);
-  const int n = r / p.G, head = id.hk * p.G + r % p.G;
+  const PackedRow pk = packed(p, r);
+  const int n = pk.n, head = id.hk * p.G + pk.g;
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const bool live = r < rows && n < qlen;
   const int ln = live ? n : 0, lh = live ? head : 0;
   const long long srow = ((long long)id.b * p.H + lh) * p.Nq + ln;
 
+  int k0, k1;
+  split_range(p, klen, id.split, k0, k1);
+  KvStage<CT, DP, KT, 256, VEC, VEC> st;
+  const int nt = (k1 - k0 + KT - 1) / KT;
+  if (nt > 0) {  // (the first tile's loads start before delta waits for its own)
+    st.init(p, id.b, id.hk, k0, k1, KT, tid);
+    st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
+  }
   typename V8<CT>::T qf[KS], gf[KS];
   float delta = 0.f;
 #pragma unroll
@@ -846,7 +889,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
   delta = other_half_sum(delta);
   float lse = live ? p.lse[srow] : -INFINITY;
   if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every P is 0
-  if (p.delta && id.split == 0 && r < rows && h == 0) p.delta[((long long)id.b * p.H + head) * p.Nq + n] = delta;
+  if (id.split == 0 && r < rows && h == 0) p.delta[((long long)id.b * p.H + head) * p.Nq + n] = delta;
 
   f32x16 acc[DT];
 #pragma unroll
@@ -854,15 +897,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  int k0, k1;
-  split_range(klen, p.nsplit, id.split, k0, k1);
-  KvStage<CT, DP, KT, 256, VEC, VEC> st;
-  const int nt = (k1 - k0 + KT - 1) / KT;
-  if (nt > 0) {
-    st.init(p, id.b, id.hk, k0, k1, KT, tid);
-    st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
-    st.finish(p, Ks, Vs, kbs, flag, tid);
-  }
+  if (nt > 0) st.finish(p, Ks, Vs, kbs, flag, tid);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const int cur = t & 1;
@@ -875,10 +910,10 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
     for (int kt = 0; kt < NT; ++kt) {
       f32x16 s1[1], g = zero16();
       f32x16& s = s1[0];
-      key_scores<CT, DP, 1>(s1, Kc + 32 * kt * DP, qf, kbs + cur * KT + 32 * kt, holes, lane);
+      key_scores<CT, DP, 1>(s1, Kc + 32 * kt * DP, qf, kbs + cur * KT + 32 * kt, holes, p.D, lane);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        g = mma<CT>(row_frag<CT, DP>(Vc, 32 * kt + (lane & 31), 16 * ks, lane), gf[ks], g);
+        if (step_there<CT, DP>(ks, p.D)) g = mma<CT>(row_frag<CT, DP>(Vc, 32 * kt + (lane & 31), 16 * ks, lane), gf[ks], g);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse)) * (g[i] - delta);
 #pragma unroll
@@ -923,7 +958,7 @@ struct RowStage {
     return ASYNC ? ((tid >> 6) * P + i) * 64 + (tid & 63) : i * 256 + tid;
   }
   __device__ __forceinline__ void begin(const CrossP& p, CT* Qs, CT* Gs, int b, int hk, int row0, int end, int tid) {
-    const int n0 = row0 / p.G;
+    const int n0 = packed(p, row0).n;
     const CT* qb = vrow<CT>(p.q, b, n0, hk * p.G);
     const CT* gb = vrow<CT>(p.dout, b, n0, hk * p.G);
     u32x4 qr, gr;
@@ -931,7 +966,9 @@ struct RowStage {
     const unsigned first = __builtin_amdgcn_readfirstlane(tid >> 6) * P * 1024;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int lr = slot(i, tid) / CPR, row = row0 + lr, n = row / p.G, hd = row - n * p.G;
+      const int lr = slot(i, tid) / CPR, row = row0 + lr;
+      const PackedRow pk = packed(p, row);
+      const int n = pk.n, hd = pk.g;
       if constexpr (ASYNC) {
         const int c = slot(i, tid) % CPR ^ chunk_xor<CT, DP>(lr);
         const bool in = row < end && c * N < p.D;
@@ -949,7 +986,8 @@ struct RowStage {
     }
     lse = INFINITY, delta = 0.f;  // (every P of a row past the end, or without keys, is 0)
     if (tid < QT && row0 + tid < end) {
-      const int row = row0 + tid, n = row / p.G, hd = hk * p.G + row % p.G;
+      const PackedRow pk = packed(p, row0 + tid);
+      const int n = pk.n, hd = hk * p.G + pk.g;
       const long long i = ((long long)b * p.H + hd) * p.Nq + n;
       lse = p.lse[i], delta = p.delta[i];
       if (lse == -INFINITY) lse = INFINITY;
@@ -1020,6 +1058,7 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
       f32x16 s = zero16(), g = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        if (!step_there<CT, DP>(ks, p.D)) continue;
         s = mma<CT>(row_frag<CT, DP>(Qc, qt + (lane & 31), 16 * ks, lane), kf[ks], s);
         g = mma<CT>(row_frag<CT, DP>(Gc, qt + (lane & 31), 16 * ks, lane), vf[ks], g);
       }
@@ -1084,12 +1123,13 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossP p, int kv) 
     const float4 t = *reinterpret_cast<const float4*>(p.part + (s * nout * total + row) * DP + d0);
     v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
   }
-  const long long r0 = row % total;
-  const int bh = (int)(r0 / rows), r = (int)(r0 % rows), b = bh / p.Hk, hk = bh % p.Hk;
+  const int r0 = (int)(row < total ? row : row - total), bh = quot(r0, p.by_rows), r = r0 - bh * (int)rows;
+  const int b = quot(bh, p.by_hk), hk = bh - b * p.Hk;
   if (kv) {
     st_out<CT, VEC>(wrow<CT>(row < total ? p.dk : p.dv, b, r, hk), d0, p.D, v.x, v.y, v.z, v.w);
   } else {
-    st_out<CT, VEC>(wrow<CT>(p.dq, b, r / p.G, hk * p.G + r % p.G), d0, p.D, v.x * p.scale, v.y * p.scale,
+    const PackedRow pk = packed(p, r);
+    st_out<CT, VEC>(wrow<CT>(p.dq, b, pk.n, hk * p.G + pk.g), d0, p.D, v.x * p.scale, v.y * p.scale,
                v.z * p.scale, v.w * p.scale);
   }
 }
@@ -1125,8 +1165,14 @@ CrossP params(const mdg_attn_cross& a) {
   p.mb = a.mask_sb, p.mn = a.mask_sn;
   p.B = a.B, p.Nq = a.Nq, p.Nk = a.Nk, p.H = a.H, p.Hk = a.Hk, p.G = a.H / a.Hk, p.D = a.D;
   p.c = a.scale * kLog2e, p.scale = a.scale, p.lse = a.lse;
-  p.delta = nullptr, p.part = p.part_ml = nullptr, p.nsplit = 1;
+  p.delta = nullptr, p.part = p.part_ml = nullptr;
+  p.by_g = divisor(p.G), p.by_hk = divisor(p.Hk);
   return p;
+}
+// one launch's blocks: tiles x splits x (batch, key head), each of `rows` rows
+void shape(CrossP& p, long long tiles, int split, long long rows) {
+  p.nsplit = split;
+  p.by_split = divisor(split), p.by_tiles = divisor(tiles), p.by_rows = divisor(rows);
 }
 
 // 16-byte pieces: the head dim a multiple of a piece, every base and stride 16-byte aligned; and a tile's
@@ -1192,7 +1238,7 @@ hipError_t fwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
   constexpr int KT = sizeof(CT) == 2 ? 64 : 32;
   const Plan w = fwd_plan(a, VEC);
   CrossP p = params(a);
-  p.nsplit = w.split;
+  shape(p, w.tiles, w.split, (long long)a.Nq * p.G);
   if (w.split > 1) {
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.ml);
@@ -1234,7 +1280,7 @@ hipError_t bwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
   const size_t smk = (size_t)4 * QT * DP * sizeof(CT) + 4 * QT * 4;
   if ((e = allow_lds(cross_dq_kernel<CT, DP, KT, VEC>, smq)) != hipSuccess) return e;
   if ((e = allow_lds(cross_dkv_kernel<CT, DP, QT, VEC>, smk)) != hipSuccess) return e;
-  p.nsplit = w.qsplit;
+  shape(p, w.qtiles, w.qsplit, (long long)a.Nq * p.G);
   hipLaunchKernelGGL((cross_dq_kernel<CT, DP, KT, VEC>), dim3((unsigned)(w.qtiles * w.qsplit * a.B * a.Hk)), dim3(256), smq, s, p,
                      (int)w.qtiles);
   if (w.qsplit > 1) {
@@ -1242,7 +1288,7 @@ hipError_t bwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((cross_sum_kernel<CT, DP, VEC>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 0);
   }
   if (!a.dk.p || a.Nk == 0) return hipGetLastError();  // a frozen encoder, or none
-  p.nsplit = w.ksplit;
+  shape(p, w.ktiles, w.ksplit, a.Nk);
   hipLaunchKernelGGL((cross_dkv_kernel<CT, DP, QT, VEC>), dim3((unsigned)(w.ktiles * w.ksplit * a.B * a.Hk)), dim3(256), smk, s, p,
                      (int)w.ktiles);
   if (w.ksplit > 1) {
@@ -1278,7 +1324,8 @@ size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back) {
 bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back) {
   const long long lim = (1LL << 31) - 1, bh = (long long)a.B * a.Hk, dp4 = dp_of_head(a.D) / 4;
   const long long rows = (long long)a.Nq * (a.H / a.Hk);
-  if (rows > lim || rows * bh > lim || (long long)a.Nk * bh > lim) return false;
+  // (row and key numbers of the last tile, and a length rounded up to splits, must not pass 2^31 either)
+  if (rows > lim || rows * bh > lim - 8192 || (long long)a.Nk * bh > lim - 8192) return false;
   if (!back) {
     const Plan w = fwd_plan(a, false);  // (the other has half the tiles)
     return w.tiles * w.split * bh <= lim;
