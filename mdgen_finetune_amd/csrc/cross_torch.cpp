@@ -14,6 +14,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <initializer_list>
 #include <sstream>
@@ -93,8 +95,12 @@ Tensor bytes(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// (forward-mode tangents have no rule here and must not be dropped)
 bool any_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error("mdgen_finetune_amd.cross_hip: no forward-mode derivative, detach the tangent first");
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
@@ -309,6 +315,51 @@ struct RopeNode : OnceNode {
   }
 };
 
+// Writing in place, each element must be one memory location.  Dims are told apart by their strides, each
+// of which must span all that lies inside it (other layouts are taken to overlap).
+struct Dim {
+  int64_t stride, nx, ny;
+};
+using Dims = std::array<Dim, 4>;
+bool nested(Dims& dims) {  // sorts them, strides descending
+  std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+  int64_t reach = 0;
+  for (int i = 3; i >= 0; --i) {
+    const int64_t n = std::max(dims[i].nx, dims[i].ny);
+    if (n > 1 && dims[i].stride <= reach) return false;
+    reach += (n - 1) * dims[i].stride;
+  }
+  return true;
+}
+// whether sum (i_x - i_y) stride = d for some indices
+bool meets(const Dims& dims, int i, int64_t d) {
+  if (i == 4) return d == 0;
+  const int64_t s = dims[i].stride;
+  if (s == 0) return meets(dims, i + 1, d);
+  const int64_t f = d >= 0 ? d / s : -((-d + s - 1) / s);
+  for (int64_t n : {f, f + 1})
+    if (n < dims[i].nx && -n < dims[i].ny && meets(dims, i + 1, d - n * s)) return true;
+  return false;
+}
+bool may_share(const Tensor& x, const Tensor& y) {
+  if (!x.numel() || !y.numel()) return false;
+  const int64_t e = x.element_size(), d = static_cast<char*>(y.data_ptr()) - static_cast<char*>(x.data_ptr());
+  int64_t xend = e, yend = e;
+  for (int i = 0; i < 4; ++i) xend += (x.size(i) - 1) * x.stride(i) * e, yend += (y.size(i) - 1) * y.stride(i) * e;
+  if (d >= xend || -d >= yend) return false;
+  Dims dims;
+  for (int i = 0; i < 4; ++i) {
+    if (x.size(i) > 1 && y.size(i) > 1 && x.stride(i) != y.stride(i)) return true;
+    dims[i] = {x.size(i) > 1 ? x.stride(i) : y.size(i) > 1 ? y.stride(i) : 0, x.size(i), y.size(i)};
+  }
+  return d % e || !nested(dims) || meets(dims, 0, d / e);
+}
+bool apart(const Tensor& t) {
+  Dims dims;
+  for (int i = 0; i < 4; ++i) dims[i] = {t.size(i) > 1 ? t.stride(i) : 0, t.size(i), 1};
+  return nested(dims);
+}
+
 py::object rope_axes(const RopePlan& plan, Tensor pos, const Tensor& q, const MaybeTensor& k_, bool inverse, bool inplace) {
   variable_list x = {q};
   if (k_.has_value()) x.push_back(*k_);
@@ -332,11 +383,10 @@ py::object rope_axes(const RopePlan& plan, Tensor pos, const Tensor& q, const Ma
   variable_list y;
   if (inplace) {
     if (grad) value_error(Text() << "rope_axes: inplace on a tensor that requires grad");
-    for (const Tensor& t : x) {
-      bool ok = t.stride(3) == 1 || D == 1;
-      for (int i = 0; i < 3; ++i) ok = ok && (t.stride(i) != 0 || t.size(i) <= 1);
-      if (!ok) value_error(Text() << "rope_axes: inplace needs a contiguous head dim and no memory shared between tokens or heads");
-    }
+    for (const Tensor& t : x)
+      if ((t.stride(3) != 1 && D != 1) || !apart(t))
+        value_error(Text() << "rope_axes: inplace needs a contiguous head dim and no memory shared between tokens or heads");
+    if (x.size() == 2 && may_share(x[0], x[1])) value_error(Text() << "rope_axes: inplace on q and k that share memory");
     rope_launch(plan, pos, x, x, inverse);
     for (const Tensor& t : x)
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

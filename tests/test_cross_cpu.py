@@ -55,6 +55,7 @@ def _cross(**kw):
     (dict(mask_type=1), b"mask_type"), (dict(mask=0x1000), b"mask_type"), (dict(q=_lib.MdgHeads(None, 1, 1, 1)), b"null q"),
     (dict(k=_lib.MdgHeads(None, 1, 1, 1)), b"null k"), (dict(v=_lib.MdgHeads(0x1001, 1, 1, 1)), b"aligned"),
     (dict(q=_lib.MdgHeads(0x1000, -1, 1, 1)), b"strides"), (dict(B=1 << 20, Nq=1 << 20), b"grid"),
+    (dict(B=1, Nq=(1 << 31) - 100), b"grid"), (dict(B=1, Nk=(1 << 31) - 100), b"grid"),
 ])
 def test_cross_entry_refuses(kw, word):
     lib = _lib.load()

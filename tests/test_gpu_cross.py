@@ -713,3 +713,51 @@ def test_operators_on_a_device_that_is_not_current():
     with torch.cuda.device(1):
         other = [t.to("cuda:1") for t in ins]
     assert torch.equal(f(*other).cpu(), f(*ins).cpu()) and torch.cuda.current_device() == 0
+
+
+def test_rope_inplace_on_views_of_one_memory():
+    """q and k packed in one projection, by heads or interleaved, shared heads, a head-major cache: rotated where
+    they lie; views that share an element are refused."""
+    plan = X().RopeAxes([2, 2], device="cuda")
+    g = _gen(31)
+    pos = torch.randint(0, 99, (5, 2), generator=g).cuda()
+
+    def views(make, q, k):
+        base = make()
+        a, b = q(base), k(base)
+        wa, wb = X().rope_axes(plan, pos[: a.shape[1]], a.clone(), b.clone())
+        X().rope_axes(plan, pos[: a.shape[1]], a, b, inplace=True)
+        assert torch.equal(a, wa) and torch.equal(b, wb)
+
+    packed = lambda: torch.randn(2, 5, 10, 8, generator=g).cuda()
+    views(packed, lambda x: x[:, :, :8], lambda x: x[:, :, 8:9])
+    views(packed, lambda x: x[:, :, :5], lambda x: x[:, :, 5:])
+    views(packed, lambda x: x[:, :, ::2], lambda x: x[:, :, 1::2])
+    views(packed, lambda x: x[:, :1, :4], lambda x: x[:, :1, 4:8])
+    views(packed, lambda x: x[:1], lambda x: x[1:])
+    views(lambda: torch.randn(2, 10, 5, 8, generator=g).cuda(), lambda x: x[:, :6].transpose(1, 2), lambda x: x[:, 6:].transpose(1, 2))
+    views(lambda: torch.randn(2, 5, 4, 16, generator=g).cuda(), lambda x: x[..., :8], lambda x: x[..., 8:])
+    x = packed()
+    for q, k in ((x, x), (x[:, :, :5], x[:, :, 4:9]), (x[:, :, ::2], x[:, :, 2:3]), (x[:, :, :4], x[:, :, 3:9:2])):
+        with pytest.raises(ValueError, match="share memory"):
+            X().rope_axes(plan, pos, q, k, inplace=True)
+    with pytest.raises(ValueError, match="share|shared"):
+        X().rope_axes(plan, pos, x.reshape(-1).as_strided((2, 5, 2, 8), (200, 8, 8, 1)), inplace=True)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+
+    for f, ins in _small():
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(fwad.make_dual(ins[0], torch.ones_like(ins[0])), *ins[1:])
+
+
+@pytest.mark.parametrize("which", range(3), ids=["attention", "rope", "norms"])
+def test_backward_twice_with_retain_graph(which):
+    f, ins = _small()[which]
+    leaves = [t.clone().requires_grad_(True) for t in ins]
+    out = f(*leaves)
+    w = torch.randn_like(out)
+    one = torch.autograd.grad(out, leaves, w, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(one, torch.autograd.grad(out, leaves, w)))
