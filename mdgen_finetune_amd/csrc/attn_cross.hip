@@ -1320,19 +1320,19 @@ size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back) {
   return x > y ? x : y;
 }
 
-// grid sizes of every launch, for the host-side check (each must stay below 2^31)
+// Every launch within the 2^32 threads of a grid, and row and key numbers (the last tile's, past the end, and a
+// length rounded up to splits) within 31 bits.  (The joins' and sums' grids are small: splits come with
+// fewer than 1024 blocks.)
 bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back) {
-  const long long lim = (1LL << 31) - 1, bh = (long long)a.B * a.Hk, dp4 = dp_of_head(a.D) / 4;
+  const long long lim = (1LL << 31) - 8192, blocks = ((1LL << 32) - 1) / 512, bh = (long long)a.B * a.Hk;
   const long long rows = (long long)a.Nq * (a.H / a.Hk);
-  // (row and key numbers of the last tile, and a length rounded up to splits, must not pass 2^31 either)
-  if (rows > lim || rows * bh > lim - 8192 || (long long)a.Nk * bh > lim - 8192) return false;
+  if (rows > lim || rows * bh > lim || (long long)a.Nk * bh > lim) return false;
   if (!back) {
     const Plan w = fwd_plan(a, false);  // (the other has half the tiles)
-    return w.tiles * w.split * bh <= lim;
+    return w.tiles * w.split * bh <= blocks;
   }
   const BwdPlan w = bwd_plan(a);
-  return w.qtiles * w.qsplit * bh <= lim && w.ktiles * w.ksplit * bh <= lim && rows * bh * dp4 / 256 < lim &&
-         (long long)a.Nk * bh * 2 * dp4 / 256 < lim;
+  return w.qtiles * w.qsplit * bh <= blocks && w.ktiles * w.ksplit * bh <= blocks;
 }
 
 hipError_t attn_cross_launch(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s) {

@@ -133,7 +133,9 @@ hipError_t adam_step_launch(int nt, int nc, const void* table, double lr, double
 size_t attn_cross_ws_bytes(const mdg_attn_cross& a, bool back);
 bool attn_cross_grid_ok(const mdg_attn_cross& a, bool back);
 hipError_t attn_cross_launch(const mdg_attn_cross& a, bool back, void* ws, hipStream_t s);
+bool rope_axes_grid_ok(const mdg_rope_axes_desc& d);
 hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s);
+bool gate_res_norm_grid_ok(const mdg_gate_res_norm_desc& d, bool back);
 size_t gate_res_norm_ws_bytes(const mdg_gate_res_norm_desc& d);
 hipError_t gate_res_norm_fwd_launch(const mdg_gate_res_norm_desc& d, hipStream_t s);
 hipError_t gate_res_norm_bwd_launch(const mdg_gate_res_norm_desc& d, void* ws, hipStream_t s);
@@ -1700,6 +1702,7 @@ int check_grn(const mdg_gate_res_norm_desc* d, bool back, bool pointers) {
       (((uintptr_t)d->gate | (uintptr_t)d->shift | (uintptr_t)d->scale | (uintptr_t)d->post_w | (uintptr_t)d->post_b |
         (uintptr_t)d->pre_w | (uintptr_t)d->pre_b) & 3))
     return fail(MDG_E_ARG, "%s: a tensor is not aligned to its elements", who);
+  if (!mdg::gate_res_norm_grid_ok(*d, back)) return fail(MDG_E_SHAPE, "%s: grid too large", who);
   if (!back) {
     if (d->pre != MDG_NORM_NONE ? !d->xn : !d->h_out) return fail(MDG_E_ARG, "%s: no output", who);
     if (d->h_out == d->h && d->ldh != d->C) return fail(MDG_E_ARG, "%s: in place needs contiguous rows", who);
@@ -1759,6 +1762,7 @@ int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream) {
     if (d->x[i].p == d->out[i].p && (d->x[i].sb != d->out[i].sb || d->x[i].sn != d->out[i].sn || d->x[i].sh != d->out[i].sh))
       return fail(MDG_E_ARG, "rope_axes: in place needs out's strides equal to x's");
   }
+  if (!mdg::rope_axes_grid_ok(*d)) return fail(MDG_E_SHAPE, "rope_axes: grid too large");
   return hip_check(mdg::rope_axes_launch(*d, (hipStream_t)stream), "rope_axes");
 }
 

@@ -563,6 +563,15 @@ size_t gate_res_norm_ws_bytes(const mdg_gate_res_norm_desc& d) {
   return (size_t)groups(d) * (grn_chunks(d) + 1) * 4 * d.C * sizeof(float);
 }
 
+// every launch within the 2^32 threads of a grid, row numbers (the last blocks', past the end) within 31 bits
+bool gate_res_norm_grid_ok(const mdg_gate_res_norm_desc& d, bool back) {
+  const long long threads = (1LL << 32) - 4096, tpr = grn_shape(d.C, back && grn_vec(d) > 4 ? 4 : grn_vec(d)).tpr;
+  if (d.M > (1LL << 31) - 4096) return false;
+  if (!back) return d.M * tpr <= threads;
+  const long long G = groups(d);
+  return G * grn_chunks(d) * (tpr > 256 ? tpr : 256) <= threads && (!(want_y(d) || want_x(d)) || G * 1024 <= threads);
+}
+
 hipError_t gate_res_norm_fwd_launch(const mdg_gate_res_norm_desc& d, hipStream_t s) {
   grn_dispatch(d, grn_params(d), false, 0, s);
   return hipGetLastError();

@@ -235,6 +235,13 @@ static void rope_go(const RopeP& p, int dtype, int V, bool inter, unsigned grid,
 #undef ROPE_GO
 }
 
+// within the 2^32 threads of a grid
+bool rope_axes_grid_ok(const mdg_rope_axes_desc& d) {
+  int V;
+  const RopeP p = rope_params(d, V);
+  return (p.tokens - 1) / p.T < ((1LL << 32) - 1) / 256 - 1;
+}
+
 hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s) {
   int V;
   const RopeP p = rope_params(d, V);

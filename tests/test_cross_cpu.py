@@ -55,7 +55,7 @@ def _cross(**kw):
     (dict(mask_type=1), b"mask_type"), (dict(mask=0x1000), b"mask_type"), (dict(q=_lib.MdgHeads(None, 1, 1, 1)), b"null q"),
     (dict(k=_lib.MdgHeads(None, 1, 1, 1)), b"null k"), (dict(v=_lib.MdgHeads(0x1001, 1, 1, 1)), b"aligned"),
     (dict(q=_lib.MdgHeads(0x1000, -1, 1, 1)), b"strides"), (dict(B=1 << 20, Nq=1 << 20), b"grid"),
-    (dict(B=1, Nq=(1 << 31) - 100), b"grid"), (dict(B=1, Nk=(1 << 31) - 100), b"grid"),
+    (dict(B=1, Nq=(1 << 31) - 100), b"grid"), (dict(B=1, Nk=(1 << 31) - 100), b"grid"), (dict(B=1 << 23, Nq=1), b"grid"),
 ])
 def test_cross_entry_refuses(kw, word):
     lib = _lib.load()
@@ -103,6 +103,7 @@ def _rope(**kw):
     (dict(pos=None), b"null pos"), (dict(turns=0x1004), b"aligned"), (dict(pos_i64=1, pos=0x1004), b"aligned"),
     (dict(pos_sn=-1), b"strides of pos"), (dict(H=(0, 0)), b"H[0]"), (dict(x=(0, _lib.MdgHeads(None, 1, 1, 1))), b"null x"),
     (dict(out=(0, _lib.MdgHeads(0x1000, 1000, 100, 48))), b"in place"), (dict(B=(1 << 31) - 1, N=(1 << 31) - 1), b"grid"),
+    (dict(B=1 << 25, N=1, H=(0, 1024)), b"grid"),
 ])
 def test_rope_entry_refuses(kw, word):
     lib = _lib.load()
@@ -126,6 +127,7 @@ def _grn(**kw):
     (dict(ldy=1), b"ldy"), (dict(y=None), b"without y"), (dict(post=0, post_w=0x1000), b"post weights"),
     (dict(pre=0), b"without a pre norm"), (dict(gate=0x1000, mod_stride=3), b"mod_stride"), (dict(h=0x1002), b"aligned"),
     (dict(gate=0x1002, mod_stride=64), b"aligned"), (dict(xn=None), b"no output"), (dict(h_out=0x1000, ldh=128), b"in place"),
+    (dict(M=1 << 30), b"grid"), (dict(M=(1 << 31) - 1, C=1), b"grid"),
 ])
 def test_grn_entry_refuses(kw, word):
     lib = _lib.load()
@@ -137,6 +139,7 @@ def test_grn_entry_refuses(kw, word):
     (dict(), b"incoming"), (dict(dh_out=0x1000, dshift=0x1000), b"without dxn"),
     (dict(dxn=0x1000, dgate=0x1000, dmod_stride=2), b"dmod_stride"),
     (dict(dxn=0x1000, dgate=0x1000, dmod_stride=64), b"workspace"),
+    (dict(dxn=0x1000, dscale=0x1000, dmod_stride=64, M=1 << 23, rows_per_mod=1), b"grid"),
 ])
 def test_grn_backward_refuses(kw, word):
     lib = _lib.load()
