@@ -202,9 +202,7 @@ __device__ __forceinline__ bool key_kept(const CrossP& p, int b, int key) {
 // The softmax of one 32-key tile: raises the lane's maximum when a score outgrows it by 2^8 (a lagging
 // maximum costs no precision: P is floating point and stays below 2^8, sums are fp32), turns the
 // scores into P and adds their sum.  s: raw scores, -inf where the key is masked.
-// DT counts every accumulator that carries the lane's scale; SUM: l is summed here (otherwise by a
-// product with ones, in the last of them).
-template <int NT, int DT, bool SUM>
+template <int NT, int DT>
 __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NT], f32x16 (&o)[DT], float& m, float& l, float c) {
   const float grow = 8.0f / c;
   float mx = s[0][0];
@@ -230,9 +228,9 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[NT], f32x16 (&o)[DT], f
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -mc));
-      if constexpr (SUM) sum += s[t][i];
+      sum += s[t][i];
     }
-  if constexpr (SUM) l += sum;
+  l += sum;
 }
 
 // Asynchronous loads, memory -> LDS, 16 bytes per lane at lds + 16 * lane.  Offsets outside the
@@ -533,16 +531,9 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? ld_frag<CT, VEC>(qrow, 16 * ks + 8 * h, p.D) : zero8<CT>();
 
-  // narrow bf16 heads are bound by the vector unit: the row sums (of the rounded probabilities) then
-  // come from a product with ones, o[DT]
-  constexpr bool kOnes = sizeof(CT) == 2 && DP <= 64;
-  constexpr int NO = DT + (kOnes ? 1 : 0);
-  f32x16 o[NO];
+  f32x16 o[DT];
 #pragma unroll
-  for (int t = 0; t < NO; ++t) o[t] = zero16();
-  typename V8<CT>::T ones;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) ones[j] = (CT)1.f;
+  for (int t = 0; t < DT; ++t) o[t] = zero16();
   float m = kNoMax, l = 0.f;
 
   int k0, k1;
@@ -563,13 +554,12 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     const CT* Vc = Vs + cur * TILE;
     f32x16 s[NT];
     key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), p.D, lane);
-    softmax_tile<NT, NO, !kOnes>(s, o, m, l, p.c);
+    softmax_tile<NT, DT>(s, o, m, l, p.c);
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const typename V8<CT>::T pf = half_frag<CT>(s[kt], s2);
-        if constexpr (kOnes) o[DT] = mma<CT>(ones, pf, o[DT]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
           o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
@@ -578,7 +568,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     __syncthreads();
   }
 
-  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, kOnes ? o[NO - 1][0] : other_half_sum(l), lane);
+  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, other_half_sum(l), lane);
 }
 
 // The same with two groups of four waves (256 rows per block), one phase apart, each SIMD holding one wave
@@ -646,7 +636,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
       key_scores<CT, DP, NT>(s, Ks + (t & 1) * TILE, qf, kbs + (t & 1) * KT, __builtin_amdgcn_readfirstlane(flag[t & 1]), p.D, lane);
     __syncthreads();
     if (t < nt) {
-      softmax_tile<NT, DT, true>(s, o, m, l, p.c);
+      softmax_tile<NT, DT>(s, o, m, l, p.c);
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) pf[kt][0] = half_frag<CT>(s[kt], 0), pf[kt][1] = half_frag<CT>(s[kt], 1);
     }
@@ -717,7 +707,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     f32x16 s[1];
     key_scores<CT, DP, 1>(s, Ks + cur * TILE, qf, kbs, __builtin_amdgcn_readfirstlane(*flag), p.D, lane);
-    softmax_tile<1, DT, true>(s, o, m, l, p.c);
+    softmax_tile<1, DT>(s, o, m, l, p.c);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
       const typename V8<CT>::T pf = half_frag<CT>(s[0], s2);
