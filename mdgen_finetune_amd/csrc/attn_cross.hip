@@ -17,6 +17,10 @@
 // is row 8 (j >> 2) + 4h + (j & 3) of the 16-row step: col_frag reads it so, and no probability ever
 // moves between lanes.  Forward and dq hold S^T (one query per lane: its maximum, sum and offsets
 // are lane scalars); dk / dv hold S (one key per lane).
+//
+// What rounds: with bf16 inputs P and dS go to bf16 as operands of their second products (half a step of
+// 2^-8 each, the type of v and k beside them); scores, statistics, sums and every accumulator are fp32.
+// delta is formed with o + o_lo, o's own rounding residual: dP - delta cancels, and o's rounding would show.
 #include "../../include/mdgen_hip.h"
 #include "common.h"
 
@@ -199,7 +203,7 @@ __device__ __forceinline__ bool key_kept(const CrossP& p, int b, int key) {
 }
 
 
-// The softmax of one 32-key tile: raises the lane's maximum when a score outgrows it by 2^8 (a lagging
+// The softmax of NT 32-key tiles: raises the lane's maximum when a score outgrows it by 2^8 (a lagging
 // maximum costs no precision: P is floating point and stays below 2^8, sums are fp32), turns the
 // scores into P and adds their sum.  s: raw scores, -inf where the key is masked.
 template <int NT, int DT>
@@ -507,8 +511,15 @@ __device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, i
 }
 
 // ------------------------------------------------------------------------------------------ forward
-// One block = 4 waves x 32 rows of one (b, key head); k / v tiles of KT keys go through LDS, double
-// buffered through registers, one barrier per tile.
+// One block = 4 waves x 32 rows of one (b, key head), tiles of KT keys through two LDS buffers, one barrier per
+// tile; a tile's loads run under the products of the one before.  The running maximum and sum make it one
+// pass; no score is stored.
+// Narrow heads are bound by the vector unit (per 32 x 32 tile about 320 cycles of max, fma, exp, add and
+// convert against 128 of MFMA at D <= 32): [8, 4000, 16, 24] on 256 keys takes 48 us, of which 27 grow with the
+// keys and 10 are its 51 MB.  D = 64, [4, 4096, 16] on 2048 ragged keys: 152-166 us, 650 TFLOP/s.
+// Tried: two row groups per wave (the registers cost a wave per SIMD: 700 against 610 us at D = 128), 32-key
+// tiles (697), all keys in LDS with waves walking the rows (46 -> 42 us masked, equal unmasked, and
+// 37 -> 47 at D = 64 with 64 keys), row sums by a product with ones (1-2 % slower).
 template <typename CT, int DP, int KT, bool VEC>
 __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int tiles) {
   constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
@@ -578,6 +589,9 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
 //   M(t): O += V(t-1)^T P(t-1), S = K(t) Q^T;   V(t): P(t) = softmax of S
 // Group 0 loads: K(t+1) and V(t+1) start at its M(t) and are awaited at the end of its V(t); K lies in two
 // buffers, V, read a phase later, in three.
+// [2, 4096, 16, 128] on 4 heads of 8192 keys: 530 us, 1040 TFLOP/s (592 with the kernel above; a large library
+// product reaches 1130).  For D <= 64 it is no faster (654 against 654 us of training at D = 64, 51 against 52
+// at D = 24): fewer MFMA per score leave too little to run under the other phase.
 template <int DP, int KT>
 __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, int tiles) {
   using CT = bf16_t;
@@ -651,6 +665,8 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
 // At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
 // the rows.  Each wave stages its own 32-key tiles in two buffers of its own (no block barrier in the
 // loop: a wave's LDS operations are in order), and the four partial softmaxes are joined in LDS at the end.
+// Bound by memory, for which the splits keep four blocks per CU in flight: 16 sequences of one token, 32 heads
+// on 8 of 16384 keys (ragged, 806 MB) take 151 us (5.3 TB/s) and 7 of the join.  One short sequence: 4.6 us, a launch.
 // (fp32 at 128 columns: two buffers per wave would not fit, it stages through registers)
 template <typename CT, int DP, bool VEC>
 constexpr bool few_async() { return VEC && sizeof(CT) * DP <= 256; }
@@ -785,7 +801,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
 }
 
 // Joins the splits' partial softmaxes: 32 lanes per row.  A lane reads the statistics of the splits
-// lane, lane + 32, ...; then the lanes walk the splits in order, four columns each.
+// lane, lane + 32, ...; then the lanes walk the splits in order, four columns each.  6.5 us for 16016 rows of
+// 64 columns in 4 splits (16 MB), 7 for 512 rows in 8: latency.
 template <typename CT, int DP, bool VEC>
 __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
   const long long rows = (long long)p.Nq * p.G, total = rows * p.B * p.Hk;
@@ -831,7 +848,10 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
 
 // ------------------------------------------------------------------------------------------ backward
 // dq: the forward's layout (one query per lane).  delta = do . (o + o_lo) is formed here from the
-// fragments in registers and left for the dk / dv pass.
+// fragments in registers and left for the dk / dv pass.  Scores are formed anew from q, k and lse where a
+// stored P would be Nq x Nk of traffic.  dq and dk / dv are two kernels, each the sole writer of its
+// sums, so results repeat bit for bit (one kernel would have to add dq by atomics).
+// D = 64, [4, 4096, 16] on 2048 ragged keys: 202-219 us, 735 TFLOP/s; MFMA and vector unit 45 and 60 % busy.
 template <typename CT, int DP, int KT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_kernel(const CrossP p, int tiles) {
   constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
@@ -1000,6 +1020,9 @@ struct RowStage {
 // dk, dv: one key per lane; a block owns 4 x 32 keys of one (b, key head) and walks the rows in tiles
 // of QT (q and do through LDS, double buffered); splits share the rows, their fp32 partials summed in
 // order by cross_sum_kernel.
+// D = 64, [4, 4096, 16] on 2048 ragged keys: 340-370 us, 580 TFLOP/s: four accumulator tiles, the key
+// fragments and two tiles of scores take 232 registers, two waves per SIMD.  Held to 168 registers (three
+// waves) it takes 5 % longer, with an interleave of MFMA and vector instructions forced on the scheduler 1-2 %.
 template <typename CT, int DP, int QT, bool VEC>
 __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tiles) {
   constexpr int TILE = QT * DP, DT = DP / 32, KS = DP / 16;
@@ -1127,7 +1150,10 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossP p, int kv) 
 // ------------------------------------------------------------------------------------------ host
 int dp_of_head(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// Splits: enough blocks to fill 256 CUs several times over, none with less than `least` of the long axis.
+// Splits: enough blocks to fill 256 CUs `want` / 256 times over, none with less than `least` of the long axis.
+// want: 512 for blocks of four waves (dk / dv at D = 64: 1024 costs 679 against 658 us of training, the partials'
+// traffic; fp32: 768 the same as 512), 1024 for single tokens (memory), 256 for the eight waves of the
+// two-phase kernel.  least: 256, or 96 for fp32, whose products take sixteen times as long.
 int pick_split(long long blocks, long long len, int least, int want) {
   if (blocks <= 0 || blocks >= want || len <= least) return 1;
   const long long s = (want + blocks - 1) / blocks, most = (len + least - 1) / least;
@@ -1167,6 +1193,7 @@ void shape(CrossP& p, long long tiles, int split, long long rows) {
 
 // 16-byte pieces: the head dim a multiple of a piece, every base and stride 16-byte aligned; and a tile's
 // rows apart, within the 2^30 bytes that an asynchronous load's offset spans (64 keys, or 65 tokens)
+// (element by element instead: 693 against 610 us at D = 128)
 bool pieces(const mdg_attn_cross& a, bool bwd) {
   const int e = a.dtype == MDG_BF16 ? 2 : 4;
   const int64_t span = (int64_t)1 << 30;
@@ -1191,7 +1218,11 @@ size_t al(size_t n) { return (n + 255) / 256 * 256; }
 Plan fwd_plan(const mdg_attn_cross& a, bool vec) {
   Plan w;
   const long long rows = (long long)a.Nq * (a.H / a.Hk), bh = (long long)a.B * a.Hk;
+  // one 32-row tile: the waves split the keys.  (As 32-row blocks under more rows, fp32 [2, 1001, 8, 48] on 333
+  // keys: 26.8 us against 21.8 + 6.7 of the join, for four times the k / v reads: not used.)
   w.few = rows <= 32;
+  // wide bf16 heads: [8, 256, 16, 128] on 1024 keys 40.7 us against 44.3 of the plain kernel, [4, 1024, 16, 96] on 1024
+  // keys 46.0 / 47.1; below 256 rows half of its waves would idle
   w.pp = a.dtype == MDG_BF16 && vec && dp_of_head(a.D) == 128 && rows >= 256;
   w.tiles = w.few ? 1 : w.pp ? (rows + 255) / 256 : (rows + 127) / 128;
   w.split = pick_split(w.tiles * bh, a.Nk, a.dtype == MDG_F32 && !w.few ? 96 : 256, w.few ? 1024 : w.pp ? 256 : 512);
