@@ -170,6 +170,21 @@ __device__ __forceinline__ typename V8<CT>::T ld_frag(const CT* row, int c0, int
   return r;
 }
 
+// and back: the columns c0 .. (c0 < D) of a row
+template <typename CT, bool VEC>
+__device__ __forceinline__ void st_piece(CT* row, int c0, int D, const uint4& u) {
+  constexpr int N = 16 / sizeof(CT);
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(row + c0) = u;
+  } else {
+    CT e[N];
+    __builtin_memcpy(e, &u, 16);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (c0 + j < D) row[c0 + j] = e[j];
+  }
+}
+
 // four consecutive outputs d0 .. d0 + 3 of a row
 template <typename CT, bool VEC>
 __device__ __forceinline__ void st_out(CT* row, int d0, int D, float a, float b, float c, float d) {
@@ -551,6 +566,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
   split_range(p, klen, id.split, k0, k1);
   KvStage<CT, DP, KT, 256, VEC, VEC> st;
   const int nt = (k1 - k0 + KT - 1) / KT;
+  const bool busy = id.tile * 128 + wave * 32 < qlen * p.G;  // (otherwise the wave has no row, and only loads)
   if (nt > 0) {
     st.init(p, id.b, id.hk, k0, k1, KT, tid);
     st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
@@ -563,18 +579,20 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     if (t + 1 < nt) st.begin(p, Ks + other, Vs + other, id.b, k0 + (t + 1) * KT, k1, KT, tid);
     const CT* Kc = Ks + cur * TILE;
     const CT* Vc = Vs + cur * TILE;
-    f32x16 s[NT];
-    key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), p.D, lane);
-    softmax_tile<NT, DT>(s, o, m, l, p.c);
+    if (busy) {
+      f32x16 s[NT];
+      key_scores<CT, DP, NT>(s, Kc, qf, kbs + cur * KT, __builtin_amdgcn_readfirstlane(flag[cur]), p.D, lane);
+      softmax_tile<NT, DT>(s, o, m, l, p.c);
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
+      for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const typename V8<CT>::T pf = half_frag<CT>(s[kt], s2);
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const typename V8<CT>::T pf = half_frag<CT>(s[kt], s2);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
-      }
+          for (int dt = 0; dt < DT; ++dt)
+            o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
+        }
+    }
     if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
     __syncthreads();
   }
@@ -847,6 +865,43 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
 }
 
 // ------------------------------------------------------------------------------------------ backward
+// delta = do . (o + o_lo) of a lane's row, from memory; h: the lane's half of the columns
+template <typename CT, int KS, bool VEC>
+__device__ __forceinline__ float row_delta(const CrossP& p, int b, int n, int head, bool live, int h) {
+  float delta = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int c0 = 16 * ks + 8 * h;
+    const typename V8<CT>::T g = live ? ld_frag<CT, VEC>(vrow<CT>(p.dout, b, n, head), c0, p.D) : zero8<CT>();
+    const typename V8<CT>::T o = live ? ld_frag<CT, VEC>(vrow<CT>(p.o, b, n, head), c0, p.D) : zero8<CT>();
+    if (p.olo.p) {
+      const typename V8<CT>::T lo = live ? ld_frag<CT, VEC>(vrow<CT>(p.olo, b, n, head), c0, p.D) : zero8<CT>();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf((float)g[j], (float)o[j] + (float)lo[j], delta);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf((float)g[j], (float)o[j], delta);
+    }
+  }
+  return other_half_sum(delta);
+}
+
+// S, dP of 32 rows (8a + 4h + i) by one key per lane -> P, dS; ls, ds: the rows' lse and delta
+__device__ __forceinline__ void grad_scores(f32x16& s, f32x16& g, const float* ls, const float* ds, float c, int h) {
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const float4 lv = *reinterpret_cast<const float4*>(ls + 8 * a + 4 * h);
+    const float4 dl = *reinterpret_cast<const float4*>(ds + 8 * a + 4 * h);
+    const float lw[4] = {lv.x, lv.y, lv.z, lv.w}, dw[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * a + i], c, -lw[i]));
+      s[4 * a + i] = pr;
+      g[4 * a + i] = pr * (g[4 * a + i] - dw[i]);
+    }
+  }
+}
+
 // dq: the forward's layout (one query per lane).  delta = do . (o + o_lo) is formed here from the
 // fragments in registers and left for the dk / dv pass.  Scores are formed anew from q, k and lse where a
 // stored P would be Nq x Nk of traffic.  dq and dk / dv are two kernels, each the sole writer of its
@@ -867,7 +922,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
   const PackedRow pk = packed(p, r);
   const int n = pk.n, head = id.hk * p.G + pk.g;
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
-  const bool live = r < rows && n < qlen;
+  const bool live = r < rows && n < qlen, busy = id.tile * 128 + wave * 32 < qlen * p.G;
   const int ln = live ? n : 0, lh = live ? head : 0;
   const long long srow = ((long long)id.b * p.H + lh) * p.Nq + ln;
 
@@ -918,6 +973,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
     const bool holes = __builtin_amdgcn_readfirstlane(flag[cur]);
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt) {
+      if (!busy) break;  // (a wave without rows only loads)
       f32x16 s1[1], g = zero16();
       f32x16& s = s1[0];
       key_scores<CT, DP, 1>(s1, Kc + 32 * kt * DP, qf, kbs + cur * KT + 32 * kt, holes, p.D, lane);
@@ -1021,7 +1077,7 @@ struct RowStage {
 // of QT (q and do through LDS, double buffered); splits share the rows, their fp32 partials summed in
 // order by cross_sum_kernel.
 // D = 64, [4, 4096, 16] on 2048 ragged keys: 340-370 us, 580 TFLOP/s: four accumulator tiles, the key
-// fragments and two tiles of scores take 232 registers, two waves per SIMD.  Held to 168 registers (three
+// fragments and two tiles of scores take 204 registers, two waves per SIMD.  Held to 168 registers (three
 // waves) it takes 5 % longer, with an interleave of MFMA and vector instructions forced on the scheduler 1-2 %.
 template <typename CT, int DP, int QT, bool VEC>
 __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tiles) {
@@ -1037,7 +1093,7 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
   const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
   const int rows = qlen * p.G;
   const int key = id.tile * 128 + wave * 32 + (lane & 31);
-  const bool live = key < klen && key_kept(p, id.b, key);
+  const bool live = key < klen && key_kept(p, id.b, key), busy = id.tile * 128 + wave * 32 < klen;
 
   typename V8<CT>::T kf[KS], vf[KS];
 #pragma unroll
@@ -1068,6 +1124,7 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
     const CT* Gc = Gs + cur * TILE;
 #pragma unroll
     for (int qt = 0; qt < QT; qt += 32) {
+      if (!busy) break;  // (a wave without keys only loads)
       f32x16 s = zero16(), g = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -1075,18 +1132,7 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
         s = mma<CT>(row_frag<CT, DP>(Qc, qt + (lane & 31), 16 * ks, lane), kf[ks], s);
         g = mma<CT>(row_frag<CT, DP>(Gc, qt + (lane & 31), 16 * ks, lane), vf[ks], g);
       }
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const float4 lv = *reinterpret_cast<const float4*>(ls + cur * QT + qt + 8 * a + 4 * h);
-        const float4 dl = *reinterpret_cast<const float4*>(ds + cur * QT + qt + 8 * a + 4 * h);
-        const float lw[4] = {lv.x, lv.y, lv.z, lv.w}, dw[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * a + i], p.c, -lw[i]));
-          s[4 * a + i] = pr;
-          g[4 * a + i] = pr * (g[4 * a + i] - dw[i]);
-        }
-      }
+      grad_scores(s, g, ls + cur * QT + qt, ds + cur * QT + qt, p.c, h);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const typename V8<CT>::T pf = half_frag<CT>(s, s2), df = half_frag<CT>(g, s2);
@@ -1119,6 +1165,199 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
         st_out<CT, VEC>(wrow<CT>(p.dv, id.b, key, id.hk), d0, p.D, y[0], y[1], y[2], y[3]);
       }
     }
+}
+
+// The whole backward for at most 32 rows per (b, key head): one pass over the keys.  As in cross_few_kernel
+// the waves split the keys, each with 32-key tiles of its own; q and do lie in LDS for all of them.  Per tile
+//   S^T, dP^T (one query per lane) -> dS^T -> dq^T += K^T dS^T,    summed over tiles, waves and splits;
+//   S, dP (one key per lane) -> P, dS -> dv^T = dO^T P, dk^T = Q^T dS,   complete here: all rows are in the tile.
+// The same two fragments in either order give the two score tiles, and k and v are read once: bound by memory.
+// 8 sequences of one token, 16 heads of 128 on 8192 bf16 keys (k and v read, dk and dv written, 1.07 GB): 230 us,
+// 4.6 TB/s, against 102 + 460 us of the two kernels above; 4 of 7 tokens, 32 heads of 64 on 8 of 4000 keys 21 against
+// 13.6 + 24.2; fp32, 4 of 20 tokens, 8 heads of 64 on 3000 keys 57 against 47 + 33 (its products).  dk and dv leave
+// through LDS, 16 bytes per lane.  fp32 wider than 64 columns would spill (160 us against 78 + 64): not built.
+template <typename CT, int DP>
+constexpr bool few_bwd() { return sizeof(CT) * DP <= 256; }
+template <typename CT, int DP, bool VEC>
+__global__ __launch_bounds__(256) void cross_few_bwd_kernel(const CrossP p) {
+  constexpr int W = 4, TILE = 32 * DP, DT = DP / 32, KS = DP / 16, LO = DP + 4;
+  constexpr int BUFS = few_async<CT, DP, VEC>() ? 2 : 1, N = 16 / sizeof(CT), CPR = DP / N;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  CT* Qs = reinterpret_cast<CT*>(smem);
+  CT* Gs = Qs + TILE;
+  CT* Ks = Gs + TILE + wave * 2 * BUFS * TILE;
+  CT* Vs = Ks + BUFS * TILE;
+  float* ls = reinterpret_cast<float*>(Qs + (2 + 2 * BUFS * W) * TILE);  // [32], then delta [32]
+  float* ds = ls + 32;
+  float* kbs = ds + 32 + wave * 32;
+  int* flag = reinterpret_cast<int*>(ds + 32 + W * 32) + wave;
+
+  const BlockId id = block_id(p, 1);
+  const int rows = p.Nq * p.G, r = lane & 31;
+  const PackedRow pk = packed(p, r);
+  const int qlen = clamp_len(p.qlen, id.b, p.Nq), klen = clamp_len(p.klen, id.b, p.Nk);
+  const bool live = r < rows && pk.n < qlen;
+  const int n = live ? pk.n : 0, head = live ? id.hk * p.G + pk.g : 0;
+
+  int k0, kend;  // this block's keys; those past the sequence's end have gradients too, zeros
+  split_range(p, p.Nk, id.split, k0, kend);
+  const int k1 = min(kend, klen);
+  using S = KvStage<CT, DP, 32, 64, VEC, BUFS == 2>;
+  S st;
+  int key = k0 + 32 * wave, cur = 0;
+  if (key < k1) {
+    st.init(p, id.b, id.hk, key, k1, 32 * W, lane);
+    st.begin(p, Ks, Vs, id.b, key, k1, 32 * W, lane);
+  }
+  for (int i = tid; i < 32 * CPR; i += 64 * W) {
+    const int row = i / CPR, c = i % CPR;
+    const PackedRow q = packed(p, row);
+    const bool in = row < rows && q.n < qlen && c * N < p.D;
+    const int hd = id.hk * p.G + q.g;
+    *reinterpret_cast<uint4*>(Qs + lds_at<CT, DP>(row, c)) =
+        in ? ld_piece<CT, VEC>(vrow<CT>(p.q, id.b, q.n, hd), c * N, p.D) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(Gs + lds_at<CT, DP>(row, c)) =
+        in ? ld_piece<CT, VEC>(vrow<CT>(p.dout, id.b, q.n, hd), c * N, p.D) : make_uint4(0, 0, 0, 0);
+  }
+  const float delta = row_delta<CT, KS, VEC>(p, id.b, n, head, live, h);
+  float lse = live ? p.lse[((long long)id.b * p.H + head) * p.Nq + n] : -INFINITY;
+  if (lse == -INFINITY) lse = INFINITY;  // a row without keys, or none: every P is 0
+  if (wave == 0 && h == 0) ls[r] = lse, ds[r] = delta;
+  __syncthreads();
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = zero16();
+  for (; key < k1; key += 32 * W) {
+    st.finish_kb(kbs, flag, lane);
+    const bool more = key + 32 * W < k1;
+    if constexpr (BUFS == 2) {
+      if (more) {
+        st.begin(p, Ks + (cur ^ 1) * TILE, Vs + (cur ^ 1) * TILE, id.b, key + 32 * W, k1, 32 * W, lane);
+        async_wait<2 * S::P>();  // this tile's loads, not the next one's
+      } else {
+        async_wait();
+      }
+    } else {
+      st.finish_rows(p, Ks, Vs, lane);
+      if (more) st.begin(p, Ks, Vs, id.b, key + 32 * W, k1, 32 * W, lane);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const CT* Kt = Ks + cur * TILE;
+    const CT* Vt = Vs + cur * TILE;
+    const bool holes = __builtin_amdgcn_readfirstlane(*flag);
+    {
+      typename V8<CT>::T qf[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = row_frag<CT, DP>(Qs, r, 16 * ks, lane);
+      f32x16 s[1], g = zero16();
+      key_scores<CT, DP, 1>(s, Kt, qf, kbs, holes, p.D, lane);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (step_there<CT, DP>(ks, p.D)) g = mma<CT>(row_frag<CT, DP>(Vt, r, 16 * ks, lane), row_frag<CT, DP>(Gs, r, 16 * ks, lane), g);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(fmaf(s[0][i], p.c, -lse)) * (g[i] - delta);
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const typename V8<CT>::T df = half_frag<CT>(s[0], s2);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mma<CT>(col_frag<CT, DP>(Kt, 16 * s2, 32 * dt, lane), df, acc[dt]);
+      }
+    }
+    if (p.dk.p) {
+      f32x16 s = zero16(), g = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (!step_there<CT, DP>(ks, p.D)) continue;
+        s = mma<CT>(row_frag<CT, DP>(Qs, r, 16 * ks, lane), row_frag<CT, DP>(Kt, r, 16 * ks, lane), s);
+        g = mma<CT>(row_frag<CT, DP>(Gs, r, 16 * ks, lane), row_frag<CT, DP>(Vt, r, 16 * ks, lane), g);
+      }
+      const bool there = kbs[r] == 0.f;  // (key `key + r`)
+      grad_scores(s, g, ls, ds, p.c, h);
+      typename V8<CT>::T pf[2], df[2];
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) pf[s2] = half_frag<CT>(s, s2), df[s2] = half_frag<CT>(g, s2);
+      // over the k and v tiles, which are done with, then out by whole rows
+      CT* Kw = Ks + cur * TILE;
+      CT* Vw = Vs + cur * TILE;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        f32x16 x = zero16(), y = zero16();
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          if (16 * s2 >= rows) continue;  // (the rows past them are zeros)
+          x = mma<CT>(col_frag<CT, DP>(Qs, 16 * s2, 32 * dt, lane), df[s2], x);
+          y = mma<CT>(col_frag<CT, DP>(Gs, 16 * s2, 32 * dt, lane), pf[s2], y);
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int d0 = 32 * dt + 8 * a + 4 * h, at = lds_at<CT, DP>(r, d0 / N) + d0 % N;
+          st4<CT>(Kw + at, there ? x[4 * a] * p.scale : 0.f, there ? x[4 * a + 1] * p.scale : 0.f,
+                  there ? x[4 * a + 2] * p.scale : 0.f, there ? x[4 * a + 3] * p.scale : 0.f);
+          st4<CT>(Vw + at, there ? y[4 * a] : 0.f, there ? y[4 * a + 1] : 0.f, there ? y[4 * a + 2] : 0.f, there ? y[4 * a + 3] : 0.f);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      CT* dk = wrow<CT>(p.dk, id.b, key, id.hk);
+      CT* dv = wrow<CT>(p.dv, id.b, key, id.hk);
+      for (int i = lane; i < 32 * CPR; i += 64) {
+        const int row = i / CPR, c = i % CPR, at = lds_at<CT, DP>(row, c);
+        if (key + row < kend && c * N < p.D) {
+          st_piece<CT, VEC>(dk + row * p.dk.sn, c * N, p.D, *reinterpret_cast<const uint4*>(Kw + at));
+          st_piece<CT, VEC>(dv + row * p.dv.sn, c * N, p.D, *reinterpret_cast<const uint4*>(Vw + at));
+        }
+      }
+    }
+    // the next turn's loads overwrite this buffer: its reads are done before they start
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if constexpr (BUFS == 2) cur ^= 1;
+  }
+  if (p.dk.p)
+    for (; key < kend; key += 32 * W)
+      for (int i = lane; i < 32 * CPR; i += 64) {
+        const int at = key + i / CPR, c0 = i % CPR * N;
+        if (at < kend && c0 < p.D) {
+          st_piece<CT, VEC>(wrow<CT>(p.dk, id.b, at, id.hk), c0, p.D, make_uint4(0, 0, 0, 0));
+          st_piece<CT, VEC>(wrow<CT>(p.dv, id.b, at, id.hk), c0, p.D, make_uint4(0, 0, 0, 0));
+        }
+      }
+
+  // dq of the waves, [W][32][DP + 4] over the tiles, summed in order
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last tile's reads are done
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  float* jo = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      *reinterpret_cast<float4*>(jo + (32 * wave + r) * LO + 32 * dt + 8 * a + 4 * h) =
+          make_float4(acc[dt][4 * a], acc[dt][4 * a + 1], acc[dt][4 * a + 2], acc[dt][4 * a + 3]);
+  __syncthreads();
+  for (int i = tid; i < rows * (DP / 4); i += 64 * W) {
+    const int row = i / (DP / 4), d0 = (i % (DP / 4)) * 4;
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float4 t = *reinterpret_cast<const float4*>(jo + (32 * w + row) * LO + d0);
+      v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+    }
+    if (p.nsplit > 1) {
+      *reinterpret_cast<float4*>(p.part + part_row(p, id.split, id.b, id.hk, row) * DP + d0) = v;
+    } else {
+      const PackedRow q = packed(p, row);
+      st_out<CT, VEC>(wrow<CT>(p.dq, id.b, q.n, id.hk * p.G + q.g), d0, p.D, v.x * p.scale, v.y * p.scale, v.z * p.scale,
+                      v.w * p.scale);
+    }
+  }
 }
 
 // sums the splits' fp32 partials in order: nout planes [rows][DP] per split -> the strided outputs.
@@ -1235,6 +1474,7 @@ Plan fwd_plan(const mdg_attn_cross& a, bool vec) {
 }
 
 struct BwdPlan {
+  bool few;  // one pass over the keys for one 32-row tile
   long long qtiles, ktiles;
   int qsplit, ksplit;  // splits of the dq pass (over keys) and of the dk / dv pass (over rows)
   size_t delta, part, bytes;
@@ -1243,8 +1483,9 @@ BwdPlan bwd_plan(const mdg_attn_cross& a) {
   BwdPlan w;
   const long long rows = (long long)a.Nq * (a.H / a.Hk), bh = (long long)a.B * a.Hk;
   w.qtiles = (rows + 127) / 128, w.ktiles = ((long long)a.Nk + 127) / 128;
-  w.qsplit = pick_split(w.qtiles * bh, a.Nk, a.dtype == MDG_F32 ? 96 : 256, 512);
-  w.ksplit = pick_split(w.ktiles * bh, rows, a.dtype == MDG_F32 ? 96 : 256, 512);
+  w.few = rows <= 32 && dp_of_head(a.D) * (a.dtype == MDG_F32 ? 4 : 2) <= 256;
+  w.qsplit = w.few ? pick_split(bh, a.Nk, 256, 1024) : pick_split(w.qtiles * bh, a.Nk, a.dtype == MDG_F32 ? 96 : 256, 512);
+  w.ksplit = w.few ? 1 : pick_split(w.ktiles * bh, rows, a.dtype == MDG_F32 ? 96 : 256, 512);
   w.delta = 0;
   w.part = al((size_t)a.B * a.H * a.Nq * 4);
   const size_t dp = dp_of_head(a.D);
@@ -1297,6 +1538,20 @@ hipError_t bwd(const mdg_attn_cross& a, void* ws, hipStream_t s) {
   p.delta = reinterpret_cast<float*>(static_cast<char*>(ws) + w.delta);
   p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);
   hipError_t e;
+  if (w.few) {
+    if constexpr (few_bwd<CT, DP>()) {
+    const size_t tiles = (size_t)(2 + 8 * (few_async<CT, DP, VEC>() ? 2 : 1)) * 32 * DP * sizeof(CT) + (64 + 128 + 4) * 4;
+    const size_t join = (size_t)128 * (DP + 4) * 4, sm = tiles > join ? tiles : join;
+    if ((e = allow_lds(cross_few_bwd_kernel<CT, DP, VEC>, sm)) != hipSuccess) return e;
+    shape(p, 1, w.qsplit, (long long)a.Nq * p.G);
+    hipLaunchKernelGGL((cross_few_bwd_kernel<CT, DP, VEC>), dim3((unsigned)(w.qsplit * a.B * a.Hk)), dim3(256), sm, s, p);
+    if (w.qsplit > 1) {
+      const long long n = (long long)a.B * a.H * a.Nq * (DP / 4);
+      hipLaunchKernelGGL((cross_sum_kernel<CT, DP, VEC>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, 0);
+    }
+    return hipGetLastError();
+    }
+  }
   const size_t smq = (size_t)4 * KT * DP * sizeof(CT) + 2 * KT * 4 + 16;
   const size_t smk = (size_t)4 * QT * DP * sizeof(CT) + 4 * QT * 4;
   if ((e = allow_lds(cross_dq_kernel<CT, DP, KT, VEC>, smq)) != hipSuccess) return e;

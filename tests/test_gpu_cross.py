@@ -169,6 +169,25 @@ def test_cross_attention_forward_backward(case, dt):
         _near(got, w, t, n)
 
 
+# at most 32 rows per key head: the backward in one pass over the keys, its waves and splits, ends of sequences
+FEW = [
+    (1, 1, 33, 1, 1, 64, "", "tokens"),
+    (2, 32, 257, 2, 2, 32, "len q", "tokens"),
+    (3, 4, 700, 16, 2, 128, "len mask", "heads"),
+    (2, 17, 1300, 2, 2, 96, "mask", "tokens"),
+    (4, 1, 2100, 16, 4, 64, "len", "odd"),
+    (2, 2, 1111, 15, 1, 36, "mask bool len q", "dfirst"),
+    (1, 31, 3000, 1, 1, 72, "len", "heads"),
+    (2, 6, 96, 5, 1, 128, "mask len q", "odd"),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", FEW, ids=lambda c: "-".join(str(x) for x in c))
+def test_cross_attention_few_rows(case, dt):
+    test_cross_attention_forward_backward(case, dt)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("Nq,Nk,G", [(1, 5000, 4), (2, 20000, 1), (45, 6000, 1)])
 def test_cross_attention_splits_a_long_key_axis(Nq, Nk, G, dt):
