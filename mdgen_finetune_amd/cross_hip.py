@@ -13,8 +13,9 @@ position on each of several axes (frame, residue, ...), and the branch is normal
 
 Tensors are fp32 or bf16 on a ROCm device, any strides with a contiguous last dim (other orders are
 copied).  Calls run on the current stream of the tensors' device, allocate only outputs and
-workspaces through torch's caching allocator (so they may be captured into a HIP graph), and are
-differentiable where an input requires grad.  Wrong types and shapes raise TypeError / ValueError
+workspaces through torch's caching allocator (so they may be captured into a HIP graph; a backward pass
+only while no eager graph of the same leaves is alive, whose accumulation torch ties to its own stream), and
+are differentiable, once, where an input requires grad.  Wrong types and shapes raise TypeError / ValueError
 before any launch; a missing library or a CPU tensor raises RuntimeError (there is no other path).
 """
 from __future__ import annotations
@@ -87,10 +88,11 @@ class RopeAxes:
         elif pairs == "interleaved":
             first, second = list(range(0, 2 * n, 2)), list(range(1, 2 * n, 2))
         self.sections, self.pairs, self.npairs = sections, pairs, n
-        device = torch.device("cuda" if device is None else device)
-        self.turns = (freq / (2.0 * math.pi)).to(device)
-        self.axis = torch.tensor([a for a, s in enumerate(sections) for _ in range(s)], dtype=torch.int32).to(device)
-        self.cols = torch.tensor(first + second, dtype=torch.int32).to(device)
+        axis = [a for a, s in enumerate(sections) for _ in range(s)]
+        # one copy to the device: the frequencies in turns (fp64), then three int32 tables
+        tables = torch.cat([(freq / (2.0 * math.pi)).view(torch.int32), torch.tensor(axis + first + second, dtype=torch.int32)])
+        tables = tables.to(torch.device("cuda" if device is None else device))
+        self.turns, self.axis, self.cols = tables[: 2 * n].view(torch.float64), tables[2 * n : 3 * n], tables[3 * n :]
         self._plan = None
 
     def __getstate__(self):
