@@ -5,13 +5,14 @@
 // sin per pair into LDS, once for all heads (the angle is formed in double as a number of turns and
 // reduced there: a position of 10^6 in fp32 would lose it), then a sweep over the tokens' rows in
 // memory order.  q and k go in one launch: their heads are one list.
-// fp32 [2, 50001] tokens of 16 heads x 64 columns (820 MB): 203 us, 4.0 TB/s; bf16 [8, 4000] tokens of 32 heads x
-// 24 columns on two axes of 6 pairs (98 MB in 4-byte runs): 27 us, 3.6 TB/s; one token 3 us.  A large copy
+// fp32 [2, 50001] tokens of 16 heads x 64 columns (820 MB): 203 us, 4.0 TB/s; one token 3 us.  A large copy
 // reaches 5.1 TB/s.  Tried: token bases in LDS (57 -> 69 us for both directions: a dependent read before every
 // load), the division by N as a multiplication, half and a quarter of the LDS entries (the same),
 // non-temporal accesses and heads unrolled per thread (slower).
 #include "../../include/mdgen_hip.h"
 #include "common.h"
+
+#include <initializer_list>
 
 namespace mdg {
 namespace {
@@ -35,6 +36,7 @@ struct RopeP {
   int rot_tasks, tasks;  // per head row: rotations of V pairs, then copies of copy_w columns (2V or V)
   int copy_w;
   int T;  // tokens per block
+  int lds;  // rope_tile_kernel's bytes, 0: the other kernel
   float inv_np, inv_tasks, inv_row;  // 1 / pairs, tasks, tasks of a token
 };
 
@@ -43,6 +45,17 @@ constexpr int kRopeLds = 2048;  // (token, pair) entries of a block
 // i / d for 0 <= i < 2^21 and d < 2^21: (i + 1/2) / d is at least 1 / (2 d) from a whole number, well
 // beyond the products' rounding there
 __device__ __forceinline__ int small_div(int i, float inv_d) { return (int)(((float)i + 0.5f) * inv_d); }
+
+// cos and (signed) sin of pair pr at token (b, n)
+__device__ __forceinline__ void turn_of(const RopeP& p, unsigned b, unsigned n, int pr, float& cs, float& sn) {
+  const long long at = b * p.pb + n * p.pn + p.axis[pr];
+  const double ps = p.i64 ? (double)reinterpret_cast<const long long*>(p.pos)[at]
+                          : (double)reinterpret_cast<const int*>(p.pos)[at];
+  const double turn = ps * p.turns[pr];
+  float s, c;
+  sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);  // half turns in [-1, 1]
+  cs = c, sn = p.inverse ? -s : s;
+}
 
 template <typename CT, int W> struct Pack { CT v[W]; };
 template <typename CT, int W>
@@ -99,13 +112,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeP p) {
   for (int i = tid; i < T * p.np; i += 256) {
     const int t = small_div(i, p.inv_np), pr = i - t * p.np;
     const unsigned b = (t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
-    const long long at = b * p.pb + n * p.pn + p.axis[pr];
-    const double ps = p.i64 ? (double)reinterpret_cast<const long long*>(p.pos)[at]
-                            : (double)reinterpret_cast<const int*>(p.pos)[at];
-    const double turn = ps * p.turns[pr];
-    float s, c;
-    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);  // half turns in [-1, 1]
-    cs[i] = c, sn[i] = p.inverse ? -s : s;
+    turn_of(p, b, n, pr, cs[i], sn[i]);
   }
   __syncthreads();
   constexpr int W = INTER ? 2 * V : V;
@@ -151,6 +158,64 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeP p) {
   }
 }
 
+// The same where an item would be one or two pairs but head rows are whole 16-byte pieces (sections of 6 or 5
+// pairs, odd pair counts): rows go through LDS, in and out 16 bytes per lane, and are rotated there.  A
+// thread keeps its (token, run) and walks the heads, so its cos, sin and columns stay in registers.
+// [8, 4000] tokens of 16 heads x 64, us with the kernel above / this one: bf16 axis 11 + 11 + 10 pairs 56 / 32,
+// interleaved 10 + 12 39 / 28 and 9 + 8 69 / 27; fp32 axis 11 + 11 + 10 57 / 49, 10 + 6 57 / 47, interleaved 9 + 6 69 / 46
+// (5.7 TB/s, partly from cache); 32 heads x 24 bf16, axis 6 + 6, 27 / 24.  bf16 axis 12 + 20, four pairs at a time: 26 / 30.
+constexpr int kRopeTile = 24576;  // bytes of rows per block
+template <typename CT, int V>
+__global__ __launch_bounds__(256) void rope_tile_kernel(const RopeP p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int N = 16 / sizeof(CT);
+  const int tid = threadIdx.x, pieces = p.D / N;
+  const int t0 = blockIdx.x * p.T, T = min(p.T, (int)p.tokens - t0);
+  // a token's rows, one piece apart from a multiple of the banks
+  const int per = p.HT * pieces, step = (per | 1) * N;
+  CT* tile = reinterpret_cast<CT*>(smem);
+  for (int i = tid; i < T * per; i += 256) {
+    const int t = small_div(i, p.inv_row), j = i - t * per, hd = small_div(j, p.inv_tasks), c = j - hd * pieces;
+    const unsigned b = (unsigned)(t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
+    const int second = hd >= p.H0, h = second ? hd - p.H0 : hd;
+    const RopeSeg& g = p.seg[second];
+    const CT* x = reinterpret_cast<const CT*>(g.x) + b * g.xb + n * g.xn + h * g.xh;
+    *reinterpret_cast<uint4*>(tile + t * step + j * N) = *reinterpret_cast<const uint4*>(x + c * N);
+  }
+  __syncthreads();
+  const int runs = p.np / V, combos = T * runs, groups = combos < 256 ? 256 / combos : 1;
+  for (int c = tid; c < combos * groups; c += 256) {
+    const int grp = c / combos, cc = c - grp * combos, t = cc / runs, p0 = (cc - t * runs) * V;
+    const unsigned b = (unsigned)(t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
+    float cs[V], sn[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) turn_of(p, b, n, p0 + k, cs[k], sn[k]);
+    const int c1 = p.cols[p0], c2 = p.cols[p.np + p0];
+    CT* row = tile + t * step + grp * p.D;
+    for (int hd = grp; hd < p.HT; hd += groups, row += groups * p.D) {
+      const Pack<CT, V> a = ldw<CT, V>(row + c1), d = ldw<CT, V>(row + c2);
+      Pack<CT, V> r, q;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float v = (float)a.v[k], w = (float)d.v[k];
+        r.v[k] = (CT)(v * cs[k] - w * sn[k]);
+        q.v[k] = (CT)(w * cs[k] + v * sn[k]);
+      }
+      stw<CT, V>(row + c1, r);
+      stw<CT, V>(row + c2, q);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < T * per; i += 256) {
+    const int t = small_div(i, p.inv_row), j = i - t * per, hd = small_div(j, p.inv_tasks), c = j - hd * pieces;
+    const unsigned b = (unsigned)(t0 + t) / (unsigned)p.N, n = t0 + t - b * p.N;
+    const int second = hd >= p.H0, h = second ? hd - p.H0 : hd;
+    const RopeSeg& g = p.seg[second];
+    CT* y = reinterpret_cast<CT*>(g.y) + b * g.yb + n * g.yn + h * g.yh;
+    *reinterpret_cast<uint4*>(y + c * N) = *reinterpret_cast<const uint4*>(tile + t * step + j * N);
+  }
+}
+
 }  // namespace
 
 // largest run V (columns) such that every run starts at a multiple of V and V elements are aligned
@@ -173,6 +238,16 @@ static int rope_v(const mdg_rope_axes_desc& d, int e) {
   return 1;
 }
 
+// Items of one or two pairs, shorter than 16 bytes, whole 16-byte pieces per head row, and a token's rows in a tile
+static bool rope_tiled(const mdg_rope_axes_desc& d, int V, int heads) {
+  const int e = d.dtype == MDG_BF16 ? 2 : 4, run = V * e * (d.pairs == MDG_ROPE_INTERLEAVED ? 2 : 1);
+  if (V > 2 || run >= 16 || d.D * e % 16 || heads * d.D * e > kRopeTile - 16) return false;
+  for (int i = 0; i < d.nseg; ++i)
+    for (const mdg_heads* t : {&d.x[i], &d.out[i]})
+      if (((uintptr_t)t->p | (uintptr_t)(t->sb * e) | (uintptr_t)(t->sn * e) | (uintptr_t)(t->sh * e)) & 15) return false;
+  return true;
+}
+
 static RopeP rope_params(const mdg_rope_axes_desc& d, int& V) {
   const int e = d.dtype == MDG_BF16 ? 2 : 4;
   V = rope_v(d, e);
@@ -192,6 +267,16 @@ static RopeP rope_params(const mdg_rope_axes_desc& d, int& V) {
   p.rot_tasks = d.npairs / V;
   p.copy_w = tail % (2 * V) == 0 ? 2 * V : V;
   p.tasks = p.rot_tasks + tail / p.copy_w;
+  p.lds = 0;
+  if (rope_tiled(d, V, p.HT)) {
+    if (d.pairs == MDG_ROPE_INTERLEAVED) V = 1;  // (two runs of one column)
+    const int per = p.HT * d.D * e / 16, row = (per | 1) * 16;
+    int T = kRopeTile / row, few = (int)((p.tokens + 1023) / 1024);
+    if (T > few) T = few;
+    p.T = T < 1 ? 1 : T, p.lds = p.T * row;
+    p.inv_np = 0.f, p.inv_tasks = 1.0f / (d.D * e / 16), p.inv_row = 1.0f / per;  // of pieces
+    return p;
+  }
   // tokens per block: about 2048 items, and 1024 blocks where there are that many tokens
   const int row = p.HT * p.tasks;
   int T = 2048 / row, few = (int)((p.tokens + 1023) / 1024);
@@ -212,6 +297,18 @@ bool rope_axes_pair_aligned(const mdg_rope_axes_desc& d) {
         return false;
   }
   return true;
+}
+
+static void rope_tile_go(const RopeP& p, int dtype, int V, unsigned grid, hipStream_t s) {
+#define ROPE_GO(CT, V_) hipLaunchKernelGGL((rope_tile_kernel<CT, V_>), dim3(grid), dim3(256), p.lds, s, p)
+  if (dtype == MDG_BF16) {
+    if (V == 2) ROPE_GO(bf16_t, 2);
+    else ROPE_GO(bf16_t, 1);
+  } else {
+    if (V == 2) ROPE_GO(float, 2);
+    else ROPE_GO(float, 1);
+  }
+#undef ROPE_GO
 }
 
 static void rope_go(const RopeP& p, int dtype, int V, bool inter, unsigned grid, hipStream_t s) {
@@ -252,7 +349,9 @@ hipError_t rope_axes_launch(const mdg_rope_axes_desc& d, hipStream_t s) {
   const RopeP p = rope_params(d, V);
   // (interleaved pairs that do not lie on a word of two elements take the two-run kernel: V is 1 then)
   const bool inter = d.pairs == MDG_ROPE_INTERLEAVED && rope_axes_pair_aligned(d);
-  rope_go(p, d.dtype, V, inter, (p.tokens + p.T - 1) / p.T, s);
+  const unsigned grid = (p.tokens + p.T - 1) / p.T;
+  if (p.lds) rope_tile_go(p, d.dtype, V, grid, s);
+  else rope_go(p, d.dtype, V, inter, grid, s);
   return hipGetLastError();
 }
 

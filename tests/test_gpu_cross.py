@@ -302,6 +302,16 @@ def _rope_oracle(x, pos, sections, pairs, base, sign):
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("pairs", ["half", "interleaved", "axis"])
+@pytest.mark.parametrize("B,N,H,Hk,D,sections,store", [  # (runs of one or two pairs in whole 16-byte pieces)
+    (2, 300, 5, 3, 64, [11, 11, 9], "tokens"), (1, 77, 2, 1, 24, [6, 6], "heads"), (3, 40, 40, 8, 32, [3, 5], "tokens"),
+    (1, 2, 300, 20, 16, [1, 0, 6], "tokens"), (5, 1, 1, 1, 8, [1, 1], "heads"), (2, 700, 3, 1, 128, [14, 18, 2], "tokens"),
+])
+def test_rope_axes_short_runs(B, N, H, Hk, D, sections, store, pairs, dt):
+    test_rope_axes_forward_backward(B, N, H, Hk, D, sections, store, pairs, dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("pairs", ["half", "interleaved", "axis"])
 @pytest.mark.parametrize("B,N,H,Hk,D,sections,store", [
     (1, 1, 1, 1, 2, [1], "tokens"), (2, 5, 4, 2, 24, [6, 6], "tokens"), (3, 7, 2, 1, 64, [8, 8, 16], "heads"),
     (2, 9, 3, 3, 33, [3, 5, 0, 7], "odd"), (1, 300, 12, 4, 128, [16, 24, 24], "tokens"), (2, 4, 40, 8, 48, [16], "dfirst"),
