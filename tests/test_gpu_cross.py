@@ -229,6 +229,51 @@ def test_cross_attention_broadcast_inputs_and_frozen_encoder():
     assert torch.isfinite(ds).all()
 
 
+@pytest.mark.parametrize("dt,D", [(torch.bfloat16, 128), (torch.bfloat16, 24), (torch.float32, 64)], ids=str)
+def test_cross_attention_few_rows_frozen_broadcast_captured(dt, D):
+    """Three query tokens in two splits: what masked keys hold (NaN) is without effect, a frozen encoder's dq is the
+    same bits, k and v shared by the batch, and a captured pass replayed on new inputs."""
+    B, Nq, Nk, H, Hk = 2, 3, 900, 4, 2
+    g = _gen(77)
+    q, k, v, do = (torch.randn(B, n, h, D, generator=g).to(dt).cuda() for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
+    ln = torch.tensor([900, 411], dtype=torch.int32, device="cuda")
+    mask = (torch.rand(B, Nk, generator=g) < 0.8).cuda()
+    gone = ~mask | (torch.arange(Nk, device="cuda")[None] >= ln[:, None])
+
+    def grads(q, k, v, do, **kw):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(X().cross_attention(*leaves, mask=mask, kv_len=ln, **kw), leaves, do)
+
+    base = grads(q, k, v, do)
+    kn, vn = (torch.where(gone[..., None, None], float("nan"), t) for t in (k, v))
+    again = grads(q, kn, vn, do)
+    assert all(torch.equal(a, b) for a, b in zip(base, again))
+    assert not base[1][gone].any() and not base[2][gone].any()
+    ql = q.clone().requires_grad_(True)
+    (dq,) = torch.autograd.grad(X().cross_attention(ql, k, v, mask=mask, kv_len=ln), ql, do)
+    assert torch.equal(dq, base[0])
+    wide = [t.expand(B, -1, -1, -1) for t in (k[:1], v[:1])]
+    assert all(torch.equal(a, b) for a, b in zip(grads(q, *wide, do), grads(q, *(t.contiguous() for t in wide), do)))
+
+    static = [t.clone() for t in (q, k, v, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grads(*static)
+    for turn in range(4):
+        new = [torch.randn(t.shape, generator=g).to(dt).cuda() for t in static]
+        for a, b in zip(static, new):
+            a.copy_(b)
+        graph.replay()
+        want = grads(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
 def test_cross_attention_gradient_against_differences():
     B, Nq, Nk, H, D = 1, 3, 6, 2, 8
     q, k, v, do, *_ = _attn_inputs(B, Nq, Nk, H, 1, D, torch.float32, "", 9)
