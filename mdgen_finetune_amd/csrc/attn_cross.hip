@@ -684,7 +684,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
 // the rows.  Each wave stages its own 32-key tiles in two buffers of its own (no block barrier in the
 // loop: a wave's LDS operations are in order), and the four partial softmaxes are joined in LDS at the end.
 // Bound by memory, for which the splits keep four blocks per CU in flight: 16 sequences of one token, 32 heads
-// on 8 of 16384 keys (ragged, 806 MB) take 151 us (5.3 TB/s) and 7 of the join.  One short sequence: 4.6 us, a launch.
+// on 8 of 16384 keys (ragged, 806 MB) take 151 us (5.3 TB/s) and 4.5 of the join.  One short sequence: 4.6 us, a launch.
 // (fp32 at 128 columns: two buffers per wave would not fit, it stages through registers)
 template <typename CT, int DP, bool VEC>
 constexpr bool few_async() { return VEC && sizeof(CT) * DP <= 256; }
@@ -819,8 +819,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
 }
 
 // Joins the splits' partial softmaxes: 32 lanes per row.  A lane reads the statistics of the splits
-// lane, lane + 32, ...; then the lanes walk the splits in order, four columns each.  6.5 us for 16016 rows of
-// 64 columns in 4 splits (16 MB), 7 for 512 rows in 8: latency.
+// lane, lane + 32, ...; then the lanes walk the splits in order, four columns each.  5.9 us for 16016 rows of
+// 64 columns in 4 splits (16 MB), 4.5 for 512 rows of 128 in 8.
 template <typename CT, int DP, bool VEC>
 __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
   const long long rows = (long long)p.Nq * p.G, total = rows * p.B * p.Hk;
@@ -841,12 +841,16 @@ __global__ __launch_bounds__(256) void cross_join_kernel(const CrossP p) {
       lf = f * ml.y;
     }
     const int n = min(32, p.nsplit - s0);
-    for (int s = 0; s < n; ++s) {
-      const float fs = __shfl(f, (threadIdx.x & 32) + s, 64);
-      L += __shfl(lf, (threadIdx.x & 32) + s, 64);
-      if (d0 < DP) {
-        const float4 t = *reinterpret_cast<const float4*>(p.part + ((s0 + s) * total + pr) * DP + d0);
-        v.x = fmaf(fs, t.x, v.x), v.y = fmaf(fs, t.y, v.y), v.z = fmaf(fs, t.z, v.z), v.w = fmaf(fs, t.w, v.w);
+    for (int s = 0; s < n; s += 4) {  // four loads in flight; past the last split f is 0
+      float4 t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t[j] = d0 < DP && s + j < n ? *reinterpret_cast<const float4*>(p.part + ((s0 + s + j) * total + pr) * DP + d0) : make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float fs = __shfl(f, (threadIdx.x & 32) + s + j, 64);
+        L += __shfl(lf, (threadIdx.x & 32) + s + j, 64);
+        v.x = fmaf(fs, t[j].x, v.x), v.y = fmaf(fs, t[j].y, v.y), v.z = fmaf(fs, t[j].z, v.z), v.w = fmaf(fs, t[j].w, v.w);
       }
     }
   }
@@ -1371,6 +1375,7 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossP p, int kv) 
   const int d0 = (int)(i % Q) * 4, nout = kv ? 2 : 1;
   if (row >= total * nout) return;
   float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
   for (int s = 0; s < p.nsplit; ++s) {
     const float4 t = *reinterpret_cast<const float4*>(p.part + (s * nout * total + row) * DP + d0);
     v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
@@ -1458,7 +1463,7 @@ Plan fwd_plan(const mdg_attn_cross& a, bool vec) {
   Plan w;
   const long long rows = (long long)a.Nq * (a.H / a.Hk), bh = (long long)a.B * a.Hk;
   // one 32-row tile: the waves split the keys.  (As 32-row blocks under more rows, fp32 [2, 1001, 8, 48] on 333
-  // keys: 26.8 us against 21.8 + 6.7 of the join, for four times the k / v reads: not used.)
+  // keys: 26.8 us against 21.8 + 5.9 of the join, for four times the k / v reads: not used.)
   w.few = rows <= 32;
   // wide bf16 heads: [8, 256, 16, 128] on 1024 keys 40.7 us against 44.3 of the plain kernel, [4, 1024, 16, 96] on 1024
   // keys 46.0 / 47.1; below 256 rows half of its waves would idle
