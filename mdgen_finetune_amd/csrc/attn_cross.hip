@@ -1082,7 +1082,8 @@ struct RowStage {
 // order by cross_sum_kernel.
 // D = 64, [4, 4096, 16] on 2048 ragged keys: 340-370 us, 580 TFLOP/s: four accumulator tiles, the key
 // fragments and two tiles of scores take 204 registers, two waves per SIMD.  Held to 168 registers (three
-// waves) it takes 5 % longer, with an interleave of MFMA and vector instructions forced on the scheduler 1-2 %.
+// waves) it takes 5 % longer, with an interleave of MFMA and vector instructions forced on the scheduler 1-2 %,
+// with more splits 5-8 %, also where the blocks past a sequence's end are dealt out evenly over the CUs.
 template <typename CT, int DP, int QT, bool VEC>
 __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tiles) {
   constexpr int TILE = QT * DP, DT = DP / 32, KS = DP / 16;
