@@ -161,10 +161,12 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(const RopeP p) {
 // The same where an item would be one or two pairs but head rows are whole 16-byte pieces (sections of 6 or 5
 // pairs, odd pair counts): rows go through LDS, in and out 16 bytes per lane, and are rotated there.  A
 // thread keeps its (token, run) and walks the heads, so its cos, sin and columns stay in registers.
-// [8, 4000] tokens of 16 heads x 64, us with the kernel above / this one: bf16 axis 11 + 11 + 10 pairs 56 / 32,
-// interleaved 10 + 12 39 / 28 and 9 + 8 69 / 27; fp32 axis 11 + 11 + 10 57 / 49, 10 + 6 57 / 47, interleaved 9 + 6 69 / 46
-// (5.7 TB/s, partly from cache); 32 heads x 24 bf16, axis 6 + 6, 27 / 24.  bf16 axis 12 + 20, four pairs at a time: 26 / 30.
-constexpr int kRopeTile = 24576;  // bytes of rows per block
+// [8, 4000] tokens of 16 heads x 64, us with the kernel above / this one: bf16 axis 11 + 11 + 10 pairs 56 / 31,
+// interleaved 10 + 12 39 / 28 and 9 + 8 69 / 27; fp32 axis 11 + 11 + 10 57 / 49, 10 + 6 57 / 50, interleaved 9 + 6 69 / 47
+// (5.5 TB/s, partly from cache); 32 heads x 24 bf16, axis 6 + 6, 27 / 23.  bf16 axis 12 + 20, four pairs at a time: 26 / 30.
+// Bytes of rows per block: 16 KiB, ten blocks per CU (of 24 or 12 KiB within 5 %, 32: bf16 axis 35.7 against 31 us), where one
+// token needs more than that up to twice as much.
+constexpr int kRopeTile = 16384;
 template <typename CT, int V>
 __global__ __launch_bounds__(256) void rope_tile_kernel(const RopeP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -241,7 +243,7 @@ static int rope_v(const mdg_rope_axes_desc& d, int e) {
 // Items of one or two pairs, shorter than 16 bytes, whole 16-byte pieces per head row, and a token's rows in a tile
 static bool rope_tiled(const mdg_rope_axes_desc& d, int V, int heads) {
   const int e = d.dtype == MDG_BF16 ? 2 : 4, run = V * e * (d.pairs == MDG_ROPE_INTERLEAVED ? 2 : 1);
-  if (V > 2 || run >= 16 || d.D * e % 16 || heads * d.D * e > kRopeTile - 16) return false;
+  if (V > 2 || run >= 16 || d.D * e % 16 || heads * d.D * e > 2 * kRopeTile - 16) return false;
   for (int i = 0; i < d.nseg; ++i)
     for (const mdg_heads* t : {&d.x[i], &d.out[i]})
       if (((uintptr_t)t->p | (uintptr_t)(t->sb * e) | (uintptr_t)(t->sn * e) | (uintptr_t)(t->sh * e)) & 15) return false;

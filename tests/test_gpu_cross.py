@@ -350,6 +350,7 @@ def _rope_oracle(x, pos, sections, pairs, base, sign):
 @pytest.mark.parametrize("B,N,H,Hk,D,sections,store", [  # (runs of one or two pairs in whole 16-byte pieces)
     (2, 300, 5, 3, 64, [11, 11, 9], "tokens"), (1, 77, 2, 1, 24, [6, 6], "heads"), (3, 40, 40, 8, 32, [3, 5], "tokens"),
     (1, 2, 300, 20, 16, [1, 0, 6], "tokens"), (5, 1, 1, 1, 8, [1, 1], "heads"), (2, 700, 3, 1, 128, [14, 18, 2], "tokens"),
+    (1, 5, 48, 12, 128, [7, 9], "tokens"), (1, 3, 64, 64, 128, [5, 5, 3], "tokens"),
 ])
 def test_rope_axes_short_runs(B, N, H, Hk, D, sections, store, pairs, dt):
     test_rope_axes_forward_backward(B, N, H, Hk, D, sections, store, pairs, dt)
