@@ -11,8 +11,8 @@
 //   dshift = S1, dscale = w2 S2 + b2 S1, dgate = w1 S4 + b1 S3   (per group)
 //   dw2 = sum_g (1 + scale) S2, db2 = sum_g (1 + scale) S1, dw1 = sum_g gate S4, db1 = sum_g gate S3
 // Bound by memory: forward 30 us at [32000, 384] (fp32 residual, bf16 branch: 147 MB, 4.9 TB/s of a copy's 5.1),
-// 132 us at [16383, 4096] in bf16 (537 MB, 4.1 TB/s); backward 57-64 us at [32000, 384] (221 MB, 3.7 TB/s; 168
-// registers, three waves per SIMD), its column sums 5 + 4 us.
+// 132 us at [16383, 4096] in bf16 (537 MB, 4.1 TB/s); backward 57-64 us at [32000, 384] (221 MB, 3.7 TB/s; 162
+// registers, three waves per SIMD), its column sums 5 + 4 us, and 92 us in all at [8000, 2048] (295 MB).
 // A row lives in the registers of TPR threads (32 or 64 lanes of a wave, or the whole block of 256, or of
 // 1024 for long rows of odd length), NV vectors of V elements each, so it is read once; statistics are
 // fp32, the variance from the centred row.  xn is formed from h' before h' is rounded, and the backward recomputes h' from h
@@ -495,56 +495,97 @@ Shape grn_shape(int C, int V) {
   return {256, 8};
 }
 
+// The backward's: four sums per column beside the row, so fewer vectors per thread and larger teams (registers,
+// waves per SIMD: one vector 71, 7; two 118, 4; three 162, 3; four 218, 2).  [3 x 1500, 4096] bf16 99 us, with the
+// forward's four vectors of 256 threads 135, with 1024 threads 174; [8 x 4000, 384] the same with two vectors of 64 lanes.
+Shape grn_back_shape(int C, int V) {
+  const int n = (C + V - 1) / V;
+  if (V == 1) return grn_shape(C, 1);
+  for (int nv = 1; nv <= 3; ++nv)
+    if (n <= 32 * nv) return {32, nv};
+  if (n <= 128) return {64, 2};
+  for (int nv = 1; nv <= 2; ++nv)
+    if (n <= 256 * nv) return {256, nv};
+  return n <= 1024 ? Shape{512, 2} : Shape{1024, 2};
+}
+
 template <typename RT, typename CT, int V, int TPR, int NV>
-void grn_go(const GrnP& p, bool back, int G, hipStream_t s) {
+void grn_go(const GrnP& p, hipStream_t s) {
   constexpr int BD = TPR < 256 ? 256 : TPR, TEAMS = BD / TPR, ROWS = TPR == 256 ? 2 : 1;
-  if (back) {
-    if constexpr (V <= 4) hipLaunchKernelGGL((grn_bwd_kernel<RT, CT, V, TPR, NV>), dim3((unsigned)(G * p.chunks)), dim3(BD), 0, s, p);
-    return;
-  }
   hipLaunchKernelGGL((grn_fwd_kernel<RT, CT, V, TPR, NV, ROWS>), dim3((unsigned)((p.M + TEAMS * ROWS - 1) / (TEAMS * ROWS))),
                           dim3(BD), 0, s, p);
 }
+template <typename RT, typename CT, int V, int TPR, int NV>
+void grn_back(const GrnP& p, int G, hipStream_t s) {
+  hipLaunchKernelGGL((grn_bwd_kernel<RT, CT, V, TPR, NV>), dim3((unsigned)(G * p.chunks)), dim3(TPR < 256 ? 256 : TPR), 0, s, p);
+}
 
 template <typename RT, typename CT, int V>
-void grn_by_shape(const GrnP& p, bool back, int G, hipStream_t s) {
+void grn_by_shape(const GrnP& p, hipStream_t s) {
   const Shape sh = grn_shape(p.C, V);
   if constexpr (V == 1) {
-    if (sh.tpr == 64) grn_go<RT, CT, 1, 64, 4>(p, back, G, s);
-    else if (sh.nv == 4) grn_go<RT, CT, 1, 256, 4>(p, back, G, s);
-    else if (sh.tpr == 256) grn_go<RT, CT, 1, 256, 8>(p, back, G, s);
-    else grn_go<RT, CT, 1, 1024, 8>(p, back, G, s);
+    if (sh.tpr == 64) grn_go<RT, CT, 1, 64, 4>(p, s);
+    else if (sh.nv == 4) grn_go<RT, CT, 1, 256, 4>(p, s);
+    else if (sh.tpr == 256) grn_go<RT, CT, 1, 256, 8>(p, s);
+    else grn_go<RT, CT, 1, 1024, 8>(p, s);
   } else {
     switch (sh.tpr * 16 + sh.nv) {
-      case 32 * 16 + 1: grn_go<RT, CT, V, 32, 1>(p, back, G, s); break;
-      case 32 * 16 + 2: grn_go<RT, CT, V, 32, 2>(p, back, G, s); break;
-      case 32 * 16 + 3: grn_go<RT, CT, V, 32, 3>(p, back, G, s); break;
-      case 64 * 16 + 2: grn_go<RT, CT, V, 64, 2>(p, back, G, s); break;
-      case 64 * 16 + 3: grn_go<RT, CT, V, 64, 3>(p, back, G, s); break;
-      case 64 * 16 + 4: grn_go<RT, CT, V, 64, 4>(p, back, G, s); break;
-      case 256 * 16 + 2: grn_go<RT, CT, V, 256, 2>(p, back, G, s); break;
-      case 256 * 16 + 3: grn_go<RT, CT, V, 256, 3>(p, back, G, s); break;
-      case 256 * 16 + 4: grn_go<RT, CT, V, 256, 4>(p, back, G, s); break;
+      case 32 * 16 + 1: grn_go<RT, CT, V, 32, 1>(p, s); break;
+      case 32 * 16 + 2: grn_go<RT, CT, V, 32, 2>(p, s); break;
+      case 32 * 16 + 3: grn_go<RT, CT, V, 32, 3>(p, s); break;
+      case 64 * 16 + 2: grn_go<RT, CT, V, 64, 2>(p, s); break;
+      case 64 * 16 + 3: grn_go<RT, CT, V, 64, 3>(p, s); break;
+      case 64 * 16 + 4: grn_go<RT, CT, V, 64, 4>(p, s); break;
+      case 256 * 16 + 2: grn_go<RT, CT, V, 256, 2>(p, s); break;
+      case 256 * 16 + 3: grn_go<RT, CT, V, 256, 3>(p, s); break;
+      case 256 * 16 + 4: grn_go<RT, CT, V, 256, 4>(p, s); break;
       default:
-        if constexpr (V == 4) grn_go<RT, CT, V, 256, 8>(p, back, G, s);
+        if constexpr (V == 4) grn_go<RT, CT, V, 256, 8>(p, s);
         break;
     }
   }
+}
+template <typename RT, typename CT, int V>
+void grn_back_by_shape(const GrnP& p, int G, hipStream_t s) {
+  const Shape sh = grn_back_shape(p.C, V);
+  if constexpr (V == 1) {
+    if (sh.tpr == 64) grn_back<RT, CT, 1, 64, 4>(p, G, s);
+    else if (sh.nv == 4) grn_back<RT, CT, 1, 256, 4>(p, G, s);
+    else if (sh.tpr == 256) grn_back<RT, CT, 1, 256, 8>(p, G, s);
+    else grn_back<RT, CT, 1, 1024, 8>(p, G, s);
+  } else {
+    switch (sh.tpr * 16 + sh.nv) {
+      case 32 * 16 + 1: grn_back<RT, CT, V, 32, 1>(p, G, s); break;
+      case 32 * 16 + 2: grn_back<RT, CT, V, 32, 2>(p, G, s); break;
+      case 32 * 16 + 3: grn_back<RT, CT, V, 32, 3>(p, G, s); break;
+      case 64 * 16 + 2: grn_back<RT, CT, V, 64, 2>(p, G, s); break;
+      case 256 * 16 + 1: grn_back<RT, CT, V, 256, 1>(p, G, s); break;
+      case 256 * 16 + 2: grn_back<RT, CT, V, 256, 2>(p, G, s); break;
+      case 512 * 16 + 2: grn_back<RT, CT, V, 512, 2>(p, G, s); break;
+      default: grn_back<RT, CT, V, 1024, 2>(p, G, s); break;
+    }
+  }
+}
+
+template <typename RT, typename CT, int V>
+void grn_dispatch_v(const GrnP& p, bool back, int G, hipStream_t s) {
+  if (!back) grn_by_shape<RT, CT, V>(p, s);
+  else if constexpr (V <= 4) grn_back_by_shape<RT, CT, V>(p, G, s);
 }
 
 void grn_dispatch(const mdg_gate_res_norm_desc& d, const GrnP& p, bool back, int G, hipStream_t s) {
   // (the backward's rows, sums and parameters fill the registers at 4 columns per vector)
   const int v = back ? (grn_vec(d) < 4 ? 1 : 4) : grn_vec(d);
   if (d.res_dtype == MDG_BF16) {
-    if (v == 8) grn_by_shape<bf16_t, bf16_t, 8>(p, back, G, s);
-    else if (v == 4) grn_by_shape<bf16_t, bf16_t, 4>(p, back, G, s);
-    else grn_by_shape<bf16_t, bf16_t, 1>(p, back, G, s);
+    if (v == 8) grn_dispatch_v<bf16_t, bf16_t, 8>(p, back, G, s);
+    else if (v == 4) grn_dispatch_v<bf16_t, bf16_t, 4>(p, back, G, s);
+    else grn_dispatch_v<bf16_t, bf16_t, 1>(p, back, G, s);
   } else if (d.dtype == MDG_BF16) {
-    if (v == 4) grn_by_shape<float, bf16_t, 4>(p, back, G, s);
-    else grn_by_shape<float, bf16_t, 1>(p, back, G, s);
+    if (v == 4) grn_dispatch_v<float, bf16_t, 4>(p, back, G, s);
+    else grn_dispatch_v<float, bf16_t, 1>(p, back, G, s);
   } else {
-    if (v == 4) grn_by_shape<float, float, 4>(p, back, G, s);
-    else grn_by_shape<float, float, 1>(p, back, G, s);
+    if (v == 4) grn_dispatch_v<float, float, 4>(p, back, G, s);
+    else grn_dispatch_v<float, float, 1>(p, back, G, s);
   }
 }
 
@@ -552,10 +593,13 @@ bool want_y(const mdg_gate_res_norm_desc& d) { return d.dgate || d.dpost_w || d.
 bool want_x(const mdg_gate_res_norm_desc& d) { return d.dshift || d.dscale || d.dpre_w || d.dpre_b; }
 int groups(const mdg_gate_res_norm_desc& d) { return (int)(((long long)d.M + d.rows_per_mod - 1) / d.rows_per_mod); }
 
-// Chunks of a group's rows: about 768 blocks in all (three per CU), each with 32 rows or more
+// Chunks of a group's rows: about 768 blocks in all (three per CU), each with four turns of its teams or more, or
+// eight rows of a whole block (a chunk's partial sums cost about as much as two rows).  [8 x 1000, 2048] 92 us against
+// 180 with 32 rows at least, [1 x 300, 2000] 38 / 79; four rows at least are no faster.
 int grn_chunks(const mdg_gate_res_norm_desc& d) {
   const int G = groups(d);
-  const int want = (768 + G - 1) / G, most = (d.rows_per_mod + 31) / 32;
+  const int least = d.C > 512 ? 8 : d.C > 384 ? 16 : 32;
+  const int want = (768 + G - 1) / G, most = (d.rows_per_mod + least - 1) / least;
   return want < most ? want : most;
 }
 
@@ -568,7 +612,8 @@ size_t gate_res_norm_ws_bytes(const mdg_gate_res_norm_desc& d) {
 
 // every launch within the 2^32 threads of a grid, row numbers (the last blocks', past the end) within 31 bits
 bool gate_res_norm_grid_ok(const mdg_gate_res_norm_desc& d, bool back) {
-  const long long threads = (1LL << 32) - 4096, tpr = grn_shape(d.C, back && grn_vec(d) > 4 ? 4 : grn_vec(d)).tpr;
+  const long long threads = (1LL << 32) - 4096, v = grn_vec(d);
+  const long long tpr = (back ? grn_back_shape(d.C, v < 4 ? 1 : 4) : grn_shape(d.C, (int)v)).tpr;
   if (d.M > (1LL << 31) - 4096) return false;
   if (!back) return d.M * tpr <= threads;
   const long long G = groups(d);
