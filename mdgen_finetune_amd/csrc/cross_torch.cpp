@@ -95,12 +95,15 @@ Tensor bytes(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-// (forward-mode tangents have no rule here and must not be dropped)
-bool any_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+// forward-mode tangents have no rule here and must not be dropped (no_grad leaves forward mode on)
+void refuse_tangents(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->_fw_grad(0).defined())
       throw std::runtime_error("mdgen_finetune_amd.cross_hip: no forward-mode derivative, detach the tangent first");
+}
+
+bool any_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
@@ -227,6 +230,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if (k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D || Hk == 0 || H % Hk || D < 1 || D > 128 ||
       B > INT32_MAX || q.size(1) > INT32_MAX || Nk > INT32_MAX || H > INT32_MAX)
     value_error(Text() << "cross_attention: q " << q.sizes() << ", k " << k.sizes() << ", v " << v.sizes());
+  refuse_tangents({&q, &k, &v});
   check_device(q, {&k, &v, &mask, &q_len, &kv_len});
   if (mask.defined()) {
     const auto t = mask.scalar_type();
@@ -371,6 +375,7 @@ py::object rope_axes(const RopePlan& plan, Tensor pos, const Tensor& q, const Ma
   }
   const int64_t B = q.size(0), N = q.size(1), D = q.size(3), axes = (int64_t)plan.sections.size();
   if (2 * plan.npairs > D || D > 1024 || B > INT32_MAX || N > INT32_MAX) value_error(Text() << "rope_axes: " << plan.npairs << " pairs in q " << q.sizes());
+  refuse_tangents({&x.front(), &x.back()});
   check_device(q, {&x.back(), &pos, &plan.turns});
   if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
     type_error(Text() << "rope_axes: pos must be int32 or int64, got " << pos.scalar_type());
@@ -552,6 +557,7 @@ py::tuple gate_residual_norm(const Tensor& h, const MaybeTensor& y_, const Maybe
   if (!cfg.pre)
     for (int i = 0; i < kIns; ++i)
       if (pre_side(i) && ins[i].defined()) value_error(Text() << "gate_residual_norm: pre weights or modulation without a pre norm");
+  refuse_tangents({&ins[0], &ins[1], &ins[2], &ins[3], &ins[4], &ins[5], &ins[6], &ins[7], &ins[8]});
   check_device(h, {&ins[1], &ins[2], &ins[3], &ins[4], &ins[5], &ins[6], &ins[7], &ins[8]});
   const int64_t M = h.numel() / C;
   int64_t G = 0;

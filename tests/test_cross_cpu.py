@@ -207,3 +207,22 @@ def test_rope_plan_tables():
     assert torch.allclose(p.turns, want, rtol=1e-15)
     assert X.RopeAxes([2, 1], pairs="half", device="cpu").cols.tolist() == [0, 1, 2, 3, 4, 5]
     assert X.RopeAxes([2, 1], pairs="interleaved", device="cpu").cols.tolist() == [0, 2, 4, 1, 3, 5]
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["grad", "no_grad"])
+def test_forward_mode_tangents_are_refused_whatever_the_grad_mode(grad):
+    """no_grad does not switch forward mode off (x * 2 keeps its tangent there): no call may drop one."""
+    import torch.autograd.forward_ad as fwd
+
+    plan = X.RopeAxes([4], device="cpu")
+    pos = _z(3, 1, dtype=torch.int32)
+    x, h = torch.randn(1, 3, 2, 8), torch.randn(4, 8)
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        dx, dh, dm = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, h, torch.ones(1, 8)))
+        assert fwd.unpack_dual(dx * 2).tangent is not None
+        for call in (lambda: X.cross_attention(dx, x, x), lambda: X.cross_attention(x, dx, x), lambda: X.cross_attention(x, x, dx),
+                     lambda: X.rope_axes(plan, pos, dx), lambda: X.rope_axes(plan, pos, x, dx),
+                     lambda: X.rope_axes(plan, pos, dx, inplace=True), lambda: X.gate_residual_norm(dh),
+                     lambda: X.gate_residual_norm(h, dh), lambda: X.gate_residual_norm(h, h, gate=dm)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
