@@ -719,7 +719,8 @@ int mdg_rope_axes(const mdg_rope_axes_desc* d, void* stream);
    xn = (pre(h_out) pre_w + pre_b) (1 + scale) + shift.  post / pre: MDG_NORM_NONE, _RMS, _LAYER (eps as
    given).  h [M][ldh], h_out res_dtype; y [M][ldy], xn dtype (y null: h_out = resid_scale h, only the
    norm before a block); res_dtype fp32, or equal to dtype.  gate / shift / scale fp32 rows
-   m / rows_per_mod of stride mod_stride (null: 1, 0, 0); weights fp32 [C] or null.  1 <= C <= 8192.
+   m / rows_per_mod of stride mod_stride (null: 1, 0, 0; rows_per_mod >= M is one group); weights fp32 [C]
+   or null.  1 <= C <= 8192.
    h_out may be h (ldh == C) or null when pre forms xn; outputs are contiguous rows of C.
    Backward: dh_out / dxn (either may be null: zero) -> dh, dy, the modulation gradients (rows of
    stride dmod_stride) and the weights' [C]; each may be null.  It reads h and y, not h_out. */

@@ -31,7 +31,7 @@ struct GrnP {
   long long mod_stride;
   const float *w1, *b1, *w2, *b2;
   float rs, eps, invC;
-  int M, C, R, post, pre;  // R = rows_per_mod
+  int M, C, R, post, pre;  // R = rows_per_mod, at most M
   long long ldh, ldy;      // row strides of h and y (outputs are contiguous)
   // backward
   const void *dho, *dxn;
@@ -262,8 +262,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void grn_bwd_kernel(const Gr
   __shared__ __attribute__((aligned(16))) float cols[TEAMS > 1 ? TPR * NV * V : 1];
   const int team = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int grp = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
-  const int g0 = grp * p.R, g1 = min(p.M, g0 + p.R);
-  const int r0 = g0 + chunk * p.rows_per_chunk, r1 = min(g1, r0 + p.rows_per_chunk);
+  // (ends from what is left: a group's first row plus its rows may pass 31 bits)
+  const int g0 = grp * p.R, g1 = g0 + min(p.R, p.M - g0);
+  const int r0 = g0 + min(g1 - g0, chunk * p.rows_per_chunk), r1 = r0 + min(g1 - r0, p.rows_per_chunk);
   const long long mo = (long long)grp * p.mod_stride;
   float S[4][NV][V];
 #pragma unroll
@@ -450,16 +451,19 @@ __global__ __launch_bounds__(1024) void grn_weights_kernel(const GrnP p, const f
   if (out) out[c] = v;
 }
 
+// rows of a modulation group; a longer run than there are rows is one group of them all
+int group_rows(const mdg_gate_res_norm_desc& d) { return d.rows_per_mod < d.M ? d.rows_per_mod : d.M; }
+
 GrnP grn_params(const mdg_gate_res_norm_desc& d) {
   GrnP p;
   p.h = d.h, p.y = d.y, p.ho = d.h_out, p.xn = d.xn;
   p.gate = d.gate, p.shift = d.shift, p.scale = d.scale, p.mod_stride = d.mod_stride;
   p.w1 = d.post_w, p.b1 = d.post_b, p.w2 = d.pre_w, p.b2 = d.pre_b;
   p.rs = d.resid_scale, p.eps = d.eps, p.invC = 1.0f / d.C;
-  p.M = d.M, p.C = d.C, p.R = d.rows_per_mod, p.post = d.post, p.pre = d.pre;
+  p.M = d.M, p.C = d.C, p.R = group_rows(d), p.post = d.post, p.pre = d.pre;
   p.ldh = d.ldh, p.ldy = d.ldy;
   p.dho = d.dh_out, p.dxn = d.dxn, p.dh = d.dh, p.dy = d.dy;
-  p.part = nullptr, p.chunks = 1, p.rows_per_chunk = d.rows_per_mod;
+  p.part = nullptr, p.chunks = 1, p.rows_per_chunk = p.R;
   p.want_y_sums = p.want_x_sums = 0;
   return p;
 }
@@ -591,7 +595,7 @@ void grn_dispatch(const mdg_gate_res_norm_desc& d, const GrnP& p, bool back, int
 
 bool want_y(const mdg_gate_res_norm_desc& d) { return d.dgate || d.dpost_w || d.dpost_b; }
 bool want_x(const mdg_gate_res_norm_desc& d) { return d.dshift || d.dscale || d.dpre_w || d.dpre_b; }
-int groups(const mdg_gate_res_norm_desc& d) { return (int)(((long long)d.M + d.rows_per_mod - 1) / d.rows_per_mod); }
+int groups(const mdg_gate_res_norm_desc& d) { return (int)(((long long)d.M + group_rows(d) - 1) / group_rows(d)); }
 
 // Chunks of a group's rows: about 768 blocks in all (three per CU), each with four turns of its teams or more, or
 // eight rows of a whole block (a chunk's partial sums cost about as much as two rows).  [8 x 1000, 2048] 92 us against
@@ -599,8 +603,8 @@ int groups(const mdg_gate_res_norm_desc& d) { return (int)(((long long)d.M + d.r
 int grn_chunks(const mdg_gate_res_norm_desc& d) {
   const int G = groups(d);
   const int least = d.C > 512 ? 8 : d.C > 384 ? 16 : 32;
-  const int want = (768 + G - 1) / G, most = (d.rows_per_mod + least - 1) / least;
-  return want < most ? want : most;
+  const long long want = (768LL + G - 1) / G, most = ((long long)group_rows(d) + least - 1) / least;
+  return (int)(want < most ? want : most);
 }
 
 }  // namespace
@@ -629,7 +633,7 @@ hipError_t gate_res_norm_bwd_launch(const mdg_gate_res_norm_desc& d, void* ws, h
   GrnP p = grn_params(d);
   const int G = groups(d);
   p.chunks = grn_chunks(d);
-  p.rows_per_chunk = (d.rows_per_mod + p.chunks - 1) / p.chunks;
+  p.rows_per_chunk = (p.R + p.chunks - 1) / p.chunks;
   p.want_y_sums = want_y(d), p.want_x_sums = want_x(d);
   const bool sums = p.want_y_sums || p.want_x_sums;
   float* S = nullptr;

@@ -226,3 +226,15 @@ def test_forward_mode_tangents_are_refused_whatever_the_grad_mode(grad):
                      lambda: X.gate_residual_norm(h, dh), lambda: X.gate_residual_norm(h, h, gate=dm)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("grads", [dict(dscale=0x1000), dict(dpost_w=0x1000), dict(dgate=0x1000, gate=0x1000, mod_stride=64)])
+@pytest.mark.parametrize("M", [1, 8, 1000, 100000])
+def test_grn_workspace_of_one_long_group(M, grads):
+    """rows_per_mod at or past M is one group of M rows, whatever its value."""
+    lib = _lib.load()
+    kw = dict(dxn=0x1000, dmod_stride=64, M=M, **grads)
+    want = lib.mdg_gate_res_norm_bwd_workspace_bytes(ctypes.byref(_grn(rows_per_mod=M, **kw)))
+    assert 0 < want <= 770 * 4 * 64 * 4  # (at most 768 chunks, and the sums)
+    for R in (M + 1, 1 << 30, (1 << 31) - 20, (1 << 31) - 1):
+        assert lib.mdg_gate_res_norm_bwd_workspace_bytes(ctypes.byref(_grn(rows_per_mod=R, **kw))) == want

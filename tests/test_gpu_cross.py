@@ -836,3 +836,33 @@ def test_backward_twice_with_retain_graph(which):
     w = torch.randn_like(out)
     one = torch.autograd.grad(out, leaves, w, retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(one, torch.autograd.grad(out, leaves, w)))
+
+
+@pytest.mark.parametrize("R", [1 << 30, (1 << 31) - 1])
+def test_norm_backward_of_one_long_group(R):
+    """rows_per_mod past the rows' count, at the C entry: one group, the results of rows_per_mod = M bit for bit."""
+    import ctypes
+
+    from mdgen_finetune_amd import _lib
+
+    lib, M, C, g = _lib.load(), 3000, 96, _gen(31)
+    h, y, dho, dxn = (torch.randn(M, C, generator=g).cuda() for _ in range(4))
+    gate, scale = (torch.randn(1, C, generator=g).cuda() for _ in range(2))
+    got = []
+    for rows in (M, R):
+        outs = {n: torch.full((M, C), 7.0, device="cuda") for n in ("h_out", "xn", "dh", "dy")}
+        outs.update({n: torch.full((C,), 7.0, device="cuda") for n in ("dgate", "dscale", "dpost_w", "dpre_w")})
+        d = _lib.MdgGateResNorm(dtype=0, res_dtype=0, M=M, C=C, rows_per_mod=rows, post=1, pre=2, resid_scale=0.9, eps=1e-6,
+                                h=h.data_ptr(), y=y.data_ptr(), ldh=C, ldy=C, gate=gate.data_ptr(), scale=scale.data_ptr(),
+                                mod_stride=C, dmod_stride=C, dh_out=dho.data_ptr(), dxn=dxn.data_ptr(),
+                                **{n: t.data_ptr() for n, t in outs.items()})
+        stream = torch.cuda.current_stream().cuda_stream
+        need = lib.mdg_gate_res_norm_bwd_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        assert lib.mdg_gate_res_norm(ctypes.byref(d), stream) == 0, lib.mdg_last_error_string()
+        assert lib.mdg_gate_res_norm_bwd(ctypes.byref(d), ws.data_ptr(), need, stream) == 0, lib.mdg_last_error_string()
+        got.append((need, outs))
+    assert got[0][0] == got[1][0]
+    for n, t in got[0][1].items():
+        assert torch.equal(t, got[1][1][n]), n
+        assert not (t == 7.0).all(), n
