@@ -297,6 +297,7 @@ struct KvStage {
   unsigned ko[ASYNC ? P : 1], vo[ASYNC ? P : 1];  // byte offsets of this thread's pieces in a tile
   bool keep[P];  // ASYNC: of the tile to begin next; else of the begun one
   float kb;
+  bool seen = false;           // (uniform in its wave) a key was there in the tiles finished so far
   const CT *kp, *vp;           // the tile's first row
   uint64_t ka, va;             // ASYNC: its address, and the strides from tile to tile, in bytes
   int64_t kstep, vstep;
@@ -381,12 +382,15 @@ struct KvStage {
     if (tid < 64) {
       if (tid < ROWS) kbs[tid] = kb;
       const bool any = __any(kb != 0.f);
+      seen = seen || !any || __any(tid < ROWS && kb == 0.f);
       if (tid == 0) *flag = any;
     }
   }
-  __device__ __forceinline__ void finish(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int tid) {
+  // keys: set where a key was there in the tiles so far (the block's threads read it after the last tile)
+  __device__ __forceinline__ void finish(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int* keys, int tid) {
     finish_rows(p, Ks, Vs, tid);
     finish_kb(kbs, flag, tid);
+    if (tid == 0) *keys = seen;
     if constexpr (ASYNC) async_wait();
   }
 };
@@ -482,9 +486,10 @@ __device__ __forceinline__ long long part_row(const CrossP& p, int sp, int b, in
   return ((long long)sp * p.B * p.Hk + (long long)b * p.Hk + hk) * rows + r;
 }
 
-// a lane's row of outputs, O^T rows 32 dt + 8a + 4h + i: normalised, or a split's partial
+// a lane's row of outputs, O^T rows 32 dt + 8a + 4h + i: normalised, or a split's partial.  keys: whether any key was
+// there; without one the sums are 0 whatever the query holds (-inf + 0 q is NaN for an infinite q).
 template <typename CT, int DP, bool VEC>
-__device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, int r, int rows, bool live,
+__device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, int r, int rows, bool live, bool keys,
                                            const f32x16* o, float m, float l, int lane) {
   constexpr int DT = DP / 32;
   const int h = lane >> 5;
@@ -492,20 +497,20 @@ __device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, i
   if (p.nsplit > 1) {
     const long long pr = part_row(p, id.split, id.b, id.hk, r);
     if (h == 0) {
-      p.part_ml[2 * pr] = m;
-      p.part_ml[2 * pr + 1] = l;
+      p.part_ml[2 * pr] = keys ? m : kNoMax;
+      p.part_ml[2 * pr + 1] = keys ? l : 0.f;
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int a = 0; a < 4; ++a)
         *reinterpret_cast<float4*>(p.part + pr * DP + 32 * dt + 8 * a + 4 * h) =
-            make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
+            keys ? make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]) : make_float4(0, 0, 0, 0);
     return;
   }
   const PackedRow pk = packed(p, r);
   const int n = pk.n, head = id.hk * p.G + pk.g;
-  const bool some = live && l != 0.f;  // (a NaN among the keys that are there stays one)
+  const bool some = live && keys && l != 0.f;  // (a NaN among the keys that are there stays one)
   const float inv = some ? 1.0f / l : 0.f;
   if (p.lse && h == 0) p.lse[((long long)id.b * p.H + head) * p.Nq + n] = some ? m * p.c + log2f(l) : -INFINITY;
   CT* orow = wrow<CT>(p.o, id.b, n, head);
@@ -570,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
   if (nt > 0) {
     st.init(p, id.b, id.hk, k0, k1, KT, tid);
     st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
-    st.finish(p, Ks, Vs, kbs, flag, tid);
+    st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
   }
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
@@ -593,11 +598,11 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
             o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
         }
     }
-    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), flag + 2, tid);
     __syncthreads();
   }
 
-  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, other_half_sum(l), lane);
+  store_rows<CT, DP, VEC>(p, id, r, rows, live, nt > 0 && flag[2], o, m, other_half_sum(l), lane);
 }
 
 // The same with two groups of four waves (256 rows per block), one phase apart, each SIMD holding one wave
@@ -646,7 +651,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
   if (nt > 0 && !second) {
     st.init(p, id.b, id.hk, k0, k1, KT, tid);
     st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
-    st.finish(p, Ks, Vs, kbs, flag, tid);
+    st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
   }
   __syncthreads();
   if (second) __syncthreads();
@@ -672,12 +677,12 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) pf[kt][0] = half_frag<CT>(s[kt], 0), pf[kt][1] = half_frag<CT>(s[kt], 1);
     }
-    if (loads) st.finish(p, Ks, Vs, kbs + ((t + 1) & 1) * KT, flag + ((t + 1) & 1), tid);
+    if (loads) st.finish(p, Ks, Vs, kbs + ((t + 1) & 1) * KT, flag + ((t + 1) & 1), flag + 2, tid);
     vnext = vnext == 2 ? 0 : vnext + 1;
     __syncthreads();
   }
   if (!second) __syncthreads();
-  store_rows<CT, DP, true>(p, id, r, rows, live, o, m, other_half_sum(l), lane);
+  store_rows<CT, DP, true>(p, id, r, rows, live, nt > 0 && flag[2], o, m, other_half_sum(l), lane);
 }
 
 // At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
@@ -756,6 +761,11 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     if constexpr (BUFS == 2) cur ^= 1;
   }
   l = other_half_sum(l);
+  if (!st.seen) {  // no key was there for this wave: nothing, whatever the queries hold
+    m = kNoMax, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = zero16();
+  }
 
   // join: [4][32] maxima and sums, then the rescaled outputs [4][32][DP + 4] over the staging area
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -966,7 +976,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  if (nt > 0) st.finish(p, Ks, Vs, kbs, flag, tid);
+  if (nt > 0) st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const int cur = t & 1;
@@ -994,10 +1004,14 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
           acc[dt] = mma<CT>(col_frag<CT, DP>(Kc, 32 * kt + 16 * s2, 32 * dt, lane), df, acc[dt]);
       }
     }
-    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), flag + 2, tid);
     __syncthreads();
   }
   if (r >= rows) return;
+  if (!(nt > 0 && flag[2])) {  // no key was there: 0, whatever the query and its gradient hold
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = zero16();
+  }
   if (p.nsplit > 1) {
     const long long pr = part_row(p, id.split, id.b, id.hk, r);
 #pragma unroll
@@ -1335,6 +1349,10 @@ __global__ __launch_bounds__(256) void cross_few_bwd_kernel(const CrossP p) {
         }
       }
 
+  if (!st.seen) {  // no key was there for this wave
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = zero16();
+  }
   // dq of the waves, [W][32][DP + 4] over the tiles, summed in order
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last tile's reads are done

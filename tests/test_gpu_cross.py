@@ -866,3 +866,41 @@ def test_norm_backward_of_one_long_group(R):
     for n, t in got[0][1].items():
         assert torch.equal(t, got[1][1][n]), n
         assert not (t == 7.0).all(), n
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,D", [
+    (2, 1, 40, 4, 2, 24),       # single tokens: one wave's tile
+    (2, 3, 3000, 4, 1, 64),     # their splits
+    (2, 1, 900, 2, 2, 128),
+    (2, 70, 50, 2, 2, 40),      # 128-row blocks
+    (2, 40, 1500, 2, 1, 24),    # their splits
+    (40, 260, 130, 16, 16, 72),  # 256-row blocks of wide bf16 heads
+    (2, 260, 1500, 1, 1, 128),  # their splits
+])
+def test_no_keys_and_a_query_that_is_not_finite(B, Nq, Nk, H, Hk, D, dt):
+    """A mask that leaves nothing and kv_len 0 say the same: o = 0 and dq = 0 whatever q and dout hold, and the other
+    sequences are as they are beside finite ones."""
+    g = _gen(41)
+    q, k, v, do = (torch.randn(B, n, h, D, generator=g).to(dt).cuda() for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
+    mask = torch.rand(B, Nk, generator=g).cuda() < 0.7
+    mask[-1] = False
+    bad = torch.tensor([float("nan"), float("inf"), float("-inf")], device="cuda").to(dt)
+    ln = torch.full((B,), Nk, dtype=torch.int32, device="cuda")
+    ln[-1] = 0
+    res = []
+    for fill, kw in ((None, dict(mask=mask)), (bad, dict(mask=mask)), (bad, dict(kv_len=ln, mask=mask | (ln == 0)[:, None]))):
+        ql, gl = q.clone(), do.clone()
+        if fill is not None:
+            ql[-1] = fill[torch.arange(D, device="cuda") % 3]
+            gl[-1] = fill[0]
+        leaves = [t.clone().requires_grad_(True) for t in (ql, k, v)]
+        o = X().cross_attention(*leaves, **kw)
+        with torch.no_grad():
+            assert torch.equal(X().cross_attention(*leaves, **kw), o)
+        res.append((o.detach(), *torch.autograd.grad(o, leaves, gl)))
+        for n, t in zip(("o", "dq", "dk", "dv"), res[-1]):
+            assert (t[-1] == 0).all(), n
+            assert torch.isfinite(t).all() and (t[0] != 0).any(), n
+    for n, a, b, c in zip(("o", "dq", "dk", "dv"), *res):
+        assert torch.equal(a, b) and torch.equal(a, c), n
