@@ -1008,7 +1008,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
     __syncthreads();
   }
   if (r >= rows) return;
-  if (!(nt > 0 && flag[2])) {  // no key was there: 0, whatever the query and its gradient hold
+  if (!(live && nt > 0 && flag[2])) {  // past q_len, or no key was there: 0, whatever keys, query and its gradient hold
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = zero16();
   }
@@ -1373,10 +1373,11 @@ __global__ __launch_bounds__(256) void cross_few_bwd_kernel(const CrossP p) {
       const float4 t = *reinterpret_cast<const float4*>(jo + (32 * w + row) * LO + d0);
       v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
     }
+    const PackedRow q = packed(p, row);
+    if (q.n >= qlen) v = make_float4(0, 0, 0, 0);  // (whatever the keys hold)
     if (p.nsplit > 1) {
       *reinterpret_cast<float4*>(p.part + part_row(p, id.split, id.b, id.hk, row) * DP + d0) = v;
     } else {
-      const PackedRow q = packed(p, row);
       st_out<CT, VEC>(wrow<CT>(p.dq, id.b, q.n, id.hk * p.G + q.g), d0, p.D, v.x * p.scale, v.y * p.scale, v.z * p.scale,
                       v.w * p.scale);
     }

@@ -904,3 +904,20 @@ def test_no_keys_and_a_query_that_is_not_finite(B, Nq, Nk, H, Hk, D, dt):
             assert torch.isfinite(t).all() and (t[0] != 0).any(), n
     for n, a, b, c in zip(("o", "dq", "dk", "dv"), *res):
         assert torch.equal(a, b) and torch.equal(a, c), n
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,D", [(2, 3, 40, 4, 2, 24), (2, 6, 3000, 4, 1, 64), (2, 200, 50, 2, 2, 128), (2, 90, 1500, 1, 1, 48)])
+def test_rows_past_q_len_beside_a_key_that_is_not_finite(B, Nq, Nk, H, Hk, D, dt):
+    """A key that is there and holds infinities makes its sequence's rows NaN, not those past q_len: o and dq are 0 there."""
+    g = _gen(43)
+    q, k, v, do = (torch.randn(B, n, h, D, generator=g).to(dt).cuda() for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
+    k[0, Nk // 2], v[0, Nk // 2] = float("inf"), float("nan")
+    ln = torch.tensor([Nq // 2, Nq - 1], dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = X().cross_attention(*leaves, q_len=ln)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    for t in (o, dq):
+        assert (t[0, Nq // 2:] == 0).all() and (t[1, Nq - 1:] == 0).all()
+        assert not torch.isfinite(t[0, :Nq // 2]).any() and torch.isfinite(t[1]).all() and (t[1, : Nq - 1] != 0).any()
+    assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
