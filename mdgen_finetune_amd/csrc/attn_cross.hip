@@ -451,11 +451,11 @@ __device__ __forceinline__ typename V8<CT>::T half_frag(const f32x16& s, int s2)
   return r;
 }
 
-// keys [k0, k1) of split `sp`: the sequence's own length shared out in multiples of 32
+// keys [k0, k1) of split `sp`: the sequence's own length shared out in multiples of 32 (k0 + per may pass 31 bits)
 __device__ __forceinline__ void split_range(const CrossP& p, int klen, int sp, int& k0, int& k1) {
   const int per = (quot(klen + p.nsplit - 1, p.by_split) + 31) / 32 * 32;
   k0 = min(klen, sp * per);
-  k1 = min(klen, k0 + per);
+  k1 = k0 + min(klen - k0, per);
 }
 
 struct BlockId {

@@ -921,3 +921,19 @@ def test_rows_past_q_len_beside_a_key_that_is_not_finite(B, Nq, Nk, H, Hk, D, dt
         assert (t[0, Nq // 2:] == 0).all() and (t[1, Nq - 1:] == 0).all()
         assert not torch.isfinite(t[0, :Nq // 2]).any() and torch.isfinite(t[1]).all() and (t[1, : Nq - 1] != 0).any()
     assert torch.isfinite(dk[1]).all() and torch.isfinite(dv[1]).all()
+
+
+@pytest.mark.parametrize("Nq", [1, 40])
+def test_cross_attention_on_the_longest_key_axis(Nq):
+    """2^31 - 8192 keys, the most that is not refused: equal scores, v = 1 at the last 2^21 keys.  Every count is a
+    whole number of 8192s below 2^31, exact in fp32, and the probabilities are powers of two: o is its own rounding
+    (2^-8) and those of a reciprocal and a product in fp32."""
+    Nk, last = (1 << 31) - 8192, 1 << 21
+    q = torch.ones(1, Nq, 1, 1, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(1, 1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(1, Nk, 1, 1)
+    v = torch.zeros(1, Nk, 1, 1, dtype=torch.bfloat16, device="cuda")
+    v[:, Nk - last:] = 1
+    with torch.no_grad():
+        o = X().cross_attention(q, k, v)
+    want = torch.full((1, Nq, 1, 1), last / Nk, dtype=torch.float64)
+    _near(o, want, (U16 + 4 * U32) * want, "o")
