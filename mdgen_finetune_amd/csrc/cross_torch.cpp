@@ -236,7 +236,8 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const auto t = mask.scalar_type();
     if ((t != at::kBool && t != at::kByte && t != at::kFloat) || mask.dim() != 2 || mask.size(1) != Nk || (mask.size(0) != 1 && mask.size(0) != B))
       value_error(Text() << "cross_attention: mask must be bool, uint8 or fp32 [" << B << " or 1, " << Nk << "], got " << mask);
-    if (mask.size(0) != B) mask = mask.expand({B, Nk});
+    if (!Nk) mask = Tensor();  // (an encoder without states has nothing to mask, and an empty mask no address)
+    else if (mask.size(0) != B) mask = mask.expand({B, Nk});
   }
   check_len("q_len", q_len, B), check_len("kv_len", kv_len, B);
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)D);

@@ -937,3 +937,17 @@ def test_cross_attention_on_the_longest_key_axis(Nq):
         o = X().cross_attention(q, k, v)
     want = torch.full((1, Nq, 1, 1), last / Nk, dtype=torch.float64)
     _near(o, want, (U16 + 4 * U32) * want, "o")
+
+
+@pytest.mark.parametrize("mdt", [torch.bool, torch.uint8, torch.float32], ids=str)
+@pytest.mark.parametrize("mB", [1, 3])
+def test_an_empty_mask_of_an_encoder_without_states(mB, mdt):
+    q = torch.randn(3, 5, 2, 24, device="cuda", requires_grad=True)
+    k, v = (torch.randn(3, 0, 1, 24, device="cuda", requires_grad=True) for _ in range(2))
+    mask, ln = torch.zeros(mB, 0, dtype=mdt, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    for kw in (dict(mask=mask), dict(mask=mask, kv_len=ln)):
+        o = X().cross_attention(q, k, v, **kw)
+        dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.ones_like(o))
+        assert (o == 0).all() and (dq == 0).all() and dk.shape == dv.shape == k.shape
+    with pytest.raises(ValueError):
+        X().cross_attention(q, k, v, mask=torch.zeros(2, 0, dtype=mdt, device="cuda"))
