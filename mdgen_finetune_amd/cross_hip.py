@@ -15,7 +15,8 @@ Tensors are fp32 or bf16 on a ROCm device, any strides with a contiguous last di
 copied).  Calls run on the current stream of the tensors' device, allocate only outputs and
 workspaces through torch's caching allocator (so they may be captured into a HIP graph; a backward pass
 only while no eager graph of the same leaves is alive, whose accumulation torch ties to its own stream), and
-are differentiable, once, where an input requires grad.  Wrong types and shapes raise TypeError / ValueError
+are differentiable, once, where an input requires grad; forward-mode tangents and tracing (torch.jit.trace,
+make_fx, fake tensors) raise RuntimeError.  Wrong types and shapes raise TypeError / ValueError
 before any launch; a missing library or a CPU tensor raises RuntimeError (there is no other path).
 """
 from __future__ import annotations

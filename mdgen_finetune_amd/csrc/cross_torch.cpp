@@ -9,10 +9,12 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -100,6 +102,15 @@ void refuse_tangents(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->_fw_grad(0).defined())
       throw std::runtime_error("mdgen_finetune_amd.cross_hip: no forward-mode derivative, detach the tangent first");
+}
+
+// A recording of torch operations holds the allocation of an output and not the call that fills it: what is traced
+// (torch.jit.trace, make_fx) would return memory as it was found.  Fake tensors have no memory at all.
+void refuse_tracing() {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(Mode::PROXY).has_value() ||
+      c10::impl::TorchDispatchModeTLS::get_mode(Mode::FAKE).has_value())
+    throw std::runtime_error("mdgen_finetune_amd.cross_hip: its calls cannot be traced or run on fake tensors");
 }
 
 bool any_grad(std::initializer_list<const Tensor*> ts) {
@@ -230,6 +241,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if (k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D || Hk == 0 || H % Hk || D < 1 || D > 128 ||
       B > INT32_MAX || q.size(1) > INT32_MAX || Nk > INT32_MAX || H > INT32_MAX)
     value_error(Text() << "cross_attention: q " << q.sizes() << ", k " << k.sizes() << ", v " << v.sizes());
+  refuse_tracing();
   refuse_tangents({&q, &k, &v});
   check_device(q, {&k, &v, &mask, &q_len, &kv_len});
   if (mask.defined()) {
@@ -376,6 +388,7 @@ py::object rope_axes(const RopePlan& plan, Tensor pos, const Tensor& q, const Ma
   }
   const int64_t B = q.size(0), N = q.size(1), D = q.size(3), axes = (int64_t)plan.sections.size();
   if (2 * plan.npairs > D || D > 1024 || B > INT32_MAX || N > INT32_MAX) value_error(Text() << "rope_axes: " << plan.npairs << " pairs in q " << q.sizes());
+  refuse_tracing();
   refuse_tangents({&x.front(), &x.back()});
   check_device(q, {&x.back(), &pos, &plan.turns});
   if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
@@ -558,6 +571,7 @@ py::tuple gate_residual_norm(const Tensor& h, const MaybeTensor& y_, const Maybe
   if (!cfg.pre)
     for (int i = 0; i < kIns; ++i)
       if (pre_side(i) && ins[i].defined()) value_error(Text() << "gate_residual_norm: pre weights or modulation without a pre norm");
+  refuse_tracing();
   refuse_tangents({&ins[0], &ins[1], &ins[2], &ins[3], &ins[4], &ins[5], &ins[6], &ins[7], &ins[8]});
   check_device(h, {&ins[1], &ins[2], &ins[3], &ins[4], &ins[5], &ins[6], &ins[7], &ins[8]});
   const int64_t M = h.numel() / C;

@@ -238,3 +238,19 @@ def test_grn_workspace_of_one_long_group(M, grads):
     assert 0 < want <= 770 * 4 * 64 * 4  # (at most 768 chunks, and the sums)
     for R in (M + 1, 1 << 30, (1 << 31) - 20, (1 << 31) - 1):
         assert lib.mdg_gate_res_norm_bwd_workspace_bytes(ctypes.byref(_grn(rows_per_mod=R, **kw))) == want
+
+
+def test_tracing_is_refused():
+    """A trace would hold an output's allocation without the call that fills it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    plan, pos = X.RopeAxes([4], device="cpu"), _z(3, 1, dtype=torch.int32)
+    for f, x in ((lambda t: X.cross_attention(t, t, t), _z(1, 3, 2, 8)), (lambda t: X.rope_axes(plan, pos, t), _z(1, 3, 2, 8)),
+                 (lambda t: X.gate_residual_norm(t)[1], _z(4, 8))):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(x)
+        with FakeTensorMode(), pytest.raises(RuntimeError, match="traced"):
+            f(torch.empty(x.shape))
