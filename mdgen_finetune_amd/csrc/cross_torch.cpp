@@ -184,21 +184,18 @@ void cross_forward(const CrossArgs& c, const Tensor& o, const Tensor& side, int6
 }
 
 struct CrossNode : OnceNode {
-  SavedVariable q, k, v, o, mask, q_len, kv_len;
-  Tensor side;
+  SavedVariable q, k, v, o, side, mask, q_len, kv_len;  // (all of them, so that saved-tensor hooks see what is kept)
   int64_t low = -1;
   double scale = 1.0;
   std::string name() const override { return "CrossAttentionBackward"; }
   void release_variables() override {
-    for (SavedVariable* s : {&q, &k, &v, &o, &mask, &q_len, &kv_len}) s->reset_data();
-    side.reset();
+    for (SavedVariable* s : {&q, &k, &v, &o, &side, &mask, &q_len, &kv_len}) s->reset_data();
   }
   variable_list backward(const variable_list& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
     const CrossArgs c{unit(q.unpack()), unit(k.unpack()), unit(v.unpack()), mask.unpack(), q_len.unpack(), kv_len.unpack(), scale};
-    const Tensor ou = unit(o.unpack(shared_from_this()));
-    TORCH_CHECK(side.defined(), "Trying to backward through the graph a second time");
+    const Tensor ou = unit(o.unpack(shared_from_this())), kept = side.unpack();
     const c10::DeviceGuard guard(c.q.device());
     const bool keys = should_compute_output(1) || should_compute_output(2);  // (a frozen encoder: dq alone)
     const Tensor dq = at::empty(c.q.sizes(), c.q.options());
@@ -206,7 +203,7 @@ struct CrossNode : OnceNode {
     if (keys) dk = at::empty(c.k.sizes(), c.k.options()), dv = at::empty(c.v.sizes(), c.v.options());
     if (c.q.numel()) {
       const Tensor g = unit(grads[0]);
-      mdg_attn_cross d = cross_desc(c, ou, side, low);
+      mdg_attn_cross d = cross_desc(c, ou, kept, low);
       d.dout = heads(g), d.dq = heads(dq);
       if (keys) d.dk = heads(dk), d.dv = heads(dv);
       const size_t n = lib.cross_ws(&d, 1);
@@ -272,10 +269,10 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   // what the backward reads beside o, one allocation
   const bool bf16 = q.scalar_type() == at::kBFloat16;
   const int64_t n = q.numel(), rows = (n / D + 3) / 4 * 16;
-  node->side = at::empty({rows + (bf16 ? 2 * n : 0) + 16}, q.options().dtype(at::kByte));
+  const Tensor side = at::empty({rows + (bf16 ? 2 * n : 0) + 16}, q.options().dtype(at::kByte));
   node->low = bf16 ? rows : -1, node->scale = scale;
-  cross_forward(c, o, node->side, node->low);
-  node->q = save(c.q), node->k = save(c.k), node->v = save(c.v);
+  cross_forward(c, o, side, node->low);
+  node->side = save(side), node->q = save(c.q), node->k = save(c.k), node->v = save(c.v);
   node->mask = save(mask), node->q_len = save(q_len), node->kv_len = save(kv_len);
   ag::set_history(o, node);
   node->o = SavedVariable(o, true);

@@ -951,3 +951,22 @@ def test_an_empty_mask_of_an_encoder_without_states(mB, mdt):
         assert (o == 0).all() and (dq == 0).all() and dk.shape == dv.shape == k.shape
     with pytest.raises(ValueError):
         X().cross_attention(q, k, v, mask=torch.zeros(2, 0, dtype=mdt, device="cuda"))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_all_that_attention_keeps_passes_the_saved_tensor_hooks(dt):
+    """Moved to the host by the hooks, nothing of the forward stays allocated but its output, and the gradients are the same."""
+    B, Nq, Nk, H, D = 2, 4096, 64, 8, 64
+    g = _gen(47)
+    q, k, v = (torch.randn(B, n, H, D, generator=g).to(dt).cuda().requires_grad_(True) for n in (Nq, Nk, Nk))
+    do = torch.ones(B, Nq, H, D, dtype=dt, device="cuda")
+    want = torch.autograd.grad(X().cross_attention(q, k, v), (q, k, v), do)
+    at = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        o = X().cross_attention(q, k, v)
+    kept = torch.cuda.memory_allocated() - at
+    assert kept < o.numel() * o.element_size() + (1 << 18), kept  # (lse alone is B H Nq 4 bytes, o's residual as large as o)
+    got = torch.autograd.grad(o, (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o, (q, k, v), do)
