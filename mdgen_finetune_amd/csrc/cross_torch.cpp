@@ -71,8 +71,11 @@ void check_rc(int rc, const char* what) {
 bool known(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
 int code(at::ScalarType t) { return t == at::kBFloat16 ? MDG_BF16 : MDG_F32; }
 
+// values as they lie in memory (a view such as z.conj().imag holds them negated)
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // the tensor with its last dim contiguous (a copy only where it is not)
-Tensor unit(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor unit(const Tensor& t) { return plain(t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous()); }
 
 mdg_heads heads(const Tensor& t) { return mdg_heads{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
@@ -450,6 +453,8 @@ Tensor rows2d(const Tensor& t, int64_t C, int64_t& ld) {
 // the inputs' part of the descriptor; ins is left holding the tensors that it points into
 mdg_gate_res_norm_desc grn_desc(const GrnCfg& c, std::array<Tensor, kIns>& ins) {
   mdg_gate_res_norm_desc d = {};
+  for (Tensor& t : ins)
+    if (t.defined() && t.is_neg()) t = t.resolve_neg();
   const int64_t C = ins[kH].size(-1);
   d.res_dtype = code(ins[kH].scalar_type()), d.dtype = code(c.xt);
   d.M = (int)(ins[kH].numel() / C), d.C = (int)C, d.rows_per_mod = (int)c.R, d.post = c.post, d.pre = c.pre;
@@ -498,7 +503,7 @@ struct GrnNode : OnceNode {
     const Tensor like = ins[kH];
     const bool rows = like.numel() > 0;
     mdg_gate_res_norm_desc d = grn_desc(cfg, ins);
-    const Tensor dho = gh.defined() ? gh.contiguous() : gh, dxn = gx.defined() ? gx.contiguous() : gx;
+    const Tensor dho = plain(gh.defined() ? gh.contiguous() : gh), dxn = plain(gx.defined() ? gx.contiguous() : gx);
     const auto f32 = like.options().dtype(at::kFloat);
     if (should_compute_output(kH)) out[kH] = at::empty(shape, like.options());
     if (should_compute_output(kY)) out[kY] = at::empty(shape, ins[kY].options());

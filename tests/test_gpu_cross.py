@@ -970,3 +970,27 @@ def test_all_that_attention_keeps_passes_the_saved_tensor_hooks(dt):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError):
         torch.autograd.grad(o, (q, k, v), do)
+
+
+@pytest.mark.parametrize("which", range(3), ids=["attention", "rope", "norms"])
+def test_negated_views(which):
+    """Views that hold their values negated (as z.conj().imag does), as inputs and as gradients."""
+    f, ins = _small()[which]
+    neg = lambda t: torch._neg_view(-t)  # noqa: E731
+    leaves = [t.clone().requires_grad_(True) for t in ins]
+    out = f(*leaves)
+    up = torch.randn_like(out)
+    base = torch.autograd.grad(out, leaves, up)
+    twins = [neg(t).requires_grad_(True) for t in ins]
+    assert all(t.is_neg() and torch.equal(t, u) for t, u in zip(twins, ins))
+    got = f(*twins)
+    assert torch.equal(got, out)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, twins, neg(up)), base))
+
+
+def test_negated_views_rotated_in_place():
+    plan = X().RopeAxes([4, 4])
+    q, pos = torch.randn(2, 5, 3, 16, device="cuda"), torch.arange(10, device="cuda", dtype=torch.int32).reshape(5, 2)
+    want = X().rope_axes(plan, pos, q)
+    twin = torch._neg_view(-q)
+    assert torch.equal(X().rope_axes(plan, pos, twin, inplace=True), want) and torch.equal(twin, want)
