@@ -64,7 +64,7 @@ def cross_attention(q, k, v, mask=None, q_len=None, kv_len=None, scale=None):
 class RopeAxes:
     """The rotary plan of a head: sections[a] pairs of columns turn by a token's position on axis a, pair i
     of an axis with n pairs at frequency base ** (-i / n) (or freq: one frequency per pair, all sections in
-    order).  pairs: "half" couples column p with p + sum(sections), "interleaved" 2p with 2p + 1, "axis"
+    order, constants).  pairs: "half" couples column p with p + sum(sections), "interleaved" 2p with 2p + 1, "axis"
     halves within each axis's own section.  Columns past 2 * sum(sections) pass through."""
 
     def __init__(self, sections, base=10000.0, pairs="half", freq=None, device=None):
@@ -77,6 +77,8 @@ class RopeAxes:
         if freq is None:
             freq = [float(base) ** (-i / s) for s in sections for i in range(s)]
         freq = torch.as_tensor(freq, dtype=torch.float64).cpu()
+        if freq.requires_grad:
+            raise ValueError("RopeAxes: frequencies are constants of the plan and get no gradient, detach them first")
         if tuple(freq.shape) != (n,):
             raise ValueError(f"RopeAxes: {n} pairs but freq {tuple(freq.shape)}")
         first, second, at = [], [], 0

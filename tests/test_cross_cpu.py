@@ -254,3 +254,11 @@ def test_tracing_is_refused():
             make_fx(f)(x)
         with FakeTensorMode(), pytest.raises(RuntimeError, match="traced"):
             f(torch.empty(x.shape))
+
+
+def test_rope_plan_refuses_frequencies_that_require_grad():
+    freq = torch.ones(4, dtype=torch.float64, requires_grad=True)
+    for f in (freq, freq * 2, torch.nn.Parameter(torch.ones(4))):
+        with pytest.raises(ValueError, match="gradient"):
+            X.RopeAxes([2, 2], freq=f, device="cpu")
+    assert torch.equal(X.RopeAxes([2, 2], freq=freq.detach(), device="cpu").turns, freq.detach() / (2 * torch.pi))
