@@ -90,13 +90,19 @@ class RopeAxes:
             first, second = list(range(n)), list(range(n, 2 * n))
         elif pairs == "interleaved":
             first, second = list(range(0, 2 * n, 2)), list(range(1, 2 * n, 2))
-        self.sections, self.pairs, self.npairs = sections, pairs, n
+        self.sections, self.pairs, self.npairs = tuple(sections), pairs, n
         axis = [a for a, s in enumerate(sections) for _ in range(s)]
         # one copy to the device: the frequencies in turns (fp64), then three int32 tables
         tables = torch.cat([(freq / (2.0 * math.pi)).view(torch.int32), torch.tensor(axis + first + second, dtype=torch.int32)])
         tables = tables.to(torch.device("cuda" if device is None else device))
         self.turns, self.axis, self.cols = tables[: 2 * n].view(torch.float64), tables[2 * n : 3 * n], tables[3 * n :]
         self._plan = None
+
+    def __setattr__(self, name, value):
+        # (the extension's handle holds the tables, and the kernels trust their columns)
+        if name in self.__dict__ and name != "_plan":
+            raise AttributeError(f"RopeAxes: {name} of a plan is fixed, make another plan")
+        super().__setattr__(name, value)
 
     def __getstate__(self):
         return {**self.__dict__, "_plan": None}  # (the extension's handle is made anew where it is needed)

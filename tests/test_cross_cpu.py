@@ -262,3 +262,17 @@ def test_rope_plan_refuses_frequencies_that_require_grad():
         with pytest.raises(ValueError, match="gradient"):
             X.RopeAxes([2, 2], freq=f, device="cpu")
     assert torch.equal(X.RopeAxes([2, 2], freq=freq.detach(), device="cpu").turns, freq.detach() / (2 * torch.pi))
+
+
+def test_rope_plan_is_fixed():
+    """A call keeps the tables behind a handle: assigning others is refused, not ignored."""
+    import copy
+
+    plan = X.RopeAxes([2, 2], device="cpu")
+    for n in ("turns", "axis", "cols", "sections", "pairs", "npairs"):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(plan, n, getattr(plan, n))
+    with pytest.raises(TypeError):
+        plan.sections[0] = 3
+    twin = copy.deepcopy(plan)
+    assert torch.equal(twin.turns, plan.turns) and twin.sections == plan.sections == (2, 2)
