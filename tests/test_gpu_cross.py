@@ -994,3 +994,50 @@ def test_negated_views_rotated_in_place():
     want = X().rope_axes(plan, pos, q)
     twin = torch._neg_view(-q)
     assert torch.equal(X().rope_axes(plan, pos, twin, inplace=True), want) and torch.equal(twin, want)
+
+
+# wide bf16 heads over 256 rows and more: key tiles of 64 through two and three buffers, 4 to 8 of them per block (a
+# buffer is written again from the fourth on), alone and in splits, rows of grouped heads and rows past q_len
+WIDE = [  # B, Nq, Nk, H, Hk, D, padding, layout
+    (4, 130, 461, 128, 64, 72, "", "tokens"),           # one split, 8 tiles
+    (4, 260, 449, 32, 32, 96, "mask len q", "heads"),
+    (2, 520, 401, 64, 32, 128, "mask", "tokens"),
+    (1, 100, 1500, 4, 1, 128, "", "heads"),             # 6 splits of 4 tiles
+    (1, 65, 1777, 8, 1, 80, "mask bool q", "tokens"),
+    (2, 150, 3000, 16, 8, 96, "mask len", "tokens"),    # 8 splits of 6 tiles
+]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "-".join(str(x) for x in c))
+def test_cross_attention_wide_heads(case):
+    test_cross_attention_forward_backward(case, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [72, 128])
+def test_cross_attention_wide_heads_ragged_splits(D):
+    """Lengths of 0, 1, one tile and all keys where every sequence's keys are shared out over splits."""
+    B, Nq, Nk, Hk, G, dt = 4, 75, 2100, 1, 4, torch.bfloat16
+    q, k, v, do, *_ = _attn_inputs(B, Nq, Nk, Hk * G, Hk, D, dt, "", 21)
+    ln = torch.tensor([Nk, 0, 1, 64], dtype=torch.int32)
+    keep = torch.arange(Nk)[None] < ln[:, None]
+    k[~keep], v[~keep] = float("nan"), float("inf")
+    want, tol = _attn_oracle(q, k, v, do, keep, torch.ones(B, Nq, dtype=torch.bool), D ** -0.5, dt)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = X().cross_attention(*leaves, kv_len=ln.cuda())
+    for n, got, w, t in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, do.cuda())), want, tol):
+        _near(got, w, t, n)
+
+
+@pytest.mark.parametrize("B,H,Nk", [(1, 1, 2000), (64, 2, 461)])
+def test_cross_attention_wide_heads_maximum_raised_late(B, H, Nk):
+    """Scores that rise over the tiles for one row and fall for its neighbour, by 8 and more in log2 per tile or less."""
+    Nq, D, dt = 300, 128, torch.bfloat16
+    q, k = torch.zeros(B, Nq, H, D), torch.zeros(B, Nk, H, D)
+    r = torch.arange(Nq)
+    q[..., 0] = (torch.where(r % 2 == 0, 1.0, -1.0) * 2.0 ** -(r % 5).float())[None, :, None]
+    k[..., 0] = torch.linspace(-256, 256, Nk).round()[None, :, None]  # (whole numbers, exact in bf16)
+    v = torch.randn(B, Nk, H, D, generator=_gen(6))
+    args = [t.to(dt) for t in (q, k, v)]
+    want, tol = _attn_oracle(*args, args[0], torch.ones(B, Nk, dtype=torch.bool), torch.ones(B, Nq, dtype=torch.bool), 1.0, dt)
+    # exponents up to 512 * log2 e < 2^10: the argument of exp2 is rounded by 2^-14, in the sum and in its normaliser
+    _near(X().cross_attention(*(t.cuda() for t in args), scale=1.0), want[0], tol[0] + 2.0 ** -13 * v.abs().max().item(), "o")
