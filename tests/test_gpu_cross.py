@@ -1041,3 +1041,16 @@ def test_cross_attention_wide_heads_maximum_raised_late(B, H, Nk):
     want, tol = _attn_oracle(*args, args[0], torch.ones(B, Nk, dtype=torch.bool), torch.ones(B, Nq, dtype=torch.bool), 1.0, dt)
     # exponents up to 512 * log2 e < 2^10: the argument of exp2 is rounded by 2^-14, in the sum and in its normaliser
     _near(X().cross_attention(*(t.cuda() for t in args), scale=1.0), want[0], tol[0] + 2.0 ** -13 * v.abs().max().item(), "o")
+
+
+def test_cross_attention_gradients_that_arrive_expanded_or_in_another_order():
+    """An expanded gradient (of a sum) and one whose head dim is not contiguous: the bits of their contiguous copies."""
+    for B, Nq, Nk, H, Hk, D in ((3, 37, 50, 2, 1, 24), (2, 5, 70, 2, 2, 64)):
+        q, k, v, do, *_ = _attn_inputs(B, Nq, Nk, H, Hk, D, torch.float32, "", 3)
+        leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+        grads = lambda up: torch.autograd.grad(X().cross_attention(*leaves), leaves, up)  # noqa: E731
+        one = torch.ones(1, device="cuda")
+        flipped = do.permute(3, 2, 1, 0).contiguous().permute(3, 2, 1, 0).cuda()
+        assert flipped.stride(-1) != 1 and one.expand(B, Nq, H, D).stride(-1) == 0
+        for up in (one.expand(B, Nq, H, D), flipped, flipped[:1].expand(B, -1, -1, -1)):
+            assert all(torch.equal(a, b) and (a != 0).any() for a, b in zip(grads(up), grads(up.contiguous())))
