@@ -1054,3 +1054,28 @@ def test_cross_attention_gradients_that_arrive_expanded_or_in_another_order():
         assert flipped.stride(-1) != 1 and one.expand(B, Nq, H, D).stride(-1) == 0
         for up in (one.expand(B, Nq, H, D), flipped, flipped[:1].expand(B, -1, -1, -1)):
             assert all(torch.equal(a, b) and (a != 0).any() for a, b in zip(grads(up), grads(up.contiguous())))
+
+
+# the norms' other widths per thread and team: one, four and eight columns, odd numbers of rows (two share a wide block)
+GRN_WIDTHS = [  # G, rows, C, post, pre, gate/mod/affine, type of h
+    (1, 3, 257, "rms", "layer", "gate mod affine", "same"),
+    (1, 5, 1001, "layer", "rms", "gate mod affine", "f32"),
+    (3, 1, 1537, "layer", "layer", "gate mod affine", "f32"),
+    (1, 7, 1999, "rms", "rms", "gate mod", "same"),
+    (3, 3, 400, "rms", "layer", "gate mod affine", "same"),
+    (1, 5, 600, "layer", "layer", "gate mod affine", "same"),
+    (1, 3, 700, "layer", "rms", "gate mod affine", "f32"),
+    (3, 1, 1200, "rms", "rms", "gate mod affine", "same"),
+    (1, 7, 1800, "layer", "layer", "gate mod affine", "same"),
+    (1, 7, 2000, "layer", "layer", "gate mod affine", "f32"),
+    (1, 5, 2500, "rms", "layer", "gate mod affine", "same"),
+    (3, 5, 5000, "rms", "layer", "gate mod affine", "same"),
+    (1, 5, 6000, "layer", "rms", "gate affine", "f32"),
+    (1, 3, 7000, "none", "layer", "gate mod affine", "same"),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", GRN_WIDTHS, ids=lambda c: "-".join(str(x) for x in c))
+def test_gate_residual_norm_widths(case, dt):
+    test_gate_residual_norm_forward_backward(case, dt)
