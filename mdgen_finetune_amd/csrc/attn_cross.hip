@@ -297,7 +297,6 @@ struct KvStage {
   unsigned ko[ASYNC ? P : 1], vo[ASYNC ? P : 1];  // byte offsets of this thread's pieces in a tile
   bool keep[P];  // ASYNC: of the tile to begin next; else of the begun one
   float kb;
-  bool seen = false;           // (uniform in its wave) a key was there in the tiles finished so far
   const CT *kp, *vp;           // the tile's first row
   uint64_t ka, va;             // ASYNC: its address, and the strides from tile to tile, in bytes
   int64_t kstep, vstep;
@@ -382,15 +381,12 @@ struct KvStage {
     if (tid < 64) {
       if (tid < ROWS) kbs[tid] = kb;
       const bool any = __any(kb != 0.f);
-      seen = seen || !any || __any(tid < ROWS && kb == 0.f);
       if (tid == 0) *flag = any;
     }
   }
-  // keys: set where a key was there in the tiles so far (the block's threads read it after the last tile)
-  __device__ __forceinline__ void finish(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int* keys, int tid) {
+  __device__ __forceinline__ void finish(const CrossP& p, CT* Ks, CT* Vs, float* kbs, int* flag, int tid) {
     finish_rows(p, Ks, Vs, tid);
     finish_kb(kbs, flag, tid);
-    if (tid == 0) *keys = seen;
     if constexpr (ASYNC) async_wait();
   }
 };
@@ -486,10 +482,27 @@ __device__ __forceinline__ long long part_row(const CrossP& p, int sp, int b, in
   return ((long long)sp * p.B * p.Hk + (long long)b * p.Hk + hk) * rows + r;
 }
 
-// a lane's row of outputs, O^T rows 32 dt + 8a + 4h + i: normalised, or a split's partial.  keys: whether any key was
-// there; without one the sums are 0 whatever the query holds (-inf + 0 q is NaN for an infinite q).
+// Where a mask leaves no key the sums are 0, but -inf + 0 q is NaN for a query that is not finite.  So a wave that
+// ends with a NaN looks over the mask of its keys [k0, k1); others pay nothing (a flag kept in the loop cost 2 % at D = 24).
+__device__ __forceinline__ bool no_key(const CrossP& p, int b, int k0, int k1, bool nan, int lane) {
+  if (!p.mask || !__any(nan)) return false;
+  for (int key = k0; key < k1; key += 64)
+    if (__any(key + lane < k1 && key_kept(p, b, key + lane))) return false;
+  return true;
+}
+template <int DT>
+__device__ __forceinline__ bool has_nan(const f32x16 (&x)[DT]) {
+  bool r = false;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r |= x[t][i] != x[t][i];
+  return r;
+}
+
+// a lane's row of outputs, O^T rows 32 dt + 8a + 4h + i: normalised, or a split's partial
 template <typename CT, int DP, bool VEC>
-__device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, int r, int rows, bool live, bool keys,
+__device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, int r, int rows, bool live,
                                            const f32x16* o, float m, float l, int lane) {
   constexpr int DT = DP / 32;
   const int h = lane >> 5;
@@ -497,20 +510,20 @@ __device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, i
   if (p.nsplit > 1) {
     const long long pr = part_row(p, id.split, id.b, id.hk, r);
     if (h == 0) {
-      p.part_ml[2 * pr] = keys ? m : kNoMax;
-      p.part_ml[2 * pr + 1] = keys ? l : 0.f;
+      p.part_ml[2 * pr] = m;
+      p.part_ml[2 * pr + 1] = l;
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int a = 0; a < 4; ++a)
         *reinterpret_cast<float4*>(p.part + pr * DP + 32 * dt + 8 * a + 4 * h) =
-            keys ? make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]) : make_float4(0, 0, 0, 0);
+            make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
     return;
   }
   const PackedRow pk = packed(p, r);
   const int n = pk.n, head = id.hk * p.G + pk.g;
-  const bool some = live && keys && l != 0.f;  // (a NaN among the keys that are there stays one)
+  const bool some = live && l != 0.f;  // (a NaN among the keys that are there stays one)
   const float inv = some ? 1.0f / l : 0.f;
   if (p.lse && h == 0) p.lse[((long long)id.b * p.H + head) * p.Nq + n] = some ? m * p.c + log2f(l) : -INFINITY;
   CT* orow = wrow<CT>(p.o, id.b, n, head);
@@ -575,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
   if (nt > 0) {
     st.init(p, id.b, id.hk, k0, k1, KT, tid);
     st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
-    st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
+    st.finish(p, Ks, Vs, kbs, flag, tid);
   }
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
@@ -598,11 +611,17 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
             o[dt] = mma<CT>(col_frag<CT, DP>(Vc, 32 * kt + 16 * s2, 32 * dt, lane), pf, o[dt]);
         }
     }
-    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), flag + 2, tid);
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
     __syncthreads();
   }
 
-  store_rows<CT, DP, VEC>(p, id, r, rows, live, nt > 0 && flag[2], o, m, other_half_sum(l), lane);
+  l = other_half_sum(l);
+  if (no_key(p, id.b, k0, k1, l != l, lane)) {
+    m = kNoMax, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = zero16();
+  }
+  store_rows<CT, DP, VEC>(p, id, r, rows, live, o, m, l, lane);
 }
 
 // The same with two groups of four waves (256 rows per block), one phase apart, each SIMD holding one wave
@@ -651,7 +670,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
   if (nt > 0 && !second) {
     st.init(p, id.b, id.hk, k0, k1, KT, tid);
     st.begin(p, Ks, Vs, id.b, k0, k1, KT, tid);
-    st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
+    st.finish(p, Ks, Vs, kbs, flag, tid);
   }
   __syncthreads();
   if (second) __syncthreads();
@@ -677,12 +696,18 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) pf[kt][0] = half_frag<CT>(s[kt], 0), pf[kt][1] = half_frag<CT>(s[kt], 1);
     }
-    if (loads) st.finish(p, Ks, Vs, kbs + ((t + 1) & 1) * KT, flag + ((t + 1) & 1), flag + 2, tid);
+    if (loads) st.finish(p, Ks, Vs, kbs + ((t + 1) & 1) * KT, flag + ((t + 1) & 1), tid);
     vnext = vnext == 2 ? 0 : vnext + 1;
     __syncthreads();
   }
   if (!second) __syncthreads();
-  store_rows<CT, DP, true>(p, id, r, rows, live, nt > 0 && flag[2], o, m, other_half_sum(l), lane);
+  l = other_half_sum(l);
+  if (no_key(p, id.b, k0, k1, l != l, lane)) {
+    m = kNoMax, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = zero16();
+  }
+  store_rows<CT, DP, true>(p, id, r, rows, live, o, m, l, lane);
 }
 
 // At most 32 rows per (b, key head), the single-token form: the 4 waves split the keys instead of
@@ -761,7 +786,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     if constexpr (BUFS == 2) cur ^= 1;
   }
   l = other_half_sum(l);
-  if (!st.seen) {  // no key was there for this wave: nothing, whatever the queries hold
+  if (no_key(p, id.b, k0, k1, l != l, lane)) {
     m = kNoMax, l = 0.f;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = zero16();
@@ -976,7 +1001,7 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  if (nt > 0) st.finish(p, Ks, Vs, kbs, flag, flag + 2, tid);
+  if (nt > 0) st.finish(p, Ks, Vs, kbs, flag, tid);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const int cur = t & 1;
@@ -1004,11 +1029,12 @@ __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_
           acc[dt] = mma<CT>(col_frag<CT, DP>(Kc, 32 * kt + 16 * s2, 32 * dt, lane), df, acc[dt]);
       }
     }
-    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), flag + 2, tid);
+    if (t + 1 < nt) st.finish(p, Ks + other, Vs + other, kbs + (cur ^ 1) * KT, flag + (cur ^ 1), tid);
     __syncthreads();
   }
+  const bool none = no_key(p, id.b, k0, k1, has_nan(acc), lane);
   if (r >= rows) return;
-  if (!(live && nt > 0 && flag[2])) {  // past q_len, or no key was there: 0, whatever keys, query and its gradient hold
+  if (!live || none) {  // 0, whatever keys, query and its gradient hold
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = zero16();
   }
@@ -1349,7 +1375,7 @@ __global__ __launch_bounds__(256) void cross_few_bwd_kernel(const CrossP p) {
         }
       }
 
-  if (!st.seen) {  // no key was there for this wave
+  if (no_key(p, id.b, k0, k1, has_nan(acc), lane)) {
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = zero16();
   }
