@@ -165,3 +165,15 @@ def test_adam_table_image_without_gpu():
     tab[1].n, tab[2].step = 5, None
     assert lib.mdg_adam_table_build(len(sizes), tab, buf, nbytes) != 0
     assert b"null" in lib.mdg_last_error_string()
+
+
+def test_build_compiles_what_is_up_to_date(monkeypatch):
+    """build() is the check that the sources compile: it does so where a library is there already."""
+    import subprocess
+
+    import __graft_entry__ as g
+
+    calls = []
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd, **kw: calls.append(cmd))
+    g.build()
+    assert len(calls) == 1 and calls[0][0] == "make" and "-B" in calls[0]
