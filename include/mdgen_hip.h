@@ -673,8 +673,8 @@ enum { MDG_MASK_NONE = 0, MDG_MASK_U8 = 1, MDG_MASK_F32 = 2 };
    H % Hk == 0 (query head h reads key head h / (H / Hk)), 1 <= D <= 128, dtype MDG_F32 or MDG_BF16.
    Key j of sequence b is there when j < kv_len[b] (null: Nk; values are clamped to 0..Nk) and
    mask[b * mask_sb + j * mask_sn] != 0 (MDG_MASK_U8 bytes or MDG_MASK_F32, null: all); what k / v
-   hold elsewhere, NaN included, is without effect.  A row without keys gives 0; query rows at or past
-   q_len[b] give 0 and their dout is not read.  scale: 1e-18 .. 1e18.
+   hold elsewhere, NaN included, is without effect.  A row without keys gives 0, in o and dq, whatever its q
+   and dout hold; query rows at or past q_len[b] give 0 and their dout is not read.  scale: 1e-18 .. 1e18.
    lse [B][H][Nq] fp32 (log2 of the row's normaliser in scaled log2 units, -inf without keys) and o_lo
    (o's rounding residual, as o; bf16) are what the backward reads: null in inference.
    Backward: dout as o; dq as q, dk / dv as k / v (gradients of keys that are not there are 0);

@@ -127,6 +127,7 @@ def gate_residual_norm(h, y=None, gate=None, shift=None, scale=None, resid_scale
 
     h [..., C] fp32 or y's type; y [..., C] fp32 or bf16 (None: only the norm before a block; xn then has
     h's type); post / pre "none", "rms" or "layer" (pre "none": xn is None).  gate / shift / scale fp32
-    [G, C], one row per run of rows (the rows' count is a multiple of G); weights fp32 [C].  C <= 8192.
+    [G, C], one row per run of rows (the rows' count is a multiple of G; the backward slows down for runs shorter than
+    32 rows); weights fp32 [C].  C <= 8192.
     Statistics and sums are fp32; xn is formed from h_out before its rounding."""
     return (_C or _ext()).gate_residual_norm(h, y, gate, shift, scale, resid_scale, post, pre, post_w, post_b, pre_w, pre_b, eps)

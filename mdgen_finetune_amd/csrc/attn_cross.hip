@@ -548,8 +548,9 @@ __device__ __forceinline__ void store_rows(const CrossP& p, const BlockId& id, i
 // tile; a tile's loads run under the products of the one before.  The running maximum and sum make it one
 // pass; no score is stored.
 // Narrow heads are bound by the vector unit (per 32 x 32 tile about 320 cycles of max, fma, exp, add and
-// convert against 128 of MFMA at D <= 32): [8, 4000, 16, 24] on 256 keys takes 48 us, of which 27 grow with the
-// keys and 10 are its 51 MB.  D = 64, [4, 4096, 16] on 2048 ragged keys: 152-166 us, 650 TFLOP/s.
+// convert against 128 of MFMA at D <= 32): [8, 4000, 16, 24] on 256 keys takes 48 us alone, 42 in a row of passes whose
+// ends overlap; 27 of them grow with the keys and 10 are its 51 MB.  D = 64, [4, 4096, 16] on 2048 ragged keys (110
+// GFLOP): 139-144 us, 770 TFLOP/s.
 // Tried: two row groups per wave (the registers cost a wave per SIMD: 700 against 610 us at D = 128), 32-key
 // tiles (697), all keys in LDS with waves walking the rows (46 -> 42 us masked, equal unmasked, and
 // 37 -> 47 at D = 64 with 64 keys), row sums by a product with ones (1-2 % slower).
@@ -631,8 +632,8 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
 //   M(t): O += V(t-1)^T P(t-1), S = K(t) Q^T;   V(t): P(t) = softmax of S
 // Group 0 loads: K(t+1) and V(t+1) start at its M(t) and are awaited at the end of its V(t); K lies in two
 // buffers, V, read a phase later, in three.
-// [2, 4096, 16, 128] on 4 heads of 8192 keys: 530 us, 1040 TFLOP/s (592 with the kernel above; a large library
-// product reaches 1130).  For D <= 64 it is no faster (654 against 654 us of training at D = 64, 51 against 52
+// [2, 4096, 16, 128] on 4 heads of 8192 keys: 511-528 us, 1040-1075 TFLOP/s (592 us with the kernel above; a large
+// library product reaches 1130-1165).  For D <= 64 it is no faster (654 against 654 us of training at D = 64, 51 against 52
 // at D = 24): fewer MFMA per score leave too little to run under the other phase.
 template <int DP, int KT>
 __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, int tiles) {
@@ -945,7 +946,7 @@ __device__ __forceinline__ void grad_scores(f32x16& s, f32x16& g, const float* l
 // fragments in registers and left for the dk / dv pass.  Scores are formed anew from q, k and lse where a
 // stored P would be Nq x Nk of traffic.  dq and dk / dv are two kernels, each the sole writer of its
 // sums, so results repeat bit for bit (one kernel would have to add dq by atomics).
-// D = 64, [4, 4096, 16] on 2048 ragged keys: 202-219 us, 735 TFLOP/s; MFMA and vector unit 45 and 60 % busy.
+// D = 64, [4, 4096, 16] on 2048 ragged keys (165 GFLOP): 186-192 us, 860 TFLOP/s; MFMA and vector unit 45 and 60 % busy.
 template <typename CT, int DP, int KT, bool VEC>
 __global__ __launch_bounds__(256, sizeof(CT) * DP >= 512 ? 1 : 2) void cross_dq_kernel(const CrossP p, int tiles) {
   constexpr int TILE = KT * DP, DT = DP / 32, KS = DP / 16, NT = KT / 32;
@@ -1120,7 +1121,7 @@ struct RowStage {
 // dk, dv: one key per lane; a block owns 4 x 32 keys of one (b, key head) and walks the rows in tiles
 // of QT (q and do through LDS, double buffered); splits share the rows, their fp32 partials summed in
 // order by cross_sum_kernel.
-// D = 64, [4, 4096, 16] on 2048 ragged keys: 340-370 us, 580 TFLOP/s: four accumulator tiles, the key
+// D = 64, [4, 4096, 16] on 2048 ragged keys (221 GFLOP): 288-290 us, 760 TFLOP/s: four accumulator tiles, the key
 // fragments and two tiles of scores take 204 registers, two waves per SIMD.  Held to 168 registers (three
 // waves) it takes 5 % longer, with an interleave of MFMA and vector instructions forced on the scheduler 1-2 %,
 // with more splits 5-8 %, also where the blocks past a sequence's end are dealt out evenly over the CUs.
@@ -1217,9 +1218,9 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const CrossP p, int tile
 //   S^T, dP^T (one query per lane) -> dS^T -> dq^T += K^T dS^T,    summed over tiles, waves and splits;
 //   S, dP (one key per lane) -> P, dS -> dv^T = dO^T P, dk^T = Q^T dS,   complete here: all rows are in the tile.
 // The same two fragments in either order give the two score tiles, and k and v are read once: bound by memory.
-// 8 sequences of one token, 16 heads of 128 on 8192 bf16 keys (k and v read, dk and dv written, 1.07 GB): 230 us,
-// 4.6 TB/s, against 102 + 460 us of the two kernels above; 4 of 7 tokens, 32 heads of 64 on 8 of 4000 keys 21 against
-// 13.6 + 24.2; fp32, 4 of 20 tokens, 8 heads of 64 on 3000 keys 57 against 47 + 33 (its products).  dk and dv leave
+// 8 sequences of one token, 16 heads of 128 on 8192 bf16 keys (k and v read, dk and dv written, 1.07 GB): 228 us,
+// 4.7 TB/s, against 102 + 460 us of the two kernels above; 4 of 7 tokens, 32 heads of 64 on 8 of 4000 keys 21 against
+// 13.6 + 24.2; fp32, 4 of 20 tokens, 8 heads of 64 on 3000 keys 56 against 47 + 33 (its products).  dk and dv leave
 // through LDS, 16 bytes per lane.  fp32 wider than 64 columns would spill (160 us against 78 + 64): not built.
 template <typename CT, int DP>
 constexpr bool few_bwd() { return sizeof(CT) * DP <= 256; }

@@ -10,11 +10,16 @@
 //   S1 = sum dxn, S2 = sum dxn n2, S3 = sum g, S4 = sum g n1
 //   dshift = S1, dscale = w2 S2 + b2 S1, dgate = w1 S4 + b1 S3   (per group)
 //   dw2 = sum_g (1 + scale) S2, db2 = sum_g (1 + scale) S1, dw1 = sum_g gate S4, db1 = sum_g gate S3
-// Bound by memory: forward 30 us at [32000, 384] (fp32 residual, bf16 branch: 147 MB, 4.9 TB/s of a copy's 5.1),
-// 132 us at [16383, 4096] in bf16 (537 MB, 4.1 TB/s); backward 57-64 us at [32000, 384] (221 MB, 3.7 TB/s; 162
-// registers, three waves per SIMD), its column sums 5 + 4 us, and 92 us in all at [8000, 2048] (295 MB).
+// Bound by memory: forward 37-38 us at [32000, 384] (fp32 residual, bf16 branch: 147 MB, 3.9 TB/s of a copy's 5.1; 27-30
+// where the rows are still in cache), 131 us at [16383, 4096] in bf16 (537 MB, 4.1 TB/s); backward 59-60 us at
+// [32000, 384] (221 MB, 3.7 TB/s; 160 registers, three waves per SIMD), its column sums 5 + 5 us, and 92 us in all
+// at [8000, 2048] (295 MB).
+// The backward takes one block per group at least, so short groups are slow: forward and backward of 32000 rows of
+// 384 take 96 us in groups of 4000, 195 of 32, 916 of 4 and 4606 of one row (all but one of a block's teams idle, 32
+// bytes of partials per element).
 // A row lives in the registers of TPR threads (32 or 64 lanes of a wave, or the whole block of 256, or of
-// 1024 for long rows of odd length), NV vectors of V elements each, so it is read once; statistics are
+// 1024 for long rows of odd length; in the backward also 512 and 1024 for wide ones), NV vectors of V elements each,
+// so it is read once; statistics are
 // fp32, the variance from the centred row.  xn is formed from h' before h' is rounded, and the backward recomputes h' from h
 // and y instead of reading the rounded one.  Column sums: registers over the block's rows, then LDS
 // over its teams, fp32 partials per block, summed in a fixed order: results repeat bit for bit.

@@ -5,7 +5,7 @@
 // sin per pair into LDS, once for all heads (the angle is formed in double as a number of turns and
 // reduced there: a position of 10^6 in fp32 would lose it), then a sweep over the tokens' rows in
 // memory order.  q and k go in one launch: their heads are one list.
-// fp32 [2, 50001] tokens of 16 heads x 64 columns (820 MB): 203 us, 4.0 TB/s; one token 3 us.  A large copy
+// fp32 [2, 50001] tokens of 16 heads x 64 columns (820 MB): 201-204 us, 4.0 TB/s; one token 3 us.  A large copy
 // reaches 5.1 TB/s.  Tried: token bases in LDS (57 -> 69 us for both directions: a dependent read before every
 // load), the division by N as a multiplication, half and a quarter of the LDS entries (the same),
 // non-temporal accesses and heads unrolled per thread (slower).
