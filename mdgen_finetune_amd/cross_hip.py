@@ -100,7 +100,7 @@ class RopeAxes:
 
     def __setattr__(self, name, value):
         # (the extension's handle holds the tables, and the kernels trust their columns)
-        if name in self.__dict__ and name != "_plan":
+        if name in self.__dict__ and name in ("sections", "pairs", "npairs", "turns", "axis", "cols"):
             raise AttributeError(f"RopeAxes: {name} of a plan is fixed, make another plan")
         super().__setattr__(name, value)
 

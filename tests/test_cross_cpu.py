@@ -274,5 +274,7 @@ def test_rope_plan_is_fixed():
             setattr(plan, n, getattr(plan, n))
     with pytest.raises(TypeError):
         plan.sections[0] = 3
+    plan.note = 1
+    plan.note = 2  # (what a user adds is the user's)
     twin = copy.deepcopy(plan)
     assert torch.equal(twin.turns, plan.turns) and twin.sections == plan.sections == (2, 2)
