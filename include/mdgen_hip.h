@@ -674,7 +674,8 @@ enum { MDG_MASK_NONE = 0, MDG_MASK_U8 = 1, MDG_MASK_F32 = 2 };
    Key j of sequence b is there when j < kv_len[b] (null: Nk; values are clamped to 0..Nk) and
    mask[b * mask_sb + j * mask_sn] != 0 (MDG_MASK_U8 bytes or MDG_MASK_F32, null: all); what k / v
    hold elsewhere, NaN included, is without effect.  A row without keys gives 0, in o and dq, whatever its q
-   and dout hold; query rows at or past q_len[b] give 0 and their dout is not read.  scale: 1e-18 .. 1e18.
+   and dout hold; query rows at or past q_len[b] give 0 and their dout is not read.  scale: 1e-18 .. 1e18;
+   a row whose largest score leaves fp32 when scaled is NaN.
    lse [B][H][Nq] fp32 (log2 of the row's normaliser in scaled log2 units, -inf without keys) and o_lo
    (o's rounding residual, as o; bf16) are what the backward reads: null in inference.
    Backward: dout as o; dq as q, dk / dv as k / v (gradients of keys that are not there are 0);

@@ -490,6 +490,8 @@ __device__ __forceinline__ bool no_key(const CrossP& p, int b, int k0, int k1, b
     if (__any(key + lane < k1 && key_kept(p, b, key + lane))) return false;
   return true;
 }
+// Scores past fp32 once scaled: a maximum was seen and yet every P is exp2(-inf).  NaN, not a row without keys.
+__device__ __forceinline__ float sum_in_range(float m, float l) { return l == 0.f && m != kNoMax ? __builtin_nanf("") : l; }
 template <int DT>
 __device__ __forceinline__ bool has_nan(const f32x16 (&x)[DT]) {
   bool r = false;
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void cross_fwd_kernel(const CrossP p, int t
     __syncthreads();
   }
 
-  l = other_half_sum(l);
+  l = sum_in_range(m, other_half_sum(l));
   if (no_key(p, id.b, k0, k1, l != l, lane)) {
     m = kNoMax, l = 0.f;
 #pragma unroll
@@ -702,7 +704,7 @@ __global__ __launch_bounds__(512, 2) void cross_fwd_pp_kernel(const CrossP p, in
     __syncthreads();
   }
   if (!second) __syncthreads();
-  l = other_half_sum(l);
+  l = sum_in_range(m, other_half_sum(l));
   if (no_key(p, id.b, k0, k1, l != l, lane)) {
     m = kNoMax, l = 0.f;
 #pragma unroll
@@ -786,7 +788,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p, int tile
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if constexpr (BUFS == 2) cur ^= 1;
   }
-  l = other_half_sum(l);
+  l = sum_in_range(m, other_half_sum(l));
   if (no_key(p, id.b, k0, k1, l != l, lane)) {
     m = kNoMax, l = 0.f;
 #pragma unroll

@@ -1082,3 +1082,17 @@ GRN_WIDTHS = [  # G, rows, C, post, pre, gate/mod/affine, type of h
 @pytest.mark.parametrize("case", GRN_WIDTHS, ids=lambda c: "-".join(str(x) for x in c))
 def test_gate_residual_norm_widths(case, dt):
     test_gate_residual_norm_forward_backward(case, dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,H,D", [(1, 1, 40, 2, 16), (1, 2, 3000, 1, 128), (1, 100, 50, 2, 24), (1, 40, 1500, 1, 64), (64, 260, 70, 2, 128)])
+def test_scores_past_fp32_are_not_a_row_without_keys(B, Nq, Nk, H, D, dt):
+    """q . k = 2^74 D is finite, scaled by 2^56 it is not (2^134 and more): NaN as in a plain softmax, where 0 would hide it.
+    Rows beside them are as they were."""
+    scale = 2.0 ** 56
+    q = torch.full((B, Nq, H, D), 2.0 ** 37, dtype=dt, device="cuda")
+    q[:, 0] = 0
+    k = torch.full((B, Nk, H, D), 2.0 ** 37, dtype=dt, device="cuda")
+    v = torch.ones(B, Nk, H, D, dtype=dt, device="cuda")
+    o = X().cross_attention(q, k, v, scale=scale)
+    assert torch.isnan(o[:, 1:]).all() and (o[:, 0] == 1).all()
